@@ -265,6 +265,17 @@ def lib() -> ctypes.CDLL:
         "b200q_lowering_offset": (SZ, [P, U]),
         "b200q_lowering_act_floats": (SZ, [P]),
         "b200q_node_supported": (I, [P, U]),
+        "b200q_kv4_page_bytes": (SZ, [U, U, U]),
+        "b200q_block_map": (I, [I, U, P, P, P, U, U, P, U, P, P, P, P, P, P, U, P, P, ctypes.c_char_p, U]),
+        "b200q_kv4_store": (I, [I, P, P, P, P, U, SZ, SZ, P, P, ctypes.c_char_p, U]),
+        "b200q_kv4_load": (I, [I, P, P, U, P, P, SZ, SZ, P, P, ctypes.c_char_p, U]),
+        "b200q_kv4_attn_workspace": (SZ, [I, P, U, U, U, U, U]),
+        "b200q_kv4_attn": (I, [I, P, P, P, U, U, P, U, P, P, U, U, U, ctypes.c_float, P, SZ, SZ, SZ, SZ, U, P, P,
+                               ctypes.c_char_p, U]),
+        "b200q_beam_select_workspace": (SZ, [I, U, U, U, U]),
+        "b200q_beam_select": (I, [I, P, U, P, U, U, U, P, P, P, P, SZ, SZ, P, ctypes.c_char_p, U]),
+        "b200q_beam_reorder": (I, [I, P, P, P, U, U, SZ, U, SZ, SZ, P, P, ctypes.c_char_p, U]),
+        "b200q_kv4_reorder": (I, [I, P, P, U, P, P, U, U, P, P, ctypes.c_char_p, U]),
     }
     for name, (res, args) in sig.items():
         f = getattr(L, name)
@@ -290,7 +301,9 @@ EXPORTED = ["b200q_create", "b200q_destroy", "b200q_last_error", "b200q_stream",
             "b200q_gguf_get_float", "b200q_upload_gguf_tensor", "b200q_q4_0x8_to_q4_0", "b200q_set_feature_mask",
             "b200q_feature_mask", "b200q_set_verify", "b200q_comm_init_ex", "b200q_lower", "b200q_lowering_free",
             "b200q_lowering_lists", "b200q_lowering_list", "b200q_lowering_offset", "b200q_lowering_act_floats",
-            "b200q_node_supported"]
+            "b200q_node_supported", "b200q_kv4_page_bytes", "b200q_block_map", "b200q_kv4_store", "b200q_kv4_load",
+            "b200q_kv4_attn_workspace", "b200q_kv4_attn", "b200q_beam_select_workspace", "b200q_beam_select",
+            "b200q_beam_reorder", "b200q_kv4_reorder"]
 
 
 class _LayoutInfo(ctypes.Structure):
@@ -366,6 +379,101 @@ def quantize_noalloc(device: int, x_ptr: int, n: int, fmt: int, norm_w_ptr: int 
     if rc != 0:
         raise B200QError(rc, err.value.decode() or ERR.get(rc, str(rc)))
     return q, scales, bs
+
+
+# ---- several sequences: a paged 4-bit KV cache, block maps, beam search (device pointers, no context) -----------------
+NO_SLOT = 0xFFFFFFFF  # a slot, page, parent or token that names nothing (-1 in an int32 tensor)
+SERVE_REQUEST, SERVE_PAGE, SERVE_SLOT, SERVE_SHORT, SERVE_PARENT, SERVE_WAIT = 1, 2, 4, 8, 16, 32  # status bits
+
+
+class Kv4Pool(ctypes.Structure):
+    """b200q_kv4_pool: the pages of a 4-bit KV cache. Kv4Pool(base pointer, n_pages, page_tokens, n_kv_head, head_dim)
+    for one layer; with n_layers and layer_bytes the layers that share block tables (kv4_reorder)."""
+    _fields_ = [("base", ctypes.c_void_p), ("n_pages", ctypes.c_uint32), ("page_tokens", ctypes.c_uint32),
+                ("n_kv_head", ctypes.c_uint32), ("head_dim", ctypes.c_uint32), ("n_layers", ctypes.c_uint32),
+                ("layer_bytes", ctypes.c_uint64)]
+
+
+def kv4_page_bytes(page_tokens: int, n_kv_head: int, head_dim: int) -> int:
+    """Bytes of one page of one layer (0 for a shape the cache does not take)."""
+    return int(lib().b200q_kv4_page_bytes(page_tokens, n_kv_head, head_dim))
+
+
+def _served(fn, *args):
+    err = ctypes.create_string_buffer(256)
+    rc = fn(*args, err, 256)
+    if rc != 0:
+        raise B200QError(rc, err.value.decode() or ERR.get(rc, str(rc)))
+
+
+def block_map(device: int, n_req: int, past: int, fresh: int, table: int, table_stride: int, page_tokens: int,
+              free_pages: int, n_free: int, cursor_in: int, cursor_out: int, kv_len: int, q_start: int, slots: int,
+              positions: int, n_rows: int, status: int | None = None, stream: int | None = None) -> None:
+    """b200q_block_map: block tables, slots, positions and row starts of a step, from the requests' lengths (device
+    pointers to uint32)."""
+    _served(lib().b200q_block_map, device, n_req, past, fresh, table, table_stride, page_tokens, free_pages, n_free,
+            cursor_in, cursor_out, kv_len, q_start, slots, positions, n_rows, status, stream)
+
+
+def kv4_store(device: int, pool: Kv4Pool, k: int, v: int, slots: int, n: int, k_stride: int = 0, v_stride: int = 0,
+              status: int | None = None, stream: int | None = None) -> None:
+    """b200q_kv4_store: n tokens' K and V rows (device FP32) quantized into their slots."""
+    _served(lib().b200q_kv4_store, device, ctypes.byref(pool), k, v, slots, n, k_stride, v_stride, status, stream)
+
+
+def kv4_load(device: int, pool: Kv4Pool, slots: int, n: int, k: int, v: int, k_stride: int = 0, v_stride: int = 0,
+             status: int | None = None, stream: int | None = None) -> None:
+    """b200q_kv4_load: the values that n slots hold, as device FP32 rows."""
+    _served(lib().b200q_kv4_load, device, ctypes.byref(pool), slots, n, k, v, k_stride, v_stride, status, stream)
+
+
+def kv4_attn_workspace(device: int, pool: Kv4Pool, n_rows: int, n_head: int, n_req: int, max_q: int, max_kv: int) -> int:
+    """Bytes of workspace that kv4_attn takes for this shape."""
+    n = int(lib().b200q_kv4_attn_workspace(device, ctypes.byref(pool), n_rows, n_head, n_req, max_q, max_kv))
+    if n == 0:
+        raise B200QError(-1, "kv4_attn_workspace: a shape that kv4_attn does not take")
+    return n
+
+
+def kv4_attn(device: int, pool: Kv4Pool, q: int, y: int, n_rows: int, n_head: int, table: int, table_stride: int,
+             q_start: int, kv_len: int, n_req: int, max_q: int, max_kv: int, scale: float, workspace: int,
+             workspace_bytes: int, q_stride: int = 0, q_head_stride: int = 0, y_stride: int = 0, window: int = 0,
+             status: int | None = None, stream: int | None = None) -> None:
+    """b200q_kv4_attn: causal attention of every request's new tokens (FP32 rows) over its pages of the 4-bit cache."""
+    _served(lib().b200q_kv4_attn, device, ctypes.byref(pool), q, y, n_rows, n_head, table, table_stride, q_start, kv_len,
+            n_req, max_q, max_kv, scale, workspace, workspace_bytes, q_stride, q_head_stride, y_stride, window, status,
+            stream)
+
+
+def beam_select_workspace(device: int, n_req: int, beams: int, vocab: int, n_out: int) -> int:
+    """Bytes of workspace that beam_select takes for this shape."""
+    n = int(lib().b200q_beam_select_workspace(device, n_req, beams, vocab, n_out))
+    if n == 0:
+        raise B200QError(-1, "beam_select_workspace: a shape that beam_select does not take")
+    return n
+
+
+def beam_select(device: int, logits: int, vocab: int, scores: int, n_req: int, beams: int, n_out: int, out_scores: int,
+                out_parent: int, out_token: int, workspace: int, workspace_bytes: int, logits_stride: int = 0,
+                stream: int | None = None) -> None:
+    """b200q_beam_select: the n_out best (parent beam, token) of each request, by the beam's score + the log softmax."""
+    _served(lib().b200q_beam_select, device, logits, vocab, scores, n_req, beams, n_out, out_scores, out_parent, out_token,
+            workspace, workspace_bytes, logits_stride, stream)
+
+
+def beam_reorder(device: int, src: int, dst: int, parent: int, n_req: int, beams: int, row_bytes: int, n_layers: int = 1,
+                 src_layer_bytes: int = 0, dst_layer_bytes: int = 0, status: int | None = None,
+                 stream: int | None = None) -> None:
+    """b200q_beam_reorder: every layer's state rows moved to their beams' parents (src and dst the same, or apart)."""
+    _served(lib().b200q_beam_reorder, device, src, dst, parent, n_req, beams, row_bytes, n_layers, src_layer_bytes,
+            dst_layer_bytes, status, stream)
+
+
+def kv4_reorder(device: int, pool: Kv4Pool, table: int, table_stride: int, kv_len: int, parent: int, n_req: int, beams: int,
+                status: int | None = None, stream: int | None = None) -> None:
+    """b200q_kv4_reorder: block tables and tail pages of every layer moved to their beams' parents, in place."""
+    _served(lib().b200q_kv4_reorder, device, ctypes.byref(pool), table, table_stride, kv_len, parent, n_req, beams, status,
+            stream)
 
 
 def row_slice(rows: int, world: int, rank: int, flags: int = 0) -> tuple:

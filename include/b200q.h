@@ -354,6 +354,113 @@ B200Q_API int b200q_quantize_noalloc(int device, const float *x, unsigned n, uns
                                      float norm_eps, unsigned norm_flags, void *stream, int8_t *q, void *scales,
                                      int32_t *bsums, char *err_msg, unsigned err_len);
 
+/* ---- several sequences: a paged 4-bit KV cache, block maps, beam search ----------------------------------------
+ * No counterpart in the reference, which decodes one sequence. These calls hold no context: the caller names the device,
+ * a stream of it (a cudaStream_t; NULL: the legacy default stream) and every buffer, all of it device (or managed) memory
+ * of that device. Nothing is allocated and nothing waits: the work is enqueued on the stream, and a call can be captured
+ * into a CUDA graph. Calls on different streams may overlap when they write different buffers (their workspaces among
+ * them: two graphs that may run at the same time need one each).
+ *
+ * Arguments are checked on the host before anything is launched: a bad size, a pointer that is not device memory of the
+ * device, is misaligned or holds too little, a written buffer that overlaps another one, or a stream of another device
+ * returns B200Q_ERR_ARG with the reason in err (which may be NULL). What only the device holds (lengths, table
+ * entries, slots, parents) is checked by the kernels: what does not fit is left out, and a B200Q_SERVE_* bit is set in
+ * the status word (a device uint32 that the caller zeroes and reads when it likes; NULL: not reported).
+ *
+ * The cache holds K and V as Q4_0 blocks: 32 values as codes c with an FP16 d, a code standing for d (c - 8). A page holds
+ * page_tokens tokens (a multiple of 16) of every KV head as tiles of 16 tokens: page p, head h, tile t is the run of
+ * 18 x head_dim bytes number (p x n_kv_head + h) x (page_tokens / 16) + t of the layer. In a tile lie the K codes
+ * (8 x head_dim bytes), the V codes, the K scales and the V scales (head_dim bytes each, [token][block] FP16). A
+ * block's codes are four 4-byte words; word w holds in byte i element 4 w + i (low nibble) and 16 + 4 w + i (high nibble),
+ * the bytes of a GGUF Q4_0 block in their order. Words are cut into planes of four blocks (128 dims; the last plane: what
+ * is left), K's in a plane as [token][w][block], V's as [token / 8][token % 2][w][token / 2 % 4][block].
+ * A slot is a token's place: page x page_tokens + place in the page. */
+typedef struct b200q_kv4_pool {
+    void *base;                /* the (first) layer's pages, 16-byte aligned */
+    uint32_t n_pages, page_tokens, n_kv_head, head_dim; /* head_dim: a multiple of 32 up to 256 */
+    uint32_t n_layers;         /* read by b200q_kv4_reorder only: layers that share the block tables */
+    uint64_t layer_bytes;      /* bytes from a layer's pages to the next layer's */
+} b200q_kv4_pool;
+#define B200Q_NO_SLOT 0xFFFFFFFFu /* a slot, page, parent or token that names nothing */
+#define B200Q_SERVE_REQUEST 1u  /* a request's rows or lengths lie outside the stated bounds: its rows were left out */
+#define B200Q_SERVE_PAGE 2u     /* a table entry names no page of the pool: its tokens were left out */
+#define B200Q_SERVE_SLOT 4u     /* a slot outside the pool: its token was left out */
+#define B200Q_SERVE_SHORT 8u    /* block_map ran out of free pages or of table entries: some slots are B200Q_NO_SLOT */
+#define B200Q_SERVE_PARENT 16u  /* a parent that is no beam of its request: its row was left as it was */
+#define B200Q_SERVE_WAIT 32u    /* a kernel's bounded wait ran out: the results are not complete */
+/* Bytes of one page of one layer (0 for a shape the cache does not take). */
+B200Q_API size_t b200q_kv4_page_bytes(unsigned page_tokens, unsigned n_kv_head, unsigned head_dim);
+
+/* Block tables and slot maps of a step from the requests' lengths. Request r holds past[r] tokens and gets fresh[r] more:
+ *   kv_len[r] = past[r] + fresh[r];  q_start[r] = the sum of fresh before r, q_start[n_req] = the sum of all;
+ *   table row r (table_stride entries; those of its past tokens stay): new pages, in request order, from free_pages at
+ *   *cursor_in on, for the blocks that past tokens do not reach; *cursor_out = the first free page not taken (it may be
+ *   *cursor_in itself);
+ *   row j of the step (j < n_rows, rows in request order): positions[j] and slots[j]; rows behind the last token get
+ *   B200Q_NO_SLOT and position 0, so that a step padded to a fixed n_rows stores nothing for them.
+ * Without a free page or a table entry left, a token's slot is B200Q_NO_SLOT (and kv_len stops at the table's end). */
+B200Q_API int b200q_block_map(int device, unsigned n_req, const uint32_t *past, const uint32_t *fresh, uint32_t *table,
+                              unsigned table_stride, unsigned page_tokens, const uint32_t *free_pages, unsigned n_free,
+                              const uint32_t *cursor_in, uint32_t *cursor_out, uint32_t *kv_len, uint32_t *q_start,
+                              uint32_t *slots, uint32_t *positions, unsigned n_rows, uint32_t *status, void *stream,
+                              char *err, unsigned err_len);
+
+/* n tokens' K and V rows (n_kv_head x head_dim floats, rows k_stride / v_stride floats apart; 0: packed) quantized into
+ * their slots, bit for bit as GGUF Q4_0 quantizes (d = the value of largest magnitude over -8, the first on ties; code =
+ * min(15, trunc(x (1 / d) + 8.5))); a block that holds a NaN or an infinity reads back as NaN. Slots of one call are
+ * distinct, or B200Q_NO_SLOT (nothing is stored); of a slot named twice, either token's blocks may stay. */
+B200Q_API int b200q_kv4_store(int device, const b200q_kv4_pool *pool, const float *k, const float *v, const uint32_t *slots,
+                              unsigned n, size_t k_stride, size_t v_stride, uint32_t *status, void *stream, char *err,
+                              unsigned err_len);
+/* The values that n slots hold, as FP32 rows (a row whose slot names no token is left as it was). */
+B200Q_API int b200q_kv4_load(int device, const b200q_kv4_pool *pool, const uint32_t *slots, unsigned n, float *k, float *v,
+                             size_t k_stride, size_t v_stride, uint32_t *status, void *stream, char *err,
+                             unsigned err_len);
+
+/* Attention of every request's new tokens over its pages. Rows q_start[r] .. q_start[r + 1] of q and y (n_rows rows in the
+ * buffers; rows outside every request are left as they were) are the last of request r's kv_len[r] tokens: row i stands at
+ * p = kv_len[r] - (q_start[r + 1] - q_start[r]) + i and sees the keys (p - window, p] (window 0: [0, p]); a row that sees
+ * none is zero. Query head h (of n_head, a multiple of n_kv_head) reads KV head h / (n_head / n_kv_head):
+ *   y = softmax(scale q K^T) V, with FP32 inputs, sums and outputs.
+ * q: rows q_stride and heads q_head_stride floats apart; y: rows y_stride apart, heads packed (0: packed). max_q and
+ * max_kv bound the requests' new tokens and kv_len, and shape the launch; a request beyond them is left out and
+ * reported. workspace: b200q_kv4_attn_workspace bytes for the same shape, 16-byte aligned; nothing in it has to be kept or cleared
+ * between calls. */
+B200Q_API size_t b200q_kv4_attn_workspace(int device, const b200q_kv4_pool *pool, unsigned n_rows, unsigned n_head,
+                                          unsigned n_req, unsigned max_q, unsigned max_kv);
+B200Q_API int b200q_kv4_attn(int device, const b200q_kv4_pool *pool, const float *q, float *y, unsigned n_rows,
+                             unsigned n_head, const uint32_t *table, unsigned table_stride, const uint32_t *q_start,
+                             const uint32_t *kv_len, unsigned n_req, unsigned max_q, unsigned max_kv, float scale,
+                             void *workspace, size_t workspace_bytes, size_t q_stride, size_t q_head_stride,
+                             size_t y_stride, unsigned window, uint32_t *status, void *stream, char *err,
+                             unsigned err_len);
+
+/* The n_out best continuations of each request over its beams and the vocabulary: of all
+ *   scores[b] + logits[b][t] - log sum_u e^logits[b][u]
+ * (row r x beams + b of logits, logits_stride floats apart; 0: vocab) the largest, in order, ties to the lower beam, then
+ * the lower token: out_scores, out_parent (the beam in its request) and out_token, n_out a request. A logit of -inf or NaN
+ * is no candidate and adds nothing to the sum; a beam whose score is not finite, or whose logits hold +inf or nothing
+ * finite, has none. Places without a candidate get -inf, B200Q_NO_SLOT, B200Q_NO_SLOT. Candidates are compared in 64 bits.
+ * beams <= 32, n_out <= 64, vocab <= 2^20. */
+B200Q_API size_t b200q_beam_select_workspace(int device, unsigned n_req, unsigned beams, unsigned vocab, unsigned n_out);
+B200Q_API int b200q_beam_select(int device, const float *logits, unsigned vocab, const float *scores, unsigned n_req,
+                                unsigned beams, unsigned n_out, float *out_scores, uint32_t *out_parent,
+                                uint32_t *out_token, void *workspace, size_t workspace_bytes, size_t logits_stride,
+                                void *stream, char *err, unsigned err_len);
+/* State rows moved to their beams' parents: in every layer, row r x beams + b of dst = row r x beams + parent[r x beams + b]
+ * of src (row_bytes a row, layers src_layer_bytes / dst_layer_bytes apart; 0: packed). src and dst are the same buffer or apart.
+ * A parent of B200Q_NO_SLOT leaves its row as it was. */
+B200Q_API int b200q_beam_reorder(int device, const void *src, void *dst, const uint32_t *parent, unsigned n_req,
+                                 unsigned beams, size_t row_bytes, unsigned n_layers, size_t src_layer_bytes,
+                                 size_t dst_layer_bytes, uint32_t *status, void *stream, char *err, unsigned err_len);
+/* The same for the paged cache, in place: beams of a request (rows r x beams + b of the table) hold kv_len[r x beams]
+ * tokens each. Their full pages are shared: table entries [0, kv_len / page_tokens) come from the parent's row. The page
+ * behind them is a beam's own: it keeps its table entry and receives the tokens of the parent's, in every layer of the
+ * pool. The beams' own pages are distinct. */
+B200Q_API int b200q_kv4_reorder(int device, const b200q_kv4_pool *pool, uint32_t *table, unsigned table_stride,
+                                const uint32_t *kv_len, const uint32_t *parent, unsigned n_req, unsigned beams,
+                                uint32_t *status, void *stream, char *err, unsigned err_len);
+
 /* ---- GGUF files and the CPU backend's Q4_0x8 layout (host only) ------------------------------------------------
  * For callers that load weights without llama.cpp. The reference backend receives its weights from llama.cpp's GGUF
  * loader as ggml tensors (ggml-xrt.cpp:642-653 keys them by tensor, data pointer, type, shape and bytes) and reads

@@ -1,0 +1,644 @@
+"""The operators that serve several sequences, on the GPU, against the restatements of serve_ref (64 bits): every size and
+mask where they can go wrong, what lies beside their results left as it was, status bits, refusals, streams, captured
+graphs, and a beam search that runs them together."""
+import math
+
+import numpy as np
+import pytest
+
+import serve_ref as ref
+from conftest import rng
+
+torch = pytest.importorskip("torch")
+SKIP = ref.NO_SLOT
+pytestmark = [pytest.mark.gpu, pytest.mark.filterwarnings("ignore::RuntimeWarning")]  # NaN and infinite scales on purpose
+
+
+def dev(x):
+    x = np.asarray(x)
+    if x.dtype.kind in "iu" and x.dtype != np.uint8:
+        x = x.astype(np.int64).astype(np.uint32).view(np.int32)
+    return torch.from_numpy(np.ascontiguousarray(x)).cuda()
+
+
+def u32(t):
+    return t.cpu().numpy().view(np.uint32)
+
+
+class Paged:
+    """A pool on both sides. `junk`: what lies in tokens nobody stored, NaN scales among it."""
+
+    def __init__(self, b2, r, n_pages, page, n_kv, dim, junk=True):
+        self.ref = ref.Pool(n_pages, page, n_kv, dim)
+        if junk:
+            self.ref.bytes[:] = r.integers(0, 256, self.ref.bytes.shape, dtype=np.uint8)
+            self.ref.bytes[..., 16 * dim + 1::2] |= 0x7E  # scales: NaN, infinite or huge
+        self.gpu = dev(self.ref.bytes)
+        self.h = b2.Kv4Pool(self.gpu.data_ptr(), n_pages, page, n_kv, dim, 1, 0)
+
+    def fill(self, slots, k, v):
+        """The host side stores, the device side takes its bytes."""
+        self.ref.store(slots, k, v)
+        self.gpu.copy_(torch.from_numpy(self.ref.bytes))
+
+
+# ---- store and load ------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dim", range(32, 257, 32))
+@pytest.mark.parametrize("page,n_kv,n", [(16, 1, 1), (48, 3, 37), (128, 2, 130)])
+def test_store_gives_the_formats_bits_and_touches_nothing_else(b2, dim, page, n_kv, n):
+    r = rng(80, dim, page)
+    p = Paged(b2, r, -(-n // page) + 2, page, n_kv, dim)
+    width, gap = n_kv * dim, int(r.integers(0, 4))
+    k, v = (r.normal(0, 3, (n, width + gap)).astype(np.float32) for _ in range(2))
+    k[0, :32], v[0, :32] = 0, -0.0
+    k[0, -1 - gap], v[n // 2, 0] = 1e30, -1e-30
+    if n > 4:
+        k[1, 0], k[2, 1], v[3, 2] = np.nan, np.inf, -np.inf
+        k[3, :32] = 2.5
+        v[4, :32] = np.tile([1.0, -1.0], 16)
+    slots = r.permutation(p.ref.n_pages * page)[:n].astype(np.int64)
+    if n > 6:
+        slots[5], slots[6] = SKIP, p.ref.n_pages * page  # no slot; a slot outside
+    status = dev(np.zeros(1, np.uint32))
+    dk, dv, ds = dev(k), dev(v), dev(slots)
+    b2.kv4_store(0, p.h, dk.data_ptr(), dv.data_ptr(), ds.data_ptr(), n, width + gap, width + gap, status.data_ptr())
+    p.ref.store(slots, k[:, :width], v[:, :width])
+    got, want = p.gpu.cpu().numpy(), p.ref.bytes
+    # a NaN scale may carry any payload: compare those as NaN
+    s = slice(16 * dim, None)
+    a, b = (np.ascontiguousarray(x[..., s]).view(np.float16) for x in (got, want))
+    assert ((a.view(np.uint16) == b.view(np.uint16)) | (np.isnan(a) & np.isnan(b))).all()
+    # codes of a block with a NaN are free
+    nan_tok = [int(x) for i, x in enumerate(slots) if n > 4 and i in (1, 2, 3) and x != SKIP]
+    diff = np.argwhere(got[..., :16 * dim] != want[..., :16 * dim])
+    for pg, _, t, _ in diff:
+        assert any(x // page == pg and x % page // 16 == t for x in nan_tok)
+    assert int(u32(status)[0]) == (b2.SERVE_SLOT if n > 6 else 0)
+    # and read back
+    back = [torch.full((n, width + 3), 7.0, device="cuda") for _ in range(2)]
+    b2.kv4_load(0, p.h, ds.data_ptr(), n, back[0].data_ptr(), back[1].data_ptr(), width + 3, width + 3, status.data_ptr())
+    for which, t in enumerate(back):
+        g = t.cpu().numpy()
+        assert (g[:, width:] == 7).all()
+        for i, x in enumerate(slots):
+            if x == SKIP or x >= p.ref.n_pages * page:
+                assert (g[i] == 7).all()
+                continue
+            w = p.ref.values(which, [x // page], [x % page])[0].reshape(-1)
+            assert np.array_equal(np.isnan(g[i, :width]), np.isnan(w))
+            ok = ~np.isnan(w)
+            assert np.array_equal(g[i, :width][ok], w.astype(np.float32)[ok])
+
+
+def test_store_reads_k_and_v_out_of_wider_rows_and_load_writes_them_back(b2):
+    r = rng(81)
+    n, n_kv, dim, page = 33, 2, 96, 32
+    p = Paged(b2, r, 4, page, n_kv, dim)
+    width = n_kv * dim
+    rows = r.normal(0, 1, (n, 5 + 2 * width + 6)).astype(np.float32)
+    d, slots = dev(rows), np.arange(7, 7 + n)
+    ds = dev(slots)
+    st = rows.shape[1]
+    b2.kv4_store(0, p.h, d.data_ptr() + 20, d.data_ptr() + 4 * (5 + width), ds.data_ptr(), n, st, st)
+    p.ref.store(slots, rows[:, 5:5 + width], rows[:, 5 + width:5 + 2 * width])
+    assert np.array_equal(p.gpu.cpu().numpy(), p.ref.bytes)
+    out = torch.zeros_like(d)
+    b2.kv4_load(0, p.h, ds.data_ptr(), n, out.data_ptr() + 20, out.data_ptr() + 4 * (5 + width), st, st)
+    g = out.cpu().numpy()
+    assert np.array_equal(g[:, 5:5 + width], p.ref.values(0, slots // page, slots % page).reshape(n, -1).astype(np.float32))
+    assert np.array_equal(g[:, 5 + width:5 + 2 * width], p.ref.values(1, slots // page, slots % page).reshape(n, -1).astype(np.float32))
+    assert (g[:, :5] == 0).all() and (g[:, -6:] == 0).all()
+    b2.kv4_store(0, p.h, 0, 0, 0, 0)  # no rows: nothing to do
+
+
+# ---- attention -----------------------------------------------------------------------------------------------------
+
+class Batch:
+    """Requests with (new, kv) lengths over a pool whose other tokens hold junk."""
+
+    def __init__(self, b2, r, lengths, n_kv, group, dim, page, k_std=1.0, q_std=1.5, stride=None):
+        self.b2, self.n_head = b2, n_kv * group
+        self.new, self.kv = [a for a, _ in lengths], [b for _, b in lengths]
+        held = [-(-n // page) for n in self.kv]
+        self.stride = stride or max(held + [1]) + 1
+        self.p = Paged(b2, r, sum(held) + 2, page, n_kv, dim)
+        pages = r.permutation(self.p.ref.n_pages)
+        self.table = r.integers(0, 1 << 31, (len(lengths), self.stride))  # entries behind a request's pages: anything
+        at = 0
+        for i, n in enumerate(held):
+            self.table[i, :n] = pages[at:at + n]
+            at += n
+        slots = np.concatenate([self.table[i][np.arange(n) // page] * page + np.arange(n) % page for i, n in enumerate(self.kv)] or [[]]).astype(np.int64)
+        self.p.fill(slots, *(r.normal(0, s, (len(slots), n_kv * dim)).astype(np.float32) for s in (k_std, 1.0)))
+        self.q_start = np.concatenate([[0], np.cumsum(self.new)])
+        self.rows = int(self.q_start[-1])
+        self.q = r.normal(0, q_std, (self.rows, self.n_head, dim)).astype(np.float32)
+        self.scale = 1.0 / math.sqrt(dim)
+
+    def run(self, window=0, pad=0, q_pad=0, head_pad=0, y_pad=0, max_q=None, max_kv=None, stream=None, q=None, table=None, q_start=None, kv_len=None):
+        b2, dim, nh = self.b2, self.p.ref.dim, self.n_head
+        n = self.rows + pad
+        q = self.q if q is None else q
+        wide = np.zeros((n, nh * (dim + head_pad) + q_pad), np.float32)
+        wide[:self.rows, :nh * (dim + head_pad)].reshape(self.rows, nh, dim + head_pad)[:, :, :dim] = q
+        self.status = dev(np.zeros(1, np.uint32))
+        y = torch.full((n, nh * dim + y_pad), 7.0, device="cuda")
+        max_q, max_kv = max_q or max(self.new + [1]), max_kv or max(self.kv + [1])
+        need = b2.kv4_attn_workspace(0, self.p.h, n, nh, len(self.kv), max_q, max_kv)
+        room = torch.full((need,), 0xFF, dtype=torch.uint8, device="cuda")  # NaN, should it be read before it is written
+        keep = [dev(wide), dev(self.table if table is None else table), dev(self.q_start if q_start is None else q_start),
+                dev(self.kv if kv_len is None else kv_len)]
+        torch.cuda.synchronize()
+        b2.kv4_attn(0, self.p.h, keep[0].data_ptr(), y.data_ptr(), n, nh, keep[1].data_ptr(), self.stride, keep[2].data_ptr(), keep[3].data_ptr(),
+                    len(self.kv), max_q, max_kv, self.scale, room.data_ptr(), need, wide.shape[1], dim + head_pad, nh * dim + y_pad, window,
+                    self.status.data_ptr(), stream)
+        torch.cuda.synchronize()
+        y = y.cpu().numpy()
+        assert (y[self.rows:] == 7).all() and (y[:, nh * dim:] == 7).all()  # rows behind the last sequence, gaps
+        return y[:self.rows, :nh * dim].reshape(self.rows, nh, dim)
+
+    def check(self, got, window=0, q=None):
+        """Against 64 bits. With S = scale max_t sum |q k_t|: a score is off by at most 2^-20 S (FP32 sums of up to 256 products,
+        q to 22 bits or more), the exponentials by 2^-21 more, weights and sums of up to some thousand terms in partial sums
+        of at most 64 by 2^-18; y by that share of sum p |v|, twice (numerator and denominator)."""
+        y, mag, big = ref.attention(self.p.ref, self.q if q is None else q, self.table, self.q_start, self.kv, self.scale, window)
+        tol = 2.0 ** -17 * (1 + big[:, :, None] / 8) * mag
+        assert np.isfinite(got).all()
+        bad = np.abs(got - y) - tol
+        assert bad.max(initial=0) <= 0, (bad.max(), np.unravel_index(bad.argmax(), bad.shape))
+        assert (got[mag.sum(-1) == 0] == 0).all()
+
+
+@pytest.mark.parametrize("dim", range(32, 257, 32))
+@pytest.mark.parametrize("n_kv,group,page", [(1, 1, 16), (2, 4, 48), (3, 8, 64)])
+def test_attention_of_single_tokens(b2, dim, n_kv, group, page):
+    r = rng(82, dim, group)
+    b = Batch(b2, r, [(1, 1), (1, 2), (1, 15), (1, 16), (1, 17), (1, 63), (1, 64), (1, 65), (1, 200), (1, 611)], n_kv, group, dim, page)
+    b.check(b.run())
+    assert u32(b.status)[0] == 0
+
+
+@pytest.mark.parametrize("group", [1, 2, 3, 5, 7, 9, 16, 20])
+def test_attention_groups_of_heads(b2, group):
+    b = Batch(b2, rng(83, group), [(1, 100), (2, 33), (3, 3)], 2, group, 64, 32)
+    b.check(b.run(pad=3, q_pad=5, head_pad=3, y_pad=2), 0)
+
+
+@pytest.mark.parametrize("window", [0, 1, 2, 15, 16, 17, 100])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_attention_of_ragged_requests_and_windows(b2, window, dim):
+    # several new tokens, none, requests without a key, rows before the first position, lengths around the pages' ends
+    b = Batch(b2, rng(84, window, dim), [(4, 130), (0, 50), (0, 0), (3, 2), (2, 0), (7, 7), (1, 16), (5, 97), (2, 129)], 2, 4, dim, 32)
+    b.check(b.run(window, pad=2), window)
+    assert u32(b.status)[0] == 0
+
+
+@pytest.mark.parametrize("dim,n_kv,group", [(32, 2, 2), (64, 1, 8), (96, 2, 3), (128, 2, 4), (256, 1, 4), (224, 1, 2)])
+@pytest.mark.parametrize("window", [0, 40])
+def test_attention_of_prompts(b2, dim, n_kv, group, window):
+    b = Batch(b2, rng(85, dim, window), [(100, 100), (17, 17), (1, 90), (33, 150), (64, 64), (129, 257), (20, 7)], n_kv, group, dim, 48)
+    b.check(b.run(window, pad=1, q_pad=1), window)
+
+
+def test_attention_with_one_key_far_above_the_others(b2):
+    # softmax that is almost one key: large scores, running maxima that jump late and early
+    for salt in range(3):
+        b = Batch(b2, rng(86, salt), [(1, 700), (1, 33), (20, 300)], 2, 4, 128, 16, k_std=6.0, q_std=6.0)
+        b.check(b.run())
+
+
+@pytest.mark.parametrize("power", [-30, -12, 12, 30])
+def test_attention_keeps_its_precision_at_other_magnitudes_of_q(b2, power):
+    b = Batch(b2, rng(87), [(1, 300), (18, 64)], 2, 4, 128, 16)
+    q = np.ldexp(b.q, power).astype(np.float32)
+    b.scale = math.ldexp(b.scale, -power)
+    b.check(b.run(q=q), q=q)
+
+
+@pytest.mark.parametrize("std", [1e-3, 30.0, 3000.0])
+def test_attention_keeps_its_precision_at_other_magnitudes_of_v(b2, std):
+    r = rng(88)
+    b = Batch(b2, r, [(1, 300), (18, 64)], 2, 4, 128, 16)
+    for i, n in enumerate(b.kv):
+        slots = b.table[i][np.arange(n) // 16] * 16 + np.arange(n) % 16
+        b.p.fill(slots, r.normal(0, 1, (n, 256)).astype(np.float32), r.normal(0, std, (n, 256)).astype(np.float32))
+    b.check(b.run())
+
+
+def test_attention_over_zero_values_and_equal_keys(b2):
+    b = Batch(b2, rng(89), [(1, 50), (2, 40)], 1, 4, 64, 16)
+    for i, n in enumerate(b.kv):
+        slots = b.table[i][np.arange(n) // 16] * 16 + np.arange(n) % 16
+        b.p.fill(slots, np.zeros((n, 64), np.float32), np.ones((n, 64), np.float32) * (i + 1))
+    got = b.run()
+    b.check(got)
+
+
+def test_attention_passes_a_nan_on_where_it_is_seen_and_nowhere_else(b2):
+    b = Batch(b2, rng(90), [(1, 40), (3, 40), (18, 40)], 2, 2, 64, 16)
+    k = np.ones((1, 128), np.float32)
+    k[0, 3] = np.nan                                    # KV head 0 of one key of request 1: its last
+    s = b.table[1][39 // 16] * 16 + 39 % 16
+    keep = b.p.ref.bytes.copy()
+    b.p.fill([s], k, np.ones((1, 128), np.float32))
+    got = b.run()
+    assert np.isnan(got[3, :2]).all()                   # the row at position 39, the two query heads of KV head 0
+    rest = got.copy()
+    rest[3, :2] = 0
+    assert np.isfinite(rest).all()
+    b.p.ref.bytes[:] = keep
+    b.p.gpu.copy_(torch.from_numpy(keep))
+    v = np.ones((1, 128), np.float32)
+    v[0, 64 + 40] = np.inf                              # V, KV head 1, the block of dims 32..63
+    b.p.fill([s], np.zeros((1, 128), np.float32), v)
+    got = b.run()
+    assert np.isnan(got[3, 2:, 32:]).all() and np.isfinite(got[3, 2:, :32]).all() and np.isfinite(got[:3]).all() and np.isfinite(got[4:]).all()
+    q = b.q.copy()
+    q[0, 1, 5], q[10, 3, 0] = np.nan, np.inf
+    got = b.run(q=q)
+    assert np.isnan(got[0, 1]).all() and np.isnan(got[10, 3]).all() and np.isfinite(got[0, 0]).all() and np.isfinite(got[10, :3]).all()
+
+
+def test_attention_leaves_out_what_lies_outside_and_says_so(b2):
+    b = Batch(b2, rng(91), [(1, 40), (1, 60), (2, 33)], 2, 2, 64, 16)
+    whole = b.run()
+    # a request longer than max_kv, and one with more rows than max_q
+    got = b.run(max_kv=40)
+    assert u32(b.status)[0] == b2.SERVE_REQUEST and (got[1] == 7).all() and np.array_equal(got[0], whole[0]) and np.allclose(got[2:], whole[2:], atol=1e-5)
+    got = b.run(max_q=1)
+    assert u32(b.status)[0] == b2.SERVE_REQUEST and (got[2:] == 7).all() and np.array_equal(got[:2], whole[:2])
+    # row starts that run backwards or past the buffer
+    got = b.run(q_start=[0, 1, 0, 4])
+    assert u32(b.status)[0] & b2.SERVE_REQUEST and np.array_equal(got[0], whole[0])
+    got = b.run(q_start=[0, 1, 2, 1 << 30], max_q=1 << 20)
+    assert u32(b.status)[0] == b2.SERVE_REQUEST and (got[2:] == 7).all()
+    # a page that is none: its tokens are left out
+    t = b.table.copy()
+    t[1, 1] = b.p.ref.n_pages
+    got = b.run(table=t)
+    assert u32(b.status)[0] == b2.SERVE_PAGE and np.array_equal(got[0], whole[0]) and np.isfinite(got).all()
+    key = np.r_[0:16, 32:60]
+    for h in range(4):
+        k, v = (b.p.ref.values(i, b.table[1][key // 16], key % 16)[:, h // 2] for i in (0, 1))
+        s = k @ b.q[1, h].astype(np.float64) * b.scale
+        p = np.exp(s - s.max())
+        assert np.allclose(got[1, h], p @ v / p.sum(), atol=1e-4)
+    t[1, :] = SKIP
+    got = b.run(table=t)
+    assert (got[1] == 0).all()
+
+
+def test_attention_over_a_long_cache_in_two_streams(b2):
+    r = rng(92)
+    b = Batch(b2, r, [(1, 9001), (2, 30)], 1, 4, 64, 64)
+    want = b.run()
+    b.check(want)
+    s = [torch.cuda.Stream() for _ in range(2)]
+    for x in s:
+        assert np.array_equal(b.run(stream=x.cuda_stream), want)
+    assert np.array_equal(b.run(), want)  # and the same bits each time
+
+
+def test_attention_refusals_that_need_a_device(b2):
+    b = Batch(b2, rng(93), [(1, 20)], 1, 2, 64, 16)
+    nh, dim = 2, 64
+    q, y = torch.zeros(1, nh, dim, device="cuda"), torch.zeros(1, nh, dim, device="cuda")
+    t, qs, kv = dev(b.table), dev([0, 1]), dev([20])
+    need = b2.kv4_attn_workspace(0, b.p.h, 1, nh, 1, 1, 20)
+    room = torch.zeros(need + 64, dtype=torch.uint8, device="cuda")
+    ok = dict(q=q.data_ptr(), y=y.data_ptr(), table=t.data_ptr(), q_start=qs.data_ptr(), kv=kv.data_ptr(), room=room.data_ptr(), need=need, dev=0)
+
+    def call(**kw):
+        a = dict(ok, **kw)
+        b2.kv4_attn(a["dev"], b.p.h, a["q"], a["y"], 1, nh, a["table"], b.stride, a["q_start"], a["kv"], 1, 1, 20, 0.125, a["room"], a["need"])
+
+    call()
+    host = np.zeros(4096, np.float32)
+    for kw, why in ((dict(q=host.ctypes.data), "q is not device memory"), (dict(y=host.ctypes.data), "y is not device memory"),
+                    (dict(q=0), "q is null"), (dict(kv=0), "kv_len is null"), (dict(q=q.data_ptr() + 2), "aligned"), (dict(room=room.data_ptr() + 4), "aligned"),
+                    (dict(need=need - 1), "workspace holds"), (dict(y=q.data_ptr()), "overlaps"), (dict(y=q.data_ptr() + 4), "overlaps"),
+                    (dict(y=b.p.gpu.data_ptr()), "overlaps"), (dict(room=y.data_ptr()), "overlaps|past the end")):
+        with pytest.raises(b2.B200QError, match=why):
+            call(**kw)
+    with pytest.raises(b2.B200QError):
+        call(dev=99)
+    big = b2.Kv4Pool(b.p.gpu.data_ptr(), 1 << 20, 16, 1, 64, 1, 0)
+    with pytest.raises(b2.B200QError, match="past the end"):
+        b2.kv4_attn(0, big, q.data_ptr(), y.data_ptr(), 1, nh, t.data_ptr(), b.stride, qs.data_ptr(), kv.data_ptr(), 1, 1, 20, 0.125,
+                    room.data_ptr(), need)
+    call()
+
+
+# ---- block maps ----------------------------------------------------------------------------------------------------
+
+def run_map(b2, past, fresh, table, page, free, cursor, n_rows, same=False, free_given=None):
+    past, fresh, t, f, c = dev(past), dev(fresh), dev(table), dev(list(free) + [0]), dev([cursor])
+    c2 = c if same else dev([77])
+    n = len(past)
+    kv, qs, sl, pos, st = dev([5] * n), dev([5] * (n + 1)), dev([5] * (n_rows + 1)), dev([5] * (n_rows + 1)), dev([0])
+    b2.block_map(0, n, past.data_ptr(), fresh.data_ptr(), t.data_ptr(), t.shape[1], page, f.data_ptr(), len(free) if free_given is None else free_given,
+                 c.data_ptr(), c2.data_ptr(), kv.data_ptr(), qs.data_ptr(), sl.data_ptr(), pos.data_ptr(), n_rows, st.data_ptr())
+    sl, pos = u32(sl), u32(pos)
+    assert sl[n_rows] == 5 and pos[n_rows] == 5
+    return u32(t), u32(kv), u32(qs), sl[:n_rows], pos[:n_rows], int(u32(c2)[0]), int(u32(st)[0])
+
+
+@pytest.mark.parametrize("n_req,page,most", [(1, 16, 1), (1, 64, 300), (5, 16, 40), (64, 48, 3), (1023, 16, 9), (1024, 32, 2), (1500, 16, 50), (3, 16, 9000)])
+def test_block_map(b2, n_req, page, most):
+    r = rng(94, n_req, page)
+    past = r.integers(0, 130, n_req)
+    past[::3] = past[::3] // page * page  # full pages
+    fresh = r.integers(0, most + 1, n_req)
+    fresh[0] = most
+    stride = int(max(-(-(past + fresh) // page))) + 1
+    table = r.integers(0, 1 << 20, (n_req, stride))
+    need = int(sum(-(-(past + fresh) // page) - -(-past // page)))
+    free = r.permutation(need + 9)
+    rows = int(fresh.sum()) + 7
+    for same in (False, True):
+        got = run_map(b2, past, fresh, table, page, free, 3, rows, same)
+        want = ref.block_map(past, fresh, table, page, free, 3, rows)
+        for g, w in zip(got[:5], want[:5]):
+            assert np.array_equal(np.asarray(g, np.int64), np.asarray(w, np.int64))
+        assert got[5] == want[5] and got[6] == 0
+
+
+def test_block_map_runs_short(b2):
+    past, fresh = [0, 10, 40], [20, 30, 30]
+    table = np.full((3, 4), 6)
+    for free, cursor in (([9, 8, 7], 0), ([9, 8, 7], 2), ([], 0), ([1, 2], 7)):
+        got = run_map(b2, past, fresh, table, 16, free, cursor, 90)
+        want = ref.block_map(past, fresh, table, 16, free, cursor, 90)
+        for g, w in zip(got[:5], want[:5]):
+            assert np.array_equal(np.asarray(g, np.int64), np.asarray(w, np.int64))
+        assert got[5] == want[5] and got[6] == b2.SERVE_SHORT
+    # fewer rows than tokens: the rows that there are
+    got = run_map(b2, [0], [20], np.zeros((1, 2)), 16, [3, 4], 0, 10)
+    assert got[6] == b2.SERVE_REQUEST and list(got[3]) == [48 + i for i in range(10)] and list(got[2]) == [0, 20]
+    # lengths whose sum passes 32 bits
+    got = run_map(b2, [0xFFFFFFF0], [0x20], np.zeros((1, 2)), 16, [3, 4], 0, 8)
+    assert got[6] & b2.SERVE_SHORT and list(got[1]) == [32] and (got[3] == SKIP).all()
+
+
+# ---- beam selection ------------------------------------------------------------------------------------------------
+
+def run_select(b2, x, scores, n_req, beams, n_out, pad=0, stream=None):
+    x = np.concatenate([x, np.full((len(x), pad), np.inf, np.float32)], 1) if pad else x
+    d, s = dev(x), dev(scores)
+    k, vocab = n_req * n_out, x.shape[1] - pad
+    out, par, tok = torch.full((k,), 5.0, device="cuda"), dev([5] * k), dev([5] * k)
+    need = b2.beam_select_workspace(0, n_req, beams, vocab, n_out)
+    room = torch.full((need,), 0xFF, dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    b2.beam_select(0, d.data_ptr(), vocab, s.data_ptr(), n_req, beams, n_out, out.data_ptr(), par.data_ptr(), tok.data_ptr(), room.data_ptr(), need,
+                   x.shape[1], stream)
+    torch.cuda.synchronize()
+    return out.cpu().numpy().reshape(n_req, n_out), u32(par).reshape(n_req, n_out), u32(tok).reshape(n_req, n_out)
+
+
+def check_select(got, x, scores, n_req, beams, n_out):
+    want = ref.select(x, scores, n_req, beams, n_out)
+    for r in range(n_req):
+        n = len(want[r])
+        assert [(int(a), int(b)) for a, b in zip(got[1][r, :n], got[2][r, :n])] == [(b, t) for _, b, t in want[r]]
+        # the sum of e^x is kept to FP32 (relative 2^-20 over partial sums of at most 64): lse within 2^-20, then one rounding
+        w = np.array([s for s, _, _ in want[r]])
+        assert np.all(np.abs(got[0][r, :n] - w) <= 2.0 ** -20 + np.abs(w) * 2.0 ** -24)
+        assert (got[0][r, n:] == -np.inf).all() and (got[1][r, n:] == SKIP).all() and (got[2][r, n:] == SKIP).all()
+
+
+@pytest.mark.parametrize("n_req,beams,vocab,n_out", [(1, 1, 1, 1), (1, 1, 1, 64), (2, 3, 7, 4), (1, 4, 8191, 8), (3, 2, 8192, 1), (1, 5, 8193, 10),
+                                                     (2, 8, 20000, 16), (1, 32, 3001, 64), (40, 2, 33, 2), (1, 2, 70001, 64), (1, 1, 1 << 20, 3)])
+def test_select(b2, n_req, beams, vocab, n_out):
+    r = rng(95, vocab, n_out)
+    x = r.normal(0, 2, (n_req * beams, vocab)).astype(np.float32)
+    scores = -r.uniform(0, 9, n_req * beams).astype(np.float32)
+    check_select(run_select(b2, x, scores, n_req, beams, n_out), x, scores, n_req, beams, n_out)
+    check_select(run_select(b2, x, scores, n_req, beams, n_out, pad=3), x, scores, n_req, beams, n_out)
+
+
+def test_select_ties_masks_and_dead_beams(b2):
+    r = rng(96)
+    beams, vocab, n_out = 6, 9000, 32
+    x = r.integers(-3, 4, (beams, vocab)).astype(np.float32)   # ties everywhere
+    scores = np.zeros(beams, np.float32)
+    check_select(run_select(b2, x, scores, 1, beams, n_out), x, scores, 1, beams, n_out)
+    x[:] = 1.0                                                  # nothing but ties
+    check_select(run_select(b2, x, scores, 1, beams, n_out), x, scores, 1, beams, n_out)
+    x[:] = np.where(np.arange(vocab) % 2, 0.0, -0.0)            # zeros of both signs
+    check_select(run_select(b2, x, scores, 1, beams, n_out), x, scores, 1, beams, n_out)
+    x = r.normal(0, 1, (beams, vocab)).astype(np.float32)
+    x[0, ::2], x[1], x[2, 5], x[3, 7], x[4, 1:] = -np.inf, -np.inf, np.nan, np.inf, -np.inf
+    check_select(run_select(b2, x, scores, 1, beams, n_out), x, scores, 1, beams, n_out)
+    for bad in (-np.inf, np.inf, np.nan):
+        s = np.array([0, bad, bad, bad, bad, bad], np.float32)
+        check_select(run_select(b2, x, s, 1, beams, n_out), x, s, 1, beams, n_out)
+    x[:] = -np.inf                                              # nothing at all
+    check_select(run_select(b2, x, scores, 1, beams, n_out), x, scores, 1, beams, n_out)
+    x[2, 8999] = 3.0                                            # one candidate
+    check_select(run_select(b2, x, scores, 1, beams, n_out), x, scores, 1, beams, n_out)
+    x[2, 0] = np.finfo(np.float32).max                          # sums that are one term
+    x[3, 1] = np.finfo(np.float32).min
+    check_select(run_select(b2, x, scores, 1, beams, n_out), x, scores, 1, beams, n_out)
+
+
+# ---- reordering ----------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("beams", [1, 2, 4, 5, 8, 9, 16, 17, 32])
+@pytest.mark.parametrize("row,layers,pad,off", [(1, 1, 0, 0), (3, 2, 5, 1), (4, 1, 0, 4), (16, 3, 16, 0), (100, 2, 4, 0), (4096, 1, 0, 0), (5000, 2, 8, 8)])
+def test_beam_reorder(b2, beams, row, layers, pad, off):
+    r = rng(97, beams, row)
+    n_req = 3
+    n = n_req * beams
+    layer = n * row + pad
+    host = r.integers(0, 256, off + layers * layer, dtype=np.uint8)
+    parent = r.integers(0, beams, n)
+    if beams > 4:
+        parent[1], parent[2] = SKIP, beams  # none, and no beam
+    src, dp = dev(host), dev(parent)
+    rows = host[off:].reshape(layers, layer)[:, :n * row].reshape(layers, n_req, beams, row)
+    want = rows.copy()
+    for q in range(n_req):
+        for b in range(beams):
+            p = parent[q * beams + b]
+            want[:, q, b] = rows[:, q, p] if p < beams else 99
+    for same in (False, True):
+        out, st = (src if same else torch.full_like(src, 99)), dev([0])
+        b2.beam_reorder(0, src.data_ptr() + off, out.data_ptr() + off, dp.data_ptr(), n_req, beams, row, layers, layer, layer, st.data_ptr())
+        got = out.cpu().numpy()[off:].reshape(layers, layer)
+        w = want.copy()
+        for i in np.nonzero(parent >= beams)[0]:
+            w[:, i // beams, i % beams] = rows[:, i // beams, i % beams] if same else 99
+        assert np.array_equal(got[:, :n * row].reshape(w.shape), w)
+        assert np.array_equal(got[:, n * row:], host[off:].reshape(layers, layer)[:, n * row:] if same else np.full((layers, pad), 99))
+        assert u32(st)[0] == (b2.SERVE_PARENT if beams > 4 else 0)
+
+
+@pytest.mark.parametrize("beams,kv,page,dim", [(1, 5, 16, 32), (3, 0, 16, 64), (4, 16, 16, 128), (4, 17, 16, 96), (8, 100, 64, 64), (12, 1, 32, 32),
+                                               (32, 47, 48, 64), (5, 130, 32, 256)])
+def test_kv4_reorder(b2, beams, kv, page, dim):
+    r = rng(98, beams, kv)
+    n_req, layers, n_kv = 2, 3, 2
+    n = n_req * beams
+    stride = kv // page + 2
+    n_pages = n * stride + 1
+    table = r.permutation(n_pages)[:n * stride].reshape(n, stride)
+    layer = n_pages * n_kv * (page // 16) * ref.tile_bytes(dim) + 64
+    host = r.integers(0, 256, (layers, layer), dtype=np.uint8)
+    parent = r.integers(0, beams, n)
+    if beams > 4:
+        parent[3] = SKIP
+    pool, dt, dk, dp, st = dev(host), dev(table), dev([kv] * n), dev(parent), dev([0])
+    h = b2.Kv4Pool(pool.data_ptr(), n_pages, page, n_kv, dim, layers, layer)
+    b2.kv4_reorder(0, h, dt.data_ptr(), stride, dk.data_ptr(), dp.data_ptr(), n_req, beams, st.data_ptr())
+    full, tail = divmod(kv, page)
+    wt, wp = table.copy(), host.copy()
+    pages, old = wp[:, :-64].reshape(layers, n_pages, n_kv, page // 16, -1), host[:, :-64].reshape(layers, n_pages, n_kv, page // 16, -1)
+    tiles = -(-tail // 16)
+    for i in range(n):
+        p = parent[i]
+        if p >= beams:
+            continue
+        p += i // beams * beams
+        wt[i, :full] = table[p, :full]
+        if tail:
+            pages[:, table[i, full], :, :tiles] = old[:, table[p, full], :, :tiles]
+    assert np.array_equal(u32(dt), wt) and np.array_equal(pool.cpu().numpy(), wp) and u32(st)[0] == 0
+
+
+def test_kv4_reorder_leaves_out_what_lies_outside(b2):
+    r = rng(99)
+    page, dim, n_kv, n_pages = 16, 32, 1, 6
+    host = r.integers(0, 256, (n_pages, 18 * dim), dtype=np.uint8)
+    for table, kv, parent, bit in (([[0, 9], [2, 3]], 20, [1, 0], b2.SERVE_PAGE), ([[0, 1], [2, 3]], 40, [1, 0], b2.SERVE_REQUEST),
+                                   ([[0, 1], [2, 3]], 20, [7, 0], b2.SERVE_PARENT)):
+        pool, dt, dk, dp, st = dev(host), dev(table), dev([kv] * 2), dev(parent), dev([0])
+        b2.kv4_reorder(0, b2.Kv4Pool(pool.data_ptr(), n_pages, page, n_kv, dim, 1, 0), dt.data_ptr(), 2, dk.data_ptr(), dp.data_ptr(), 1, 2, st.data_ptr())
+        got = pool.cpu().numpy()
+        assert u32(st)[0] == bit
+        if bit == b2.SERVE_PARENT:
+            host2 = host.copy()
+            host2[3] = host[1]
+            assert np.array_equal(got, host2) and np.array_equal(u32(dt), [[0, 1], [0, 3]])
+        else:
+            assert np.array_equal(got, host)
+
+
+# ---- together --------------------------------------------------------------------------------------------------------
+
+def test_beam_search_with_a_paged_cache_in_a_captured_graph(b2):
+    """Two requests of three beams: a prompt, then eight steps, each one replay of a graph that maps blocks, stores K and V, attends,
+    scores a small vocabulary and reorders a state, the tables and the tail pages by the chosen parents."""
+    r = rng(100)
+    n_req, beams, n_kv, group, dim, page, vocab, steps, prompt = 2, 3, 2, 2, 64, 16, 50, 8, [21, 30]
+    n, nh = n_req * beams, n_kv * group
+    wq, wk, wv = (r.normal(0, 0.3, (16, c)).astype(np.float32) for c in (nh * dim, n_kv * dim, n_kv * dim))
+    wo, emb = r.normal(0, 0.2, (nh * dim, vocab)).astype(np.float32), r.normal(0, 1, (vocab, 16)).astype(np.float32)
+    n_pages, stride = 80, 5
+    p = Paged(b2, r, n_pages, page, n_kv, dim)
+    order = r.permutation(n_pages)
+    table, at = np.zeros((n, stride), np.int64), 0
+    words = [r.integers(0, vocab, m) for m in prompt]
+    for i in range(n):  # every beam starts from its request's prompt: full pages shared, a tail page of its own
+        m, first = prompt[i // beams], i // beams * beams
+        for b in range(-(-m // page)):
+            if i == first or b == m // page:
+                table[i, b] = order[at]
+                at += 1
+            else:
+                table[i, b] = table[first, b]
+        x = emb[words[i // beams]]
+        slots = table[i][np.arange(m) // page] * page + np.arange(m) % page
+        p.fill(slots, (x @ wk).astype(np.float32), (x @ wv).astype(np.float32))
+    free = order[at:]
+
+    # device side
+    g = {k: dev(v) for k, v in dict(table=table, free=free, cursor=[0], past=[prompt[i // beams] for i in range(n)], fresh=[1] * n, kv=[0] * n,
+                                    qs=[0] * (n + 1), slots=[0] * n, pos=[0] * n, parent=[0] * n, token=[0] * n, status=[0],
+                                    tok=[int(words[i // beams][-1]) for i in range(n)]).items()}
+    W = [torch.from_numpy(w).cuda() for w in (wq, wk, wv, wo, emb)]
+    scores = torch.tensor([0.0] + [-math.inf] * (beams - 1), device="cuda").repeat(n_req)
+    out, state = torch.zeros(n, device="cuda"), torch.arange(n * 40, device="cuda", dtype=torch.float32).reshape(n, 40)
+    k, v, q, y = (torch.zeros(n, c, device="cuda") for c in (n_kv * dim, n_kv * dim, nh * dim, nh * dim))
+    logits = torch.zeros(n, vocab, device="cuda")
+    ptr = {a: t.data_ptr() for a, t in g.items()}
+    need = b2.kv4_attn_workspace(0, p.h, n, nh, n, 1, stride * page)
+    need2 = b2.beam_select_workspace(0, n_req, beams, vocab, beams)
+    room, room2 = (torch.empty(m, dtype=torch.uint8, device="cuda") for m in (need, need2))
+
+    def step():
+        st = torch.cuda.current_stream().cuda_stream
+        b2.block_map(0, n, ptr["past"], ptr["fresh"], ptr["table"], stride, page, ptr["free"], len(free), ptr["cursor"], ptr["cursor"], ptr["kv"],
+                     ptr["qs"], ptr["slots"], ptr["pos"], n, ptr["status"], st)
+        x = W[4][g["tok"].long()]
+        q.copy_(x @ W[0]), k.copy_(x @ W[1]), v.copy_(x @ W[2])
+        b2.kv4_store(0, p.h, k.data_ptr(), v.data_ptr(), ptr["slots"], n, status=ptr["status"], stream=st)
+        b2.kv4_attn(0, p.h, q.data_ptr(), y.data_ptr(), n, nh, ptr["table"], stride, ptr["qs"], ptr["kv"], n, 1, stride * page, 0.125, room.data_ptr(),
+                    need, status=ptr["status"], stream=st)
+        logits.copy_(y @ W[3])
+        b2.beam_select(0, logits.data_ptr(), vocab, scores.data_ptr(), n_req, beams, beams, out.data_ptr(), ptr["parent"], ptr["token"],
+                       room2.data_ptr(), need2, stream=st)
+        b2.beam_reorder(0, state.data_ptr(), state.data_ptr(), ptr["parent"], n_req, beams, 160, status=ptr["status"], stream=st)
+        b2.kv4_reorder(0, p.h, ptr["table"], stride, ptr["kv"], ptr["parent"], n_req, beams, ptr["status"], st)
+        scores.copy_(out), g["tok"].copy_(g["token"]), g["past"].copy_(g["kv"])
+
+    # host side, in step with it
+    hist = [[list(map(int, words[i // beams])) for i in range(n)]][0]
+    keys = [[int(t) for t in h] for h in hist]      # the tokens whose K and V a beam holds
+    hscore = [0.0 if i % beams == 0 else -np.inf for i in range(n)]
+    tok = [int(words[i // beams][-1]) for i in range(n)]
+    hstate = np.arange(n * 40, dtype=np.float32).reshape(n, 40)
+    stream = torch.cuda.Stream()
+    keep_all = {a: t.clone() for a, t in g.items()}, scores.clone(), state.clone(), p.gpu.clone()
+    with torch.cuda.stream(stream):
+        step()  # warm-up, then everything is put back
+        stream.synchronize()
+        for a, t in keep_all[0].items():
+            g[a].copy_(t)
+        scores.copy_(keep_all[1]), state.copy_(keep_all[2]), p.gpu.copy_(keep_all[3])
+        graph = torch.cuda.CUDAGraph()
+        stream.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            step()
+    torch.cuda.synchronize()
+
+    def q4(x):
+        c, d = ref.quantize(x.reshape(-1, dim).astype(np.float32))
+        return ((c.astype(np.float64) - 8) * np.repeat(d.astype(np.float64), 32, -1)).reshape(x.shape)
+
+    for s in range(steps):
+        graph.replay()
+        torch.cuda.synchronize()
+        lg = np.zeros((n, vocab))
+        for i in range(n):
+            keys[i].append(tok[i])
+            x = emb[keys[i]]
+            kk, vv = q4(x @ wk).reshape(-1, n_kv, dim), q4(x @ wv).reshape(-1, n_kv, dim)
+            qq = (emb[tok[i]] @ wq).astype(np.float64).reshape(nh, dim)
+            yy = []
+            for h in range(nh):
+                z = kk[:, h // group] @ qq[h] * 0.125
+                e = np.exp(z - z.max())
+                yy.append(e @ vv[:, h // group] / e.sum())
+            lg[i] = np.concatenate(yy) @ wo.astype(np.float64)
+        want = ref.select(lg, np.array(hscore), n_req, beams, beams)
+        got_p, got_t, got_s = u32(g["parent"]).reshape(n_req, -1), u32(g["token"]).reshape(n_req, -1), out.cpu().numpy().reshape(n_req, -1)
+        new_keys, new_tok, new_score, new_state = [], [], [], []
+        for q_ in range(n_req):
+            for j, (sc, b, t) in enumerate(want[q_]):
+                assert (b, t) == (int(got_p[q_, j]), int(got_t[q_, j])), (s, q_, j)
+                assert abs(sc - got_s[q_, j]) < 1e-3  # FP32 products of the host's and the device's matrices, added up over the steps
+                i = q_ * beams + b
+                new_keys.append(list(keys[i])), new_tok.append(t), new_score.append(float(got_s[q_, j])), new_state.append(hstate[i])
+        keys, tok, hscore, hstate = new_keys, new_tok, new_score, np.stack(new_state)
+        assert np.array_equal(state.cpu().numpy(), hstate)
+        assert u32(g["status"])[0] == 0 and list(u32(g["kv"])) == [prompt[i // beams] + s + 1 for i in range(n)]
+        # the cache holds each beam's own tokens, page by page
+        t = u32(g["table"]).astype(np.int64)
+        p.ref.bytes[:] = p.gpu.cpu().numpy()
+        for i in range(n):
+            m = len(keys[i])
+            vals = p.ref.values(0, t[i][np.arange(m) // page], np.arange(m) % page).reshape(m, -1)
+            assert np.abs(vals - q4(emb[keys[i]] @ wk)).max() < 0.25 * np.abs(vals).max()  # a code may differ by one where x W does by a rounding
+    del graph
