@@ -186,7 +186,7 @@ Kv4View view_of(const b200q_kv4_pool *p) {
 
 size_t rows_extent(size_t rows, size_t stride, size_t width) { return rows ? ((rows - 1) * stride + width) * 4 : 0; }
 
-constexpr unsigned kMaxReq = 65535;
+constexpr unsigned kMaxReq = 65535, kMaxAttnReq = 4096;
 constexpr size_t kMaxStride = size_t(1) << 32;
 
 int rows_call(const char *name, bool store, int device, const b200q_kv4_pool *pool, float *k, float *v, const uint32_t *slots, unsigned n,
@@ -233,7 +233,7 @@ int rows_call(const char *name, bool store, int device, const b200q_kv4_pool *po
 
 void check_attn(Call &c, const b200q_kv4_pool *pool, unsigned n_rows, unsigned n_head, unsigned n_req, unsigned max_q, unsigned max_kv) {
     c.need(n_head >= 1 && n_head <= 1024 && n_head % pool->n_kv_head == 0, "n_head is not a multiple of n_kv_head up to 1024");
-    c.need(n_req >= 1 && n_req <= kMaxReq, "n_req is not 1 to 65535");
+    c.need(n_req >= 1 && n_req <= kMaxAttnReq, "n_req is not 1 to 4096");
     c.need(n_rows <= (1u << 24), "n_rows is over 2^24");
     c.need(max_q >= 1 && max_q <= (1u << 24), "max_q is not 1 to 2^24");
     c.need(max_kv >= 1 && max_kv <= (1u << 30), "max_kv is not 1 to 2^30");
