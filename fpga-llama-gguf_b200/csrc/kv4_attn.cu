@@ -9,9 +9,9 @@
 // and the scales meet FP32 numbers only:
 //   s_t  = sum_b d_tb (sum_i q_i (c_ti - 8))      per block a 16 x 8 x 32 matrix product, scaled and added in FP32
 //   y_i  = sum_t (p_t d_tb) (c_ti - 8)            the weight of a token differs by block, not by dim
-// The FP32 factors (q, and p_t d_tb) are split as hi + lo / 2048 into two FP16 numbers, 22 bits in all, which sit in rows
-// r and r + 8 of the matrix instruction's A operand: 8 query rows fill its 16 rows, and FP32 accuracy costs no second
-// instruction. q's rows are first scaled by a power of two to below 2^11.
+// The FP32 factors (q, and p_t d_tb) are split into two FP16 numbers, 22 bits in all, which sit in rows r and r + 8 of the
+// matrix instruction's A operand: 8 query rows fill its 16 rows, and FP32 accuracy costs no second instruction. q's
+// rows are first scaled by a power of two to below 2^11, and their lower parts by 2048.
 #include <cuda_runtime.h>
 
 #include <mutex>
@@ -31,6 +31,7 @@ namespace {
 
 constexpr unsigned kWarps = 4, kThreads = kWarps * 32;
 constexpr unsigned kMaxChunkTiles = 256;  // a warp adds at most 64 tiles into its accumulators before they are merged in FP32
+constexpr unsigned kMergeChunk = 256;    // chunks whose factors the merge holds at a time
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ void tell(uint32_t *status, unsigned bit) {
@@ -160,10 +161,18 @@ __device__ __forceinline__ GroupSpan span_of(const Kv4AttnArgs &a, const Request
 }
 
 // ---- the tile product -----------------------------------------------------------------------------------------------
-__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
+// two FP32 multiply-adds in one instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n .reg .b64 x, y, z, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n fma.rn.f32x2 w, x, y, z;\n mov.b64 {%0, %1}, w;\n}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
 }
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
@@ -173,8 +182,12 @@ __device__ __forceinline__ float exp2_fast(float x) {
 __device__ __forceinline__ uint32_t h2(half2 x) { return *reinterpret_cast<uint32_t *>(&x); }
 __device__ __forceinline__ half2 as_h2(uint32_t x) { return *reinterpret_cast<half2 *>(&x); }
 
-// Two nibbles of a word (bits 0..3 and 16..19, or with shift 4: bits 4..7 and 20..23) as FP16: put into the mantissa of
-// 1024 they read 1024 + c (or 1024 + 16 c); less 1032 (1152) that is c - 8 (16 (c - 8)), exactly.
+// Two nibbles of a word, bits 0..3 and 16..19 (low) or 4..7 and 20..23 (high), as FP16.
+// K: left as they are they read c 2^-24 (16 c 2^-24), and the 8 that a code stands above its value comes off in the sum.
+__device__ __forceinline__ uint32_t low_raw(uint32_t x) { return x & 0x000f000fu; }
+__device__ __forceinline__ uint32_t high_raw(uint32_t x) { return x & 0x00f000f0u; }
+// V (whose sums run over many tokens, where that 8 would swamp them): put into the mantissa of 1024 they read 1024 + c
+// (1024 + 16 c); less 1032 (1152) that is c - 8 (16 (c - 8)), exactly.
 __device__ __forceinline__ uint32_t low_codes(uint32_t x) {
     uint32_t y;
     asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;" : "=r"(y) : "r"(x));
@@ -214,6 +227,10 @@ __device__ __forceinline__ void load_words(uint32_t *w, const uint8_t *at) {
         for (int i = 0; i < N; ++i) w[i] = *reinterpret_cast<const uint32_t *>(at + 4 * i);
     }
 }
+// halves i and j of an array of words as a pair
+__device__ __forceinline__ half2 pair_at(const uint32_t *w, int i, int j) {
+    return as_h2(__byte_perm(w[i >> 1], w[j >> 1], (i & 1 ? 0x32u : 0x10u) | (j & 1 ? 0x7600u : 0x5400u)));
+}
 // half i of an array of words
 __device__ __forceinline__ float half_at(const uint32_t *w, int i) {
     return __half2float(__ushort_as_half(uint16_t(i & 1 ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu)));
@@ -224,7 +241,7 @@ struct Shape {
     static constexpr int kTile = NB * 576;                       // bytes of a tile
     static constexpr int kSlots = NB <= 2 ? 8 : NB <= 4 ? 6 : 4;  // tiles a warp has on their way
     static constexpr bool kQInRegs = NB * MT <= 4;
-    static constexpr int kQBytes = kQInRegs ? 0 : MT * NB * 2 * 32 * 16;
+    static constexpr int kQBytes = kQInRegs ? 0 : MT * NB * 3 * 32 * 16;  // per block: two k-steps of q, and the sums' start
     static constexpr int kOutBytes = kWarps * MT * 8 * (NB * 32 + 2) * 4;  // the warps' results, in the ring's place
     static constexpr int kRing = kWarps * kSlots * kTile;
     static constexpr int kSmem = kQBytes + (kRing > kOutBytes ? kRing : kOutBytes);
@@ -306,6 +323,7 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(const Kv4AttnArgs a,
 
         // the rows' queries: split, in the order in which a block's words hold the dims
         uint32_t qa[S::kQInRegs ? MT : 1][S::kQInRegs ? NB * 2 : 1][4];
+        float start[S::kQInRegs ? MT : 1][S::kQInRegs ? NB : 1][4];  // -8 sum q over a block, of the rows' upper and lower parts
         float scale[MT];
         int pos[MT], low[MT];  // the keys a row sees: [low, pos]
         const unsigned all = rq.fresh * per, row0 = group * plan.rows;
@@ -336,26 +354,45 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(const Kv4AttnArgs a,
             top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
             top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
             int ex = int(__float_as_uint(top) >> 23) - 127 - 10;  // x / 2^ex is below 2^11
-            ex = ex < -110 ? -110 : ex > 110 ? 110 : ex;
+            ex = ex < -110 ? -110 : ex > 100 ? 100 : ex;
             const float down = __uint_as_float(unsigned(127 - ex) << 23);
-            scale[m] = a.scale * kLog2e * __uint_as_float(unsigned(127 + ex) << 23);
+            scale[m] = a.scale * kLog2e * __uint_as_float(unsigned(127 + 24 + ex) << 23);  // (K's codes come times 2^-24)
 #pragma unroll
-            for (int i = 0; i < NB * 2; ++i) {
-                const float f = i & 1 ? down * 0.0625f : down;  // the high nibbles' codes come times 16
-                uint32_t v[4];
-                split2(x[i][0] * f, x[i][2] * f, v[0], v[1]);
-                split2(x[i][1] * f, x[i][3] * f, v[2], v[3]);
+            for (int b = 0; b < NB; ++b) {
+                float hi = 0.0f, lo = 0.0f;
+#pragma unroll
+                for (int i = 2 * b; i < 2 * b + 2; ++i) {
+                    const float f = i & 1 ? down * 0.0625f : down;  // the high nibbles' codes come times 16
+                    uint32_t v[4];
+                    split2(x[i][0] * f, x[i][2] * f, v[0], v[1]);
+                    split2(x[i][1] * f, x[i][3] * f, v[2], v[3]);
+                    const float2 s0 = __half22float2(as_h2(v[0])), s1 = __half22float2(as_h2(v[1])), s2 = __half22float2(as_h2(v[2])),
+                                 s3 = __half22float2(as_h2(v[3]));
+                    const float up = i & 1 ? 16.0f : 1.0f;
+                    hi += up * ((s0.x + s0.y) + (s2.x + s2.y));
+                    lo += up * ((s1.x + s1.y) + (s3.x + s3.y));
+                    if constexpr (S::kQInRegs) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) qa[m][i][e] = v[e];
+                    } else {
+                        if (warp == 0) *reinterpret_cast<uint4 *>(smem + ((m * NB * 3 + i) * 32 + lane) * 16) = make_uint4(v[0], v[1], v[2], v[3]);
+                    }
+                }
+                hi += __shfl_xor_sync(~0u, hi, 1);
+                lo += __shfl_xor_sync(~0u, lo, 1);
+                hi = -0x1p-21f * (hi + __shfl_xor_sync(~0u, hi, 2));
+                lo = -0x1p-21f * (lo + __shfl_xor_sync(~0u, lo, 2));
                 if constexpr (S::kQInRegs) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) qa[m][i][e] = v[e];
+                    start[m][b][0] = start[m][b][1] = hi;
+                    start[m][b][2] = start[m][b][3] = lo;
                 } else {
-                    if (warp == 0) *reinterpret_cast<uint4 *>(smem + ((m * NB * 2 + i) * 32 + lane) * 16) = make_uint4(v[0], v[1], v[2], v[3]);
+                    if (warp == 0) *reinterpret_cast<float4 *>(smem + ((m * NB * 3 + NB * 2 + b) * 32 + lane) * 16) = make_float4(hi, hi, lo, lo);
                 }
             }
         }
         if constexpr (!S::kQInRegs) __syncthreads();
 
-        float o[MT][NB * 4][4], top[MT], sum[MT], limit = 0.0f, lift = 1.0f;
+        float o[MT][NB * 4][4], top[MT], sum[MT], limit = 0.0f, lift = 1.0f, lift_d = 1.0f;
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
             top[m] = -INFINITY;
@@ -373,13 +410,13 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(const Kv4AttnArgs a,
         auto take = [&](const uint8_t *tile, int key0, auto masked) {
             constexpr bool kMasked = decltype(masked)::value;
             // scores of the tile's keys 8 j + 2 t + i
-            float s[MT][2][2];
+            float2 s[MT][2];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 uint32_t ds[NB];
                 load_words<NB>(ds, tile + NB * 512 + (4 * j + t) * NB * 4);
 #pragma unroll
-                for (int m = 0; m < MT; ++m) s[m][j][0] = s[m][j][1] = 0.0f;
+                for (int m = 0; m < MT; ++m) s[m][j] = make_float2(0.0f, 0.0f);
 #pragma unroll
                 for (int p = 0; p < kPlanes; ++p) {
                     const int nbp = NB - 4 * p < 4 ? NB - 4 * p : 4;
@@ -394,42 +431,47 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(const Kv4AttnArgs a,
                         if (b >= nbp) break;
                         const int bb = 4 * p + b;
                         const uint32_t x8 = w[b] >> 8;
-                        const uint32_t l0 = low_codes(w[b]), l1 = low_codes(x8), h0 = high_codes(w[b]), h1 = high_codes(x8);
-                        const float d0 = half_at(ds, bb), d1 = half_at(ds, NB + bb);
+                        const float2 d = make_float2(half_at(ds, bb), half_at(ds, NB + bb));
 #pragma unroll
                         for (int m = 0; m < MT; ++m) {
-                            float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                            float c[4], e[4];
                             uint32_t q0[4], q1[4];
                             if constexpr (S::kQInRegs) {
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) q0[e] = qa[m][bb * 2][e], q1[e] = qa[m][bb * 2 + 1][e];
+                                for (int i = 0; i < 4; ++i) q0[i] = qa[m][bb * 2][i], q1[i] = qa[m][bb * 2 + 1][i], c[i] = start[m][bb][i];
                             } else {
-                                load_words<4>(q0, smem + ((m * NB * 2 + bb * 2) * 32 + lane) * 16);
-                                load_words<4>(q1, smem + ((m * NB * 2 + bb * 2 + 1) * 32 + lane) * 16);
+                                load_words<4>(q0, smem + ((m * NB * 3 + bb * 2) * 32 + lane) * 16);
+                                load_words<4>(q1, smem + ((m * NB * 3 + bb * 2 + 1) * 32 + lane) * 16);
+                                load_words<4>(reinterpret_cast<uint32_t *>(c), smem + ((m * NB * 3 + NB * 2 + bb) * 32 + lane) * 16);
                             }
-                            mma16816(c, q0, l0, l1);
-                            mma16816(c, q1, h0, h1);
-                            s[m][j][0] += d0 * (c[0] + c[2] * (1.0f / 2048));
-                            s[m][j][1] += d1 * (c[1] + c[3] * (1.0f / 2048));
+                            mma16816(e, q0, low_raw(w[b]), low_raw(x8), c);
+                            mma16816(c, q1, high_raw(w[b]), high_raw(x8), e);
+                            const float2 both = fma2(make_float2(c[2], c[3]), make_float2(1.0f / 2048, 1.0f / 2048), make_float2(c[0], c[1]));
+                            s[m][j] = fma2(d, both, s[m][j]);
                         }
                     }
                 }
             }
             // The running maximum. It moves only when a score passes it, and then to 4 (in powers of two) above the largest, so
             // that it moves seldom; the weights stay below 1.
-            float pr[MT][2][2];
+            float2 pr[MT][2];
+            uint32_t seen[MT][2];  // of a pair of keys, as a mask of halves
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
                 float mx = -INFINITY;
 #pragma unroll
-                for (int j = 0; j < 2; ++j)
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int key = key0 + 8 * j + 2 * int(t) + i;
-                        s[m][j][i] *= scale[m];
-                        if (kMasked && (key < low[m] || key > pos[m])) s[m][j][i] = -INFINITY;
-                        mx = fmaxf(mx, s[m][j][i]);
+                for (int j = 0; j < 2; ++j) {
+                    const int key = key0 + 8 * j + 2 * int(t);
+                    s[m][j].x *= scale[m];
+                    s[m][j].y *= scale[m];
+                    if (kMasked) {
+                        const bool x = key >= low[m] && key <= pos[m], y = key + 1 >= low[m] && key + 1 <= pos[m];
+                        seen[m][j] = (x ? 0x0000ffffu : 0u) | (y ? 0xffff0000u : 0u);
+                        if (!x) s[m][j].x = -INFINITY;
+                        if (!y) s[m][j].y = -INFINITY;
                     }
+                    mx = fmaxf(mx, fmaxf(s[m][j].x, s[m][j].y));
+                }
                 mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 1));
                 mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 2));
                 if (__any_sync(~0u, mx > top[m])) {
@@ -444,47 +486,43 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(const Kv4AttnArgs a,
                 }
                 const float ref = top[m] == -INFINITY ? 0.0f : top[m];
 #pragma unroll
-                for (int j = 0; j < 2; ++j)
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        pr[m][j][i] = exp2_fast(s[m][j][i] - ref);
-                        sum[m] += pr[m][j][i];
-                    }
+                for (int j = 0; j < 2; ++j) {
+                    pr[m][j] = make_float2(exp2_fast(s[m][j].x - ref), exp2_fast(s[m][j].y - ref));
+                    sum[m] += pr[m][j].x + pr[m][j].y;
+                }
             }
             // the weighted sum of the values: keys along k, dims along n
             uint32_t dv[2][NB];
 #pragma unroll
             for (int j = 0; j < 2; ++j) load_words<NB>(dv[j], tile + NB * 544 + (4 * j + t) * NB * 4);
-            // The weights p d are split after a scaling by 2^13 / `limit`, a power of two that no scale seen so far passes: FP16
-            // then holds them to 22 bits however small the values are.
-            float big = 0.0f;
-            if (kMasked) {
+            // A weight p d is a product of FP16 pairs: with p = ph + pl, wh = fp16(ph d) and wl = fp16(pl d + (ph d - wh)),
+            // where ph d - wh is exact in one FP16 multiply-add. p is lifted by a power of two that keeps the largest weight
+            // below 2^14 (`limit`: a power of two that no scale seen so far passes), so that small values keep 22 bits too; scales
+            // below 1/16 are lifted as well.
+            half2 big2 = __float2half2_rn(0.0f);
 #pragma unroll
-                for (int j = 0; j < 2; ++j)
+            for (int j = 0; j < 2; ++j)
 #pragma unroll
-                    for (int b = 0; b < 2 * NB; ++b) {
-                        bool seen = false;
+                for (int b = 0; b < NB; ++b) {
+                    if (kMasked) {
+                        uint32_t any = 0;
 #pragma unroll
-                        for (int m = 0; m < MT; ++m) seen = seen || s[m][j][b >= NB] != -INFINITY;
-                        if (seen) big = fmaxf(big, fabsf(half_at(dv[j], b)));
+                        for (int m = 0; m < MT; ++m) any |= seen[m][j];
+                        const half2 d = pair_at(dv[j], b, NB + b);
+                        big2 = __hmax2(big2, __habs2(as_h2(h2(d) & any)));
+                    } else {
+                        big2 = __hmax2(big2, __habs2(as_h2(dv[j][b])));
                     }
-            } else {
-                half2 h = __float2half2_rn(0.0f);
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-#pragma unroll
-                    for (int b = 0; b < NB; ++b) h = __hmax2(h, __habs2(as_h2(dv[j][b])));
-                big = fmaxf(__low2float(h), __high2float(h));
-            }
+                }
+            float big = fmaxf(__low2float(big2), __high2float(big2));
             if (__any_sync(~0u, big > limit)) {
-                big = fmaxf(big, __shfl_xor_sync(~0u, big, 1));
-                big = fmaxf(big, __shfl_xor_sync(~0u, big, 2));
 #pragma unroll
-                for (int x = 4; x < 32; x <<= 1) big = fmaxf(big, __shfl_xor_sync(~0u, big, x));  // rows may see different keys
-                const float was = lift;
+                for (int x = 1; x < 32; x <<= 1) big = fmaxf(big, __shfl_xor_sync(~0u, big, x));
+                const float was = lift * lift_d;
                 limit = __uint_as_float((__float_as_uint(fminf(big, 65504.0f)) & 0x7f800000u) + 0x00800000u);  // the next power of two
-                lift = 8192.0f / limit;
-                const float f = lift / was;
+                lift_d = limit < 0x1p-4f ? 0x1p15f : 1.0f;
+                lift = fminf(0x1p14f / (limit * lift_d), 0x1p15f);
+                const float f = lift * lift_d / was;
 #pragma unroll
                 for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -492,10 +530,23 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(const Kv4AttnArgs a,
 #pragma unroll
                         for (int e = 0; e < 4; ++e) o[m][i][e] *= f;
             }
+            if (lift_d != 1.0f) {
+                const half2 f = __float2half2_rn(lift_d);
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) dv[j][b] = h2(__hmul2(as_h2(dv[j][b]), f));
+            }
+            half2 ph[MT][2], pl[MT][2];
 #pragma unroll
             for (int m = 0; m < MT; ++m)
 #pragma unroll
-                for (int j = 0; j < 2; ++j) pr[m][j][0] *= lift, pr[m][j][1] *= lift;
+                for (int j = 0; j < 2; ++j) {
+                    const float x = pr[m][j].x * lift, y = pr[m][j].y * lift;
+                    ph[m][j] = __floats2half2_rn(x, y);
+                    const float2 back = __half22float2(ph[m][j]);
+                    pl[m][j] = __floats2half2_rn(x - back.x, y - back.y);
+                }
             const uint32_t sel = (g >> 2) * 0x2222u + 0x4400u;  // byte 2 (g / 4) of two words, each twice
 #pragma unroll
             for (int p = 0; p < kPlanes; ++p) {
@@ -520,12 +571,11 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(const Kv4AttnArgs a,
                     for (int m = 0; m < MT; ++m)
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
-                            float w0 = pr[m][j][0] * half_at(dv[j], bb), w1 = pr[m][j][1] * half_at(dv[j], NB + bb);
-                            if (kMasked) {  // a key that is not seen weighs nothing, whatever its scale holds
-                                if (s[m][j][0] == -INFINITY) w0 = 0.0f;
-                                if (s[m][j][1] == -INFINITY) w1 = 0.0f;
-                            }
-                            split2(w0, w1, wa[m][2 * j], wa[m][2 * j + 1]);
+                            uint32_t dd = h2(pair_at(dv[j], bb, NB + bb));
+                            if (kMasked) dd &= seen[m][j];  // a key that is not seen weighs nothing, whatever its scale holds
+                            const half2 wh = __hmul2(ph[m][j], as_h2(dd));
+                            wa[m][2 * j] = h2(wh);
+                            wa[m][2 * j + 1] = h2(__hfma2(pl[m][j], as_h2(dd), __hfma2(ph[m][j], as_h2(dd), __hneg2(wh))));
                         }
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
@@ -533,8 +583,8 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(const Kv4AttnArgs a,
                         const uint32_t l0 = low_codes(b0), l1 = low_codes(b1), h0 = high_codes(b0), h1 = high_codes(b1);
 #pragma unroll
                         for (int m = 0; m < MT; ++m) {
-                            mma16816(o[m][bb * 4 + x * 2], wa[m], l0, l1);
-                            mma16816(o[m][bb * 4 + x * 2 + 1], wa[m], h0, h1);
+                            mma16816(o[m][bb * 4 + x * 2], wa[m], l0, l1, o[m][bb * 4 + x * 2]);
+                            mma16816(o[m][bb * 4 + x * 2 + 1], wa[m], h0, h1, o[m][bb * 4 + x * 2 + 1]);
                         }
                     }
                 }
@@ -570,7 +620,7 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(const Kv4AttnArgs a,
 
         // the warps' results, joined in the ring's place: [warp][row][dim]
         float *out = reinterpret_cast<float *>(smem + S::kQBytes);
-        const float drop = 1.0f / lift;
+        const float drop = 1.0f / (lift * lift_d);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
             sum[m] += __shfl_xor_sync(~0u, sum[m], 1);
@@ -582,7 +632,7 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(const Kv4AttnArgs a,
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const int n = 2 * int(t) + e, b = i / 4, x = i / 2 % 2, h = i & 1;
-                    to[32 * b + 16 * h + 4 * (n & 3) + 2 * (n >> 2) + x] = (o[m][i][e] + o[m][i][2 + e] * (1.0f / 2048)) * (h ? 0.0625f : 1.0f) * drop;
+                    to[32 * b + 16 * h + 4 * (n & 3) + 2 * (n >> 2) + x] = (o[m][i][e] + o[m][i][2 + e]) * (h ? 0.0625f : 1.0f) * drop;
                 }
         }
         __syncthreads();
@@ -590,7 +640,8 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(const Kv4AttnArgs a,
         if (!direct && item >= plan.max_items) {  // rows counted twice (row starts that overlap): no room
             if (tid == 0) tell(a.status, kServeRequest);
         } else {
-            float *part = reinterpret_cast<float *>(a.room) + size_t(item) * plan.rows * (D + 2);
+            float *part = reinterpret_cast<float *>(a.room) + size_t(item) * plan.rows * D;
+            float2 *stat = reinterpret_cast<float2 *>(reinterpret_cast<float *>(a.room) + size_t(plan.max_items) * plan.rows * D) + size_t(item) * plan.rows;
             for (unsigned i = tid; i < MT * 8 * D; i += kThreads) {
                 const unsigned row = i / D, dim = i % D;
                 if (row0 + row >= all) break;
@@ -607,8 +658,8 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(const Kv4AttnArgs a,
                     const unsigned at = row0 + row;
                     a.y[(rq.start + at / per) * a.y_stride + size_t(head * per + at % per) * D + dim] = lv == 0.0f ? 0.0f : ov / lv;
                 } else {
-                    part[row * (D + 2) + dim] = ov;
-                    if (dim == 0) part[row * (D + 2) + D] = mm, part[row * (D + 2) + D + 1] = lv;
+                    part[row * D + dim] = ov;
+                    if (dim == 0) stat[row] = make_float2(mm, lv);
                 }
             }
         }
@@ -620,6 +671,8 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(const Kv4AttnArgs a,
 // Rows whose keys were split: the chunks' maxima, sums and outputs joined. One CTA a row of a unit.
 __global__ void __launch_bounds__(kThreads) kv4_attn_merge_kernel(const Kv4AttnArgs a, const Plan plan) {
     extern __shared__ unsigned prefix_units[];
+    __shared__ float red[kWarps], factor[kMergeChunk], weight[kMergeChunk], sums[kThreads];
+    __shared__ float4 joined[kThreads];
     unsigned *prefix = prefix_units, *units = prefix_units + a.n_req + 1;
     pdl_wait();
     pdl_launch_dependents();
@@ -635,20 +688,54 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_merge_kernel(const Kv4AttnA
         if (n_split <= 1 || at >= rq.fresh * per) continue;
         const unsigned first = prefix[r] + group * a.c.n_kv + head, step = rq.groups * a.c.n_kv;
         if (first + (n_split - 1) * step >= plan.max_items) continue;
-        const size_t gap = size_t(plan.rows) * (dim + 2);
-        const float *part = reinterpret_cast<const float *>(a.room) + size_t(row) * (dim + 2);
+        const size_t gap = size_t(plan.rows) * dim;
+        const float *part = reinterpret_cast<const float *>(a.room) + first * gap + size_t(row) * dim;
+        const float2 *stat = reinterpret_cast<const float2 *>(reinterpret_cast<const float *>(a.room) + plan.max_items * gap) + size_t(first) * plan.rows + row;
+        const size_t part_step = step * gap, stat_step = size_t(step) * plan.rows;
         float m = -INFINITY;
-        for (unsigned s = 0; s < n_split; ++s) m = fmaxf(m, part[(first + s * step) * gap + dim]);
+        for (unsigned s = threadIdx.x; s < n_split; s += kThreads) m = fmaxf(m, stat[s * stat_step].x);
+        for (unsigned o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+        __syncthreads();
+        if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = m;
+        __syncthreads();
+        for (unsigned w = 0; w < kWarps; ++w) m = fmaxf(m, red[w]);
         const float ref = m == -INFINITY ? 0.0f : m;
-        for (unsigned d = threadIdx.x; d < dim; d += kThreads) {
-            float o = 0.0f, l = 0.0f;
-            for (unsigned s = 0; s < n_split; ++s) {
-                const float *x = part + (first + s * step) * gap;
-                const float f = exp2_fast(x[dim] - ref);
-                o += x[d] * f;
-                l += x[dim + 1] * f;
+        // four dims a lane; the groups of lanes that cover the dims share out the chunks, whose factors lie in shared memory
+        const unsigned lanes = dim / 4, groups = kThreads / lanes, mine = threadIdx.x / lanes, d = threadIdx.x % lanes * 4;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float l = 0.0f;
+        for (unsigned s0 = 0; s0 < n_split; s0 += kMergeChunk) {
+            const unsigned n = n_split - s0 < kMergeChunk ? n_split - s0 : kMergeChunk;
+            __syncthreads();
+            for (unsigned s = threadIdx.x; s < n; s += kThreads) {
+                const float2 x = stat[(s0 + s) * stat_step];
+                const float f = exp2_fast(x.x - ref);
+                factor[s] = f;
+                weight[s] = f * x.y;
             }
-            a.y[(rq.start + at / per) * a.y_stride + size_t(head * per + at % per) * dim + d] = l == 0.0f ? 0.0f : o / l;
+            __syncthreads();
+            if (mine < groups) {
+#pragma unroll 4
+                for (unsigned s = mine; s < n; s += groups) {
+                    const float4 x = *reinterpret_cast<const float4 *>(part + (s0 + s) * part_step + d);
+                    const float f = factor[s];
+                    o.x += x.x * f, o.y += x.y * f, o.z += x.z * f, o.w += x.w * f;
+                    l += weight[s];
+                }
+            }
+        }
+        __syncthreads();
+        if (mine < groups) joined[mine * lanes + threadIdx.x % lanes] = o, sums[mine] = l;
+        __syncthreads();
+        if (mine == 0) {
+            for (unsigned i = 1; i < groups; ++i) {
+                const float4 x = joined[i * lanes + threadIdx.x];
+                o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w;
+                l += sums[i];
+            }
+            const float f = l == 0.0f ? 0.0f : 1.0f / l;
+            float *y = a.y + (rq.start + at / per) * a.y_stride + size_t(head * per + at % per) * dim + d;
+            y[0] = l == 0.0f ? 0.0f : o.x * f, y[1] = l == 0.0f ? 0.0f : o.y * f, y[2] = l == 0.0f ? 0.0f : o.z * f, y[3] = l == 0.0f ? 0.0f : o.w * f;
         }
     }
 }
@@ -700,7 +787,7 @@ Plan plan_of(const Kv4AttnArgs &a, unsigned sms) {
 
 size_t kv4_attn_room(const Kv4AttnArgs &a, unsigned sms) {
     const Plan p = plan_of(a, sms);
-    return (size_t(p.max_items) * p.rows * (a.c.dim + 2) * 4 + 15) / 16 * 16;
+    return size_t(p.max_items) * p.rows * (a.c.dim * 4 + 8);
 }
 unsigned kv4_attn_launches(const Kv4AttnArgs &a, unsigned) { return a.max_kv > kWarps * kTileTokens ? 2 : 1; }
 

@@ -162,13 +162,13 @@ class Batch:
         """Against 64 bits. With S = scale max_t sum |q k_t|: a score is off by at most 2^-20 S (FP32 sums of up to 256 products,
         q to 22 bits or more), the exponentials by 2^-21 more, weights and sums of up to some thousand terms in partial sums
         of at most 64 by 2^-18; y by that share of sum p |v|, twice (numerator and denominator).
-        And a weight p d, split into two FP16 numbers after a scaling by 2^13 / limit (limit <= 2 max d) and 2^11 more for the
-        lower one, is off by at most 2^-25 2^-11 2^-13 limit <= 2^-48 max d, where the sum of all p is at least 2^-4 and a value is
-        at most 8 d: n keys add n 8 2^4 2^-48 max d = n 2^-44 max |v| to y at most."""
+        And a weight p d is split into two FP16 numbers after p is lifted by a power of two, 2^15 at least where the largest d
+        is 2^-5 to 2^-1: the lower one is off by at most 2^-25, p by as much, together 2^-24 2^-15 <= 2^-34 max d (other d: less),
+        where the sum of all p is at least 2^-4 and a value is at most 8 d: n keys add n 2^4 2^-34 max |v| to y at most."""
         y, mag, big = ref.attention(self.p.ref, self.q if q is None else q, self.table, self.q_start, self.kv, self.scale, window)
         vmax = max([np.abs(self.p.ref.values(1, self.table[r][np.arange(n) // self.p.ref.page], np.arange(n) % self.p.ref.page)).max()
                     for r, n in enumerate(self.kv) if n] or [0])
-        tol = 2.0 ** -17 * (1 + big[:, :, None] / 8) * mag + (mag > 0) * max(self.kv) * 2.0 ** -44 * vmax
+        tol = 2.0 ** -17 * (1 + big[:, :, None] / 8) * mag + (mag > 0) * max(self.kv) * 2.0 ** -30 * vmax
         assert np.isfinite(got).all()
         bad = np.abs(got - y) - tol
         assert bad.max(initial=0) <= 0, (bad.max(), np.unravel_index(bad.argmax(), bad.shape))
