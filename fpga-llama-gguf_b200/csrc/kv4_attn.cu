@@ -9,17 +9,15 @@
 // and the scales meet FP32 numbers only:
 //   s_t  = sum_b d_tb (sum_i q_i (c_ti - 8))      per block a 16 x 8 x 32 matrix product, scaled and added in FP32
 //   y_i  = sum_t (p_t d_tb) (c_ti - 8)            the weight of a token differs by block, not by dim
-// The FP32 factors (q, and p_t d_tb) are split into two FP16 numbers, 22 bits in all, which sit in rows r and r + 8 of the
-// matrix instruction's A operand: 8 query rows fill its 16 rows, and FP32 accuracy costs no second instruction. q's
-// rows are first scaled by a power of two to below 2^11, and their lower parts by 2048.
+// The FP32 factors (q, and p_t d_tb) are split into two FP16 numbers, 22 bits in all, which sit side by side in two columns of
+// the matrix instruction's B operand: four query rows fill its eight columns, and FP32 accuracy costs no second
+// instruction. q's rows are first scaled by a power of two to below 2^11, and their lower parts by 2048.
 #include <cuda_runtime.h>
-
-#include <mutex>
-#include <type_traits>
 
 #include "common.cuh"
 #include "kv4.cuh"
 #include "pipeline.cuh"
+#include "launch.h"
 #include "serve.h"
 
 namespace b200q {
@@ -30,24 +28,31 @@ constexpr unsigned kAttnMaxReq = 4096;
 namespace {
 
 constexpr unsigned kWarps = 4, kThreads = kWarps * 32;
-constexpr unsigned kMaxChunkTiles = 256;  // a warp adds at most 64 tiles into its accumulators before they are merged in FP32
-constexpr unsigned kMergeChunk = 256;    // chunks whose factors the merge holds at a time
+#ifndef UC
+#define UC 24
+#endif
+constexpr unsigned kUnitCost = UC;        // what a unit costs besides its tiles (its queries, its joined output), in tiles
+constexpr unsigned kMaxRange = 1024;     // a warp adds at most 256 tiles into its accumulators before they are joined in FP32
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ void tell(uint32_t *status, unsigned bit) {
     if (status) atomicOr(status, bit);
 }
 
-struct Plan {
-    unsigned max_items = 0;  // items the workspace holds partial results for
-    unsigned target = 0;     // items wanted in all
-    unsigned rows = 8;       // query rows (token, head) of an item
+struct AttnPlan {
+    unsigned grid = 0;        // CTAs
+    unsigned max_ranges = 0;  // ranges the workspace holds partial results for
+    unsigned rows = 4;        // query rows (token, head) of a unit
+    bool fits = true;         // the line's places fit 32 bits
 };
 
 // ---- the schedule ---------------------------------------------------------------------------------------------------
-// An item is a chunk of the keys for up to 8 (or 16) query rows of one KV head. The lengths are on the device, so every
-// CTA counts the tiles itself, takes the chunk that gives about `target` items in all, and finds its items by
-// their prefix sums. A request outside the stated bounds has no items.
+// A unit is a group of up to 4 or 8 query rows of one KV head; its work is the tiles of keys that they see. All units' tiles
+// lie in one line, a unit's kUnitCost and its tiles behind the unit before it, and the line is cut into ranges of equal
+// length, one a CTA (several, when a range would pass kMaxRange): every CTA has the same to do whatever the requests'
+// lengths, and at most two of a range's pieces are parts of a unit: one that an earlier range began (its
+// partial result goes to slot 0 of the range) and one that a later range goes on with (slot 1). The lengths are on the
+// device, so every CTA counts the line itself. A request outside the stated bounds has no units.
 struct Request {
     unsigned start = 0, fresh = 0, len = 0, groups = 0, span = 0;  // span: tiles that a group of rows sees at most
 };
@@ -73,66 +78,53 @@ __device__ __forceinline__ Request request_of(const Kv4AttnArgs &a, unsigned r, 
 }
 
 struct Schedule {
-    unsigned chunk = 0, total = 0;  // tiles of an item; items
+    unsigned line = 0;  // its length
+    unsigned range = 0, ranges = 0;
 };
 
-__device__ __forceinline__ unsigned splits_of(const Request &q, unsigned chunk) {
-    const unsigned n = (q.span + chunk - 1) / chunk;
-    return n ? n : 1;
-}
+__device__ __forceinline__ unsigned line_of(const Kv4AttnArgs &a, const Request &q) { return q.groups * a.c.n_kv * (q.span + kUnitCost); }
 
-// prefix[r]: items before request r (n_req + 1 entries), units[r]: groups of rows x KV heads before it (or null)
-__device__ Schedule make_schedule(const Kv4AttnArgs &a, const Plan &plan, unsigned *prefix, unsigned *units) {
-    __shared__ unsigned long long tiles_in[kWarps];
-    __shared__ unsigned items_in[kWarps], units_in[kWarps];
+// before[r]: the line's length before request r (n_req + 1 entries)
+__device__ Schedule make_schedule(const Kv4AttnArgs &a, const AttnPlan &plan, unsigned *before) {
+    __shared__ unsigned line_in[kWarps], broken_in[kWarps];
     const unsigned tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, per = (a.n_req + kThreads - 1) / kThreads;
     const unsigned r0 = tid * per < a.n_req ? tid * per : a.n_req, r1 = r0 + per < a.n_req ? r0 + per : a.n_req;
-    unsigned long long tiles = 0;
-    for (unsigned r = r0; r < r1; ++r) {
-        const Request q = request_of(a, r, plan.rows, blockIdx.x == 0);
-        tiles += (unsigned long long)q.groups * q.span;
-    }
-    for (unsigned o = 16; o; o >>= 1) tiles += __shfl_xor_sync(~0u, tiles, o);
-    if (lane == 0) tiles_in[warp] = tiles;
+    unsigned broken = a.n_req;  // the first request whose rows run backwards: no rows are counted twice before it
+    for (unsigned r = r1; r > r0; --r)
+        if (a.q_start[r - 1] > a.q_start[r]) broken = r - 1;
+    broken = __reduce_min_sync(~0u, broken);
+    if (lane == 0) broken_in[warp] = broken;
     __syncthreads();
-    tiles = 0;
-    for (unsigned w = 0; w < kWarps; ++w) tiles += tiles_in[w];
-    const unsigned long long even = (tiles * a.c.n_kv + plan.target - 1) / plan.target;
-    Schedule s;
-    s.chunk = even >= kMaxChunkTiles ? kMaxChunkTiles : (unsigned(even) + kWarps - 1) / kWarps * kWarps;
-    if (s.chunk < kWarps) s.chunk = kWarps;
-    unsigned items = 0, un = 0;
+    for (unsigned w = 0; w < kWarps; ++w) broken = broken_in[w] < broken ? broken_in[w] : broken;
+    unsigned line = 0;
     for (unsigned r = r0; r < r1; ++r) {
-        const Request q = request_of(a, r, plan.rows, false);
-        items += q.groups * splits_of(q, s.chunk) * a.c.n_kv;
-        un += q.groups * a.c.n_kv;
+        before[r] = line;
+        if (r < broken) line += line_of(a, request_of(a, r, plan.rows, blockIdx.x == 0));
+        else if (blockIdx.x == 0) tell(a.status, kServeRequest);
     }
-    unsigned is = items, us = un;
+    unsigned ls = line;
     for (unsigned o = 1; o < 32; o <<= 1) {
-        const unsigned x = __shfl_up_sync(~0u, is, o), y = __shfl_up_sync(~0u, us, o);
-        if (lane >= o) is += x, us += y;
+        const unsigned x = __shfl_up_sync(~0u, ls, o);
+        if (lane >= o) ls += x;
     }
-    if (lane == 31) items_in[warp] = is, units_in[warp] = us;
+    if (lane == 31) line_in[warp] = ls;
     __syncthreads();
-    is -= items, us -= un;
-    for (unsigned w = 0; w < warp; ++w) is += items_in[w], us += units_in[w];
-    for (unsigned r = r0; r < r1; ++r) {
-        const Request q = request_of(a, r, plan.rows, false);
-        prefix[r] = is;
-        if (units) units[r] = us;
-        is += q.groups * splits_of(q, s.chunk) * a.c.n_kv;
-        us += q.groups * a.c.n_kv;
-        if (r == a.n_req - 1) {
-            prefix[a.n_req] = is;
-            if (units) units[a.n_req] = us;
-        }
+    Schedule s;
+    ls -= line;
+    for (unsigned w = 0; w < kWarps; ++w) {
+        if (w < warp) ls += line_in[w];
+        s.line += line_in[w];
     }
+    for (unsigned r = r0; r < r1; ++r) before[r] += ls;
+    if (tid == 0) before[a.n_req] = s.line;
+    const unsigned each = (s.line + plan.grid - 1) / plan.grid, turns = (each + kMaxRange - 1) / kMaxRange;
+    s.range = turns ? ((each + turns - 1) / turns + kWarps - 1) / kWarps * kWarps : kWarps;
+    s.ranges = (s.line + s.range - 1) / s.range;
     __syncthreads();
-    s.total = prefix[a.n_req];
     return s;
 }
 
-__device__ __forceinline__ unsigned find(const unsigned *prefix, unsigned n, unsigned i) {
+__device__ __forceinline__ unsigned find(const unsigned *prefix, unsigned n, unsigned i) {  // the last of n with prefix[.] <= i
     unsigned lo = 0, hi = n;
     while (hi - lo > 1) {
         const unsigned mid = (lo + hi) / 2;
@@ -160,19 +152,35 @@ __device__ __forceinline__ GroupSpan span_of(const Kv4AttnArgs &a, const Request
     return s;
 }
 
+// The workspace: the pieces' outputs, their maxima and sums (two slots a range), and for every range what its edge to the
+// range before it cuts.
+struct Edge {
+    unsigned n = 0;            // pieces of the unit that the edge cuts (0: it cuts none), in the ranges first, first + 1, ...
+    unsigned first = 0, slot0 = 0;  // piece 0 lies in slot slot0 of range `first`, the others in slot 0 of theirs
+    unsigned rows = 0;         // rows of the unit
+    unsigned row0 = 0, head = 0;  // the unit's first (token, head of the group) row of the request, its KV head
+    unsigned start = 0;        // the request's first row
+    unsigned ranges = 0;       // entry 0 alone: how many there are
+};
+struct Room {
+    float *part;
+    float2 *stat;
+    Edge *edge;
+};
+__host__ __device__ inline Room room_of(uint8_t *room, const AttnPlan &plan, unsigned dim) {
+    Room r;
+    const size_t slots = size_t(plan.max_ranges) * 2 * plan.rows;
+    r.part = reinterpret_cast<float *>(room);
+    r.stat = reinterpret_cast<float2 *>(r.part + slots * dim);
+    r.edge = reinterpret_cast<Edge *>(r.stat + slots);
+    return r;
+}
+
 // ---- the tile product -----------------------------------------------------------------------------------------------
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
-}
-// two FP32 multiply-adds in one instruction
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    float2 d;
-    asm("{\n .reg .b64 x, y, z, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n fma.rn.f32x2 w, x, y, z;\n mov.b64 {%0, %1}, w;\n}"
-        : "=f"(d.x), "=f"(d.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-    return d;
 }
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
@@ -227,6 +235,18 @@ __device__ __forceinline__ void load_words(uint32_t *w, const uint8_t *at) {
         for (int i = 0; i < N; ++i) w[i] = *reinterpret_cast<const uint32_t *>(at + 4 * i);
     }
 }
+template <int N>  // N halves, 2 N bytes aligned (N odd: 2)
+__device__ __forceinline__ void load_halves(uint32_t *w, const uint8_t *at) {
+    if constexpr (N % 2 == 0) {
+        load_words<N / 2>(w, at);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            w[i / 2] = *reinterpret_cast<const uint16_t *>(at + 2 * i);
+            if (i + 1 < N) w[i / 2] |= uint32_t(*reinterpret_cast<const uint16_t *>(at + 2 * i + 2)) << 16;
+        }
+    }
+}
 // halves i and j of an array of words as a pair
 __device__ __forceinline__ half2 pair_at(const uint32_t *w, int i, int j) {
     return as_h2(__byte_perm(w[i >> 1], w[j >> 1], (i & 1 ? 0x32u : 0x10u) | (j & 1 ? 0x7600u : 0x5400u)));
@@ -236,30 +256,49 @@ __device__ __forceinline__ float half_at(const uint32_t *w, int i) {
     return __half2float(__ushort_as_half(uint16_t(i & 1 ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu)));
 }
 
-template <int NB, int MT>
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {  // an 8 x 8 matrix of halves, two columns of row lane / 4 a lane
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+// NB: 32-dim blocks of a head; NT: sets of four query rows.
+template <int NB, int NT>
 struct Shape {
     static constexpr int kTile = NB * 576;                       // bytes of a tile
-    static constexpr int kSlots = NB <= 2 ? 8 : NB <= 4 ? 6 : 4;  // tiles a warp has on their way
-    static constexpr bool kQInRegs = NB * MT <= 4;
-    static constexpr int kQBytes = kQInRegs ? 0 : MT * NB * 3 * 32 * 16;  // per block: two k-steps of q, and the sums' start
-    static constexpr int kOutBytes = kWarps * MT * 8 * (NB * 32 + 2) * 4;  // the warps' results, in the ring's place
+    #ifndef TS
+#define TS 3
+#define TQ 4
+#define TC 3
+#endif
+    static constexpr int kSlots = NB <= 2 ? 8 : NB <= 4 ? TS * 2 : TS;  // tiles a warp has on their way
+    static constexpr int kRows = NT * 4;
+    static constexpr int kCtas = NB * NT <= 8 ? TC : 2;           // on an SM, by the accumulators' registers (8 NB NT a thread)
+    static constexpr bool kQInRegs = NB * NT <= TQ;
+    static constexpr int kQBytes = kQInRegs ? 0 : NT * NB * 2 * 32 * 8;
+    static constexpr int kOutBytes = kWarps * kRows * NB * 32 * 4;  // the warps' results
     static constexpr int kRing = kWarps * kSlots * kTile;
-    static constexpr int kSmem = kQBytes + (kRing > kOutBytes ? kRing : kOutBytes);
+    static constexpr int kSmem = kQBytes + kOutBytes + kRing;
 };
 
+// The matrix instructions are 16 x 8 x 16 with the codes as A (16 keys by dims, then 16 dims by keys) and the FP32 factor as
+// B: four query rows, an upper and a lower column each. Lane (g, t) = (lane / 4, lane % 4) then holds the scores of the keys
+// g and g + 8 for row t, and of the output the dims g and g + 8 of a set for row t.
+//
 // A warp takes every fourth tile of its CTA's chunk, with a running maximum, sum and output of its own; it fetches its
-// tiles itself (one bulk copy each), so that nothing in the loop waits for another warp. Lane (g, t) = (lane / 4, lane % 4).
-template <int NB, int MT>
-__global__ void __launch_bounds__(kThreads) kv4_attn_kernel(const Kv4AttnArgs a, const Plan plan) {
-    using S = Shape<NB, MT>;
+// tiles itself (one bulk copy each), so that nothing in the loop waits for another warp.
+template <int NB, int NT>
+__global__ void __launch_bounds__(kThreads, Shape<NB, NT>::kCtas) kv4_attn_kernel(const Kv4AttnArgs a, const AttnPlan plan) {
+    using S = Shape<NB, NT>;
     constexpr int kPlanes = (NB + 3) / 4, D = NB * 32;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint64_t bars[kWarps][S::kSlots];
-    __shared__ float m_of[kWarps][MT * 8], l_of[kWarps][MT * 8];
-    unsigned *prefix = reinterpret_cast<unsigned *>(smem + S::kSmem);
+    __shared__ float m_of[kWarps][S::kRows], l_of[kWarps][S::kRows];
+    auto *before = reinterpret_cast<unsigned *>(smem + S::kSmem);
     const unsigned tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const unsigned per = a.n_head / a.c.n_kv, tiles_per_page = a.c.page / kTileTokens;
-    uint8_t *ring = smem + S::kQBytes + warp * S::kSlots * S::kTile;
+    float *out = reinterpret_cast<float *>(smem + S::kQBytes);
+    uint8_t *ring = smem + S::kQBytes + S::kOutBytes + warp * S::kSlots * S::kTile;
     if (tid == 0) {
         for (unsigned w = 0; w < kWarps; ++w)
             for (int i = 0; i < S::kSlots; ++i) mbar_init(&bars[w][i], 1);
@@ -267,84 +306,140 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(const Kv4AttnArgs a,
     }
     pdl_wait();
     pdl_launch_dependents();
-    const Schedule sched = make_schedule(a, plan, prefix, nullptr);  // its barriers also cover the mbarriers' start
-    unsigned done = 0;  // tiles this warp has taken from its ring so far (slot and phase go by it)
-    bool late = false;
+    const Schedule sched = make_schedule(a, plan, before);  // its barriers also cover the mbarriers' start
+    const Room room = room_of(a.room, plan, D);
+    const size_t page_bytes = size_t(a.c.n_kv) * tiles_per_page * S::kTile;
+    if (sched.ranges == 0 && blockIdx.x == 0 && tid == 0) room.edge[0] = Edge{};
 
-    for (unsigned item = blockIdx.x; item < sched.total; item += gridDim.x) {
-        const unsigned r = find(prefix, a.n_req, item);
-        const Request rq = request_of(a, r, plan.rows, false);
-        unsigned in = item - prefix[r];
-        const unsigned head = in % a.c.n_kv;
-        in /= a.c.n_kv;
-        const unsigned group = in % rq.groups, split = in / rq.groups;
-        const GroupSpan sp = span_of(a, rq, group, plan.rows);
-        const unsigned n_split = (sp.tiles + sched.chunk - 1) / sched.chunk;
-        if (split && split >= n_split) continue;
-        const unsigned t0 = split * sched.chunk, t1 = t0 + sched.chunk < sp.tiles ? t0 + sched.chunk : sp.tiles;
-        const unsigned mine = t0 + warp < t1 ? (t1 - t0 - warp + kWarps - 1) / kWarps : 0;  // tiles of this warp
-        const uint32_t *table = a.table + size_t(r) * a.stride;
-        const uint8_t *head_base = a.c.base + size_t(head) * tiles_per_page * S::kTile;
-        const size_t page_bytes = size_t(a.c.n_kv) * tiles_per_page * S::kTile;
-
-        // the k-th tile of this warp: lane k % 32 keeps where it lies
-        const uint8_t *where = nullptr;
-        auto look_up = [&](unsigned k) {
-            where = nullptr;
-            if (k < mine) {
-                const unsigned tile = sp.tile0 + t0 + warp + k * kWarps, page = table[tile / tiles_per_page];
-                if (page < a.c.n_pages) where = head_base + page * page_bytes + size_t(tile % tiles_per_page) * S::kTile;
-                else tell(a.status, kServePage);
+    // The pieces of this CTA's ranges, one after another.
+    struct Piece {
+        unsigned start, all, row0, head;  // the request's first row; its rows; the unit's first row, its KV head
+        int base;                         // the position of the request's first new token
+        unsigned tile0, mine;             // this warp's first tile, and how many (each kWarps behind the one before)
+        unsigned table;                   // the request's row of the table
+        unsigned slot;                    // of its result in the workspace; kNoSlot: the piece is a whole unit
+    };
+    unsigned range = blockIdx.x, at_line = range * sched.range, req = 0;
+    bool fresh_range = true;
+    auto next_piece = [&](Piece &p) {
+        while (range < sched.ranges) {
+            const unsigned from = range * sched.range, to = sched.line - from < sched.range ? sched.line : from + sched.range;
+            if (at_line >= to) {
+                range += gridDim.x;
+                at_line = range * sched.range;
+                fresh_range = true;
+                continue;
             }
-        };
-        auto fetch = [&](unsigned k) {  // where: of k's 32 tiles
-            const uint8_t *src = reinterpret_cast<const uint8_t *>(__shfl_sync(~0u, (unsigned long long)where, k % 32));
-            const unsigned slot = (done + k) % S::kSlots;
-            if (lane == 0) {
-                if (src) {
-                    mbar_expect_tx(&bars[warp][slot], S::kTile);
-                    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                                     smem_addr(ring + slot * S::kTile)),
-                                 "l"(src), "r"(S::kTile), "r"(smem_addr(&bars[warp][slot]))
-                                 : "memory");
-                } else {
-                    mbar_expect_tx(&bars[warp][slot], 0);  // no page: the slot's phase ends at once
+            if (fresh_range) req = find(before, a.n_req, from);
+            while (before[req + 1] <= at_line) ++req;
+            const Request rq = request_of(a, req, plan.rows, false);
+            const unsigned length = rq.span + kUnitCost, unit = (at_line - before[req]) / length, begin = before[req] + unit * length;
+            const unsigned u0 = at_line - begin, u1 = (to - begin < length ? to - begin : length);
+            const GroupSpan sp = span_of(a, rq, unit / a.c.n_kv, plan.rows);
+            p.head = unit % a.c.n_kv;
+            p.row0 = unit / a.c.n_kv * plan.rows;
+            p.all = rq.fresh * per;
+            p.start = rq.start;
+            p.base = int(rq.len) - int(rq.fresh);
+            p.table = req;
+            const unsigned t0 = u0 > kUnitCost ? u0 - kUnitCost : 0, end = u1 > kUnitCost ? u1 - kUnitCost : 0, t1 = end < sp.tiles ? end : sp.tiles;
+            const bool whole = t0 == 0 && t1 == sp.tiles;
+            if (fresh_range && tid == 0) {  // what this range's edge cuts: for the merge
+                Edge e;
+                const unsigned first = (begin + kUnitCost) / sched.range;
+                unsigned last = sp.tiles ? (begin + kUnitCost + sp.tiles - 1) / sched.range : first;
+                if (last >= sched.ranges) last = sched.ranges - 1;
+                if (begin < from && first < range && range <= last) {
+                    e.n = last - first + 1;
+                    e.first = first;
+                    e.slot0 = begin >= first * sched.range;
+                    e.rows = p.all - p.row0 < plan.rows ? p.all - p.row0 : plan.rows;
+                    e.row0 = p.row0;
+                    e.head = p.head;
+                    e.start = p.start;
                 }
+                if (range == 0) e.ranges = sched.ranges;
+                room.edge[range] = e;
             }
-            return src != nullptr;
-        };
-        unsigned present = 0;  // bit s: slot s holds a tile
-        look_up(lane);
-        unsigned ahead = 0;
-        for (; ahead < unsigned(S::kSlots) && ahead < mine; ++ahead) {
-            const unsigned slot = (done + ahead) % S::kSlots;
-            present = fetch(ahead) ? present | 1u << slot : present & ~(1u << slot);
+            fresh_range = false;
+            at_line = begin + length;
+            if (sp.tiles == 0 ? u0 != 0 : t0 >= t1) continue;  // (a unit that sees nothing belongs to the range with its first place)
+            p.tile0 = sp.tile0 + t0 + warp;
+            p.mine = t0 + warp < t1 ? (t1 - t0 - warp + kWarps - 1) / kWarps : 0;
+            p.slot = whole ? kNoSlot : range * 2 + (begin >= from);
+            return true;
         }
+        return false;
+    };
 
-        // the rows' queries: split, in the order in which a block's words hold the dims
-        uint32_t qa[S::kQInRegs ? MT : 1][S::kQInRegs ? NB * 2 : 1][4];
-        float start[S::kQInRegs ? MT : 1][S::kQInRegs ? NB : 1][4];  // -8 sum q over a block, of the rows' upper and lower parts
-        float scale[MT];
-        int pos[MT], low[MT];  // the keys a row sees: [low, pos]
-        const unsigned all = rq.fresh * per, row0 = group * plan.rows;
+    // A warp's tiles: the k-th lies where lane k % 32 keeps.
+    Piece pc;
+    unsigned done = 0;     // tiles this warp has taken from its ring before this piece (slot and phase go by it)
+    unsigned ahead = 0;    // of the piece's tiles, fetched
+    unsigned present = 0;  // bit s: slot s holds a tile
+    const uint8_t *where = nullptr;
+    bool late = false;
+    auto look_up = [&](unsigned k) {
+        where = nullptr;
+        if (k < pc.mine) {
+            const unsigned tile = pc.tile0 + k * kWarps, page = a.table[size_t(pc.table) * a.stride + tile / tiles_per_page];
+            if (page < a.c.n_pages) where = a.c.base + page * page_bytes + size_t(pc.head * tiles_per_page + tile % tiles_per_page) * S::kTile;
+            else tell(a.status, kServePage);
+        }
+    };
+    auto fetch = [&](unsigned k) {
+        const uint8_t *src = reinterpret_cast<const uint8_t *>(__shfl_sync(~0u, (unsigned long long)where, k % 32));
+        const unsigned slot = (done + k) % S::kSlots;
+        if (lane == 0) {
+            if (src) {
+                mbar_expect_tx(&bars[warp][slot], S::kTile);
+                asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                                 smem_addr(ring + slot * S::kTile)),
+                             "l"(src), "r"(S::kTile), "r"(smem_addr(&bars[warp][slot]))
+                             : "memory");
+            } else {
+                mbar_expect_tx(&bars[warp][slot], 0);  // no page: the slot's phase ends at once
+            }
+        }
+        present = src ? present | 1u << slot : present & ~(1u << slot);
+    };
+    auto begin_piece = [&] {
+        look_up(lane);
+        for (ahead = 0; ahead < unsigned(S::kSlots) && ahead < pc.mine; ++ahead) fetch(ahead);
+    };
+
+    bool more = next_piece(pc);
+    if (more) begin_piece();
+    while (more) {
+        // The queries as B operands, in the order in which a block's words hold the dims: column g is the upper (g even) or
+        // lower part of row g / 2.
+        uint32_t qb[S::kQInRegs ? NT : 1][S::kQInRegs ? NB * 2 : 1][2];
+        float start[NT][NB];    // -8 sum q over a block, of row t
+        float scale[NT];        // of row t
+        int pos[NT], low[NT];   // the keys row t sees: [low, pos]
+        int wpos[NT], wlow[NT]; // and row g / 2
+        const unsigned all = pc.all, row0 = pc.row0, head = pc.head, mine = pc.mine;
+        const int base = pc.base;
+        const bool wide = ((reinterpret_cast<uintptr_t>(a.q) | a.q_stride * 4 | a.q_head_stride * 4) & 15) == 0;
+        auto sees = [&](unsigned row, int &lo, int &hi) {
+            const int p = base + int(row / per);
+            hi = row < all ? p : -1;
+            lo = a.window && p >= 0 && unsigned(p) + 1 > a.window ? p + 1 - int(a.window) : 0;
+        };
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            const unsigned row = row0 + m * 8 + g;
-            const bool real = row < all;
-            const float *src = a.q + (rq.start + (real ? row / per : 0)) * a.q_stride + (head * per + (real ? row % per : 0)) * a.q_head_stride;
-            const long long p = (long long)rq.len - rq.fresh + row / per;
-            pos[m] = real ? int(p) : -1;
-            low[m] = a.window && p + 1 > (long long)a.window ? int(p + 1 - a.window) : 0;
+        for (int m = 0; m < NT; ++m) {
+            sees(row0 + m * 4 + t, low[m], pos[m]);
+            sees(row0 + m * 4 + g / 2, wlow[m], wpos[m]);
+            const unsigned row = row0 + m * 4 + g / 2 < all ? row0 + m * 4 + g / 2 : row0;
+            const float *src = a.q + (pc.start + row / per) * a.q_stride + (head * per + row % per) * a.q_head_stride + t * 4;
             float x[NB * 2][4], top = 0.0f;
-            const bool wide = ((reinterpret_cast<uintptr_t>(a.q) | a.q_stride * 4 | a.q_head_stride * 4) & 15) == 0;
 #pragma unroll
             for (int i = 0; i < NB * 2; ++i) {
-                const float *at = src + i * 16 + t * 4;
                 if (wide) {
-                    const float4 v = *reinterpret_cast<const float4 *>(at);
+                    const float4 v = *reinterpret_cast<const float4 *>(src + i * 16);
                     x[i][0] = v.x, x[i][1] = v.y, x[i][2] = v.z, x[i][3] = v.w;
                 } else {
-                    for (int e = 0; e < 4; ++e) x[i][e] = at[e];
+                    for (int e = 0; e < 4; ++e) x[i][e] = src[i * 16 + e];
                 }
             }
 #pragma unroll
@@ -357,163 +452,167 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(const Kv4AttnArgs a,
             ex = ex < -110 ? -110 : ex > 100 ? 100 : ex;
             const float down = __uint_as_float(unsigned(127 - ex) << 23);
             scale[m] = a.scale * kLog2e * __uint_as_float(unsigned(127 + 24 + ex) << 23);  // (K's codes come times 2^-24)
+            scale[m] = __shfl_sync(~0u, scale[m], t * 8);
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                float hi = 0.0f, lo = 0.0f;
+                float sum_q = 0.0f;
 #pragma unroll
                 for (int i = 2 * b; i < 2 * b + 2; ++i) {
                     const float f = i & 1 ? down * 0.0625f : down;  // the high nibbles' codes come times 16
-                    uint32_t v[4];
-                    split2(x[i][0] * f, x[i][2] * f, v[0], v[1]);
-                    split2(x[i][1] * f, x[i][3] * f, v[2], v[3]);
-                    const float2 s0 = __half22float2(as_h2(v[0])), s1 = __half22float2(as_h2(v[1])), s2 = __half22float2(as_h2(v[2])),
-                                 s3 = __half22float2(as_h2(v[3]));
-                    const float up = i & 1 ? 16.0f : 1.0f;
-                    hi += up * ((s0.x + s0.y) + (s2.x + s2.y));
-                    lo += up * ((s1.x + s1.y) + (s3.x + s3.y));
-                    if constexpr (S::kQInRegs) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) qa[m][i][e] = v[e];
-                    } else {
-                        if (warp == 0) *reinterpret_cast<uint4 *>(smem + ((m * NB * 3 + i) * 32 + lane) * 16) = make_uint4(v[0], v[1], v[2], v[3]);
-                    }
+                    uint32_t h0, l0, h1, l1;
+                    split2(x[i][0] * f, x[i][2] * f, h0, l0);
+                    split2(x[i][1] * f, x[i][3] * f, h1, l1);
+                    const float2 s0 = __half22float2(as_h2(h0)), s1 = __half22float2(as_h2(l0)), s2 = __half22float2(as_h2(h1)),
+                                 s3 = __half22float2(as_h2(l1));
+                    sum_q += (i & 1 ? 16.0f : 1.0f) * (((s0.x + s0.y) + (s2.x + s2.y)) + ((s1.x + s1.y) + (s3.x + s3.y)) * (1.0f / 2048));
+                    const uint2 mine_q = make_uint2(g & 1 ? l0 : h0, g & 1 ? l1 : h1);
+                    if constexpr (S::kQInRegs) qb[m][i][0] = mine_q.x, qb[m][i][1] = mine_q.y;
+                    else if (warp == 0) *reinterpret_cast<uint2 *>(smem + ((m * NB * 2 + i) * 32 + lane) * 8) = mine_q;
                 }
-                hi += __shfl_xor_sync(~0u, hi, 1);
-                lo += __shfl_xor_sync(~0u, lo, 1);
-                hi = -0x1p-21f * (hi + __shfl_xor_sync(~0u, hi, 2));
-                lo = -0x1p-21f * (lo + __shfl_xor_sync(~0u, lo, 2));
-                if constexpr (S::kQInRegs) {
-                    start[m][b][0] = start[m][b][1] = hi;
-                    start[m][b][2] = start[m][b][3] = lo;
-                } else {
-                    if (warp == 0) *reinterpret_cast<float4 *>(smem + ((m * NB * 3 + NB * 2 + b) * 32 + lane) * 16) = make_float4(hi, hi, lo, lo);
-                }
+                sum_q += __shfl_xor_sync(~0u, sum_q, 1);
+                sum_q = -0x1p-21f * (sum_q + __shfl_xor_sync(~0u, sum_q, 2));
+                start[m][b] = __shfl_sync(~0u, sum_q, t * 8);
             }
         }
+
         if constexpr (!S::kQInRegs) __syncthreads();
 
-        float o[MT][NB * 4][4], top[MT], sum[MT], limit = 0.0f, lift = 1.0f, lift_d = 1.0f;
+        float o[NT][NB * 2][4], top[NT], sum[NT], limit = 0.0f, lift = 1.0f, lift_d = 1.0f;
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
+        for (int m = 0; m < NT; ++m) {
             top[m] = -INFINITY;
             sum[m] = 0.0f;
 #pragma unroll
-            for (int i = 0; i < NB * 4; ++i)
+            for (int i = 0; i < NB * 2; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[m][i][e] = 0.0f;
         }
 
         // Keys that every row of the group sees need no masks.
-        const long long all_low = a.window ? (long long)rq.len - rq.fresh + (row0 + plan.rows < all ? row0 + plan.rows - 1 : all - 1) / per + 1 - a.window : 0;
-        const long long all_high = (long long)rq.len - rq.fresh + row0 / per;
+        const int last_row = base + int((row0 + plan.rows < all ? row0 + plan.rows - 1 : all - 1) / per);
+        const int all_low = a.window && last_row >= 0 && unsigned(last_row) + 1 > a.window ? last_row + 1 - int(a.window) : 0;
+        const int all_high = base + int(row0 / per);
+        auto edge = [&](int key0) { return key0 < all_low || key0 + int(kTileTokens) - 1 > all_high; };
 
-        auto take = [&](const uint8_t *tile, int key0, auto masked) {
-            constexpr bool kMasked = decltype(masked)::value;
-            // scores of the tile's keys 8 j + 2 t + i
-            float2 s[MT][2];
+        // the scores of row t and the tile's keys g, g + 8
+        auto score = [&](const uint8_t *tile, float (&s)[NT][2]) {
+            constexpr float kZero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                uint32_t ds[NB];
-                load_words<NB>(ds, tile + NB * 512 + (4 * j + t) * NB * 4);
+            for (int m = 0; m < NT; ++m) s[m][0] = s[m][1] = 0.0f;
+            {
+                uint32_t ds[2][(NB + 1) / 2];
 #pragma unroll
-                for (int m = 0; m < MT; ++m) s[m][j] = make_float2(0.0f, 0.0f);
+                for (int j = 0; j < 2; ++j) load_halves<NB>(ds[j], tile + NB * 512 + (g + 8 * j) * NB * 2);
 #pragma unroll
                 for (int p = 0; p < kPlanes; ++p) {
                     const int nbp = NB - 4 * p < 4 ? NB - 4 * p : 4;
-                    uint32_t w[4];
-                    const uint8_t *at = tile + p * 1024 + ((8 * j + g) * 4 + t) * nbp * 4;
-                    if (nbp == 4) load_words<4>(w, at);
-                    if (nbp == 3) load_words<3>(w, at);
-                    if (nbp == 2) load_words<2>(w, at);
-                    if (nbp == 1) load_words<1>(w, at);
+                    uint32_t w[2][4];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const uint8_t *at = tile + p * 1024 + ((8 * j + g) * 4 + t) * nbp * 4;
+                        if (nbp == 4) load_words<4>(w[j], at);
+                        if (nbp == 3) load_words<3>(w[j], at);
+                        if (nbp == 2) load_words<2>(w[j], at);
+                        if (nbp == 1) load_words<1>(w[j], at);
+                    }
 #pragma unroll
                     for (int b = 0; b < 4; ++b) {
                         if (b >= nbp) break;
                         const int bb = 4 * p + b;
-                        const uint32_t x8 = w[b] >> 8;
-                        const float2 d = make_float2(half_at(ds, bb), half_at(ds, NB + bb));
+                        const uint32_t w8[2] = {w[0][b] >> 8, w[1][b] >> 8};
+                        const uint32_t lo[4] = {low_raw(w[0][b]), low_raw(w[1][b]), low_raw(w8[0]), low_raw(w8[1])};
+                        const uint32_t hi[4] = {high_raw(w[0][b]), high_raw(w[1][b]), high_raw(w8[0]), high_raw(w8[1])};
+                        const float d0 = half_at(ds[0], bb), d1 = half_at(ds[1], bb);
 #pragma unroll
-                        for (int m = 0; m < MT; ++m) {
+                        for (int m = 0; m < NT; ++m) {
                             float c[4], e[4];
-                            uint32_t q0[4], q1[4];
+                            uint2 q0, q1;
                             if constexpr (S::kQInRegs) {
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) q0[i] = qa[m][bb * 2][i], q1[i] = qa[m][bb * 2 + 1][i], c[i] = start[m][bb][i];
+                                q0 = make_uint2(qb[m][bb * 2][0], qb[m][bb * 2][1]);
+                                q1 = make_uint2(qb[m][bb * 2 + 1][0], qb[m][bb * 2 + 1][1]);
                             } else {
-                                load_words<4>(q0, smem + ((m * NB * 3 + bb * 2) * 32 + lane) * 16);
-                                load_words<4>(q1, smem + ((m * NB * 3 + bb * 2 + 1) * 32 + lane) * 16);
-                                load_words<4>(reinterpret_cast<uint32_t *>(c), smem + ((m * NB * 3 + NB * 2 + bb) * 32 + lane) * 16);
+                                q0 = *reinterpret_cast<const uint2 *>(smem + ((m * NB * 2 + bb * 2) * 32 + lane) * 8);
+                                q1 = *reinterpret_cast<const uint2 *>(smem + ((m * NB * 2 + bb * 2 + 1) * 32 + lane) * 8);
                             }
-                            mma16816(e, q0, low_raw(w[b]), low_raw(x8), c);
-                            mma16816(c, q1, high_raw(w[b]), high_raw(x8), e);
-                            const float2 both = fma2(make_float2(c[2], c[3]), make_float2(1.0f / 2048, 1.0f / 2048), make_float2(c[0], c[1]));
-                            s[m][j] = fma2(d, both, s[m][j]);
+                            mma16816(e, lo, q0.x, q0.y, kZero);
+                            mma16816(c, hi, q1.x, q1.y, e);
+                            s[m][0] += d0 * ((c[0] + start[m][bb]) + c[1] * (1.0f / 2048));
+                            s[m][1] += d1 * ((c[2] + start[m][bb]) + c[3] * (1.0f / 2048));
                         }
                     }
                 }
             }
-            // The running maximum. It moves only when a score passes it, and then to 4 (in powers of two) above the largest, so
-            // that it moves seldom; the weights stay below 1.
-            float2 pr[MT][2];
-            uint32_t seen[MT][2];  // of a pair of keys, as a mask of halves
+        };
+        // Scores to weights. The running maximum moves only when a score passes it, and then to 4 (in powers of two) above the
+        // largest, so that it moves seldom; the weights stay below 1.
+        auto weigh = [&](int key0, float (&s)[NT][2]) {
+            const bool some = edge(key0);
 #pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                float mx = -INFINITY;
+            for (int m = 0; m < NT; ++m) {
+                s[m][0] *= scale[m];
+                s[m][1] *= scale[m];
+                if (some) {
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const int key = key0 + 8 * j + 2 * int(t);
-                    s[m][j].x *= scale[m];
-                    s[m][j].y *= scale[m];
-                    if (kMasked) {
-                        const bool x = key >= low[m] && key <= pos[m], y = key + 1 >= low[m] && key + 1 <= pos[m];
-                        seen[m][j] = (x ? 0x0000ffffu : 0u) | (y ? 0xffff0000u : 0u);
-                        if (!x) s[m][j].x = -INFINITY;
-                        if (!y) s[m][j].y = -INFINITY;
+                    for (int j = 0; j < 2; ++j) {
+                        const int key = key0 + 8 * j + int(g);
+                        if (key < low[m] || key > pos[m]) s[m][j] = -INFINITY;
                     }
-                    mx = fmaxf(mx, fmaxf(s[m][j].x, s[m][j].y));
                 }
-                mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 1));
-                mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 2));
+                float mx = fmaxf(s[m][0], s[m][1]);
                 if (__any_sync(~0u, mx > top[m])) {
+#pragma unroll
+                    for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, x));
                     const float nt = mx > top[m] ? mx + 4.0f : top[m];
                     const float f = top[m] == nt ? 1.0f : exp2_fast(top[m] - nt);  // top -inf: 0
                     sum[m] *= f;
 #pragma unroll
-                    for (int i = 0; i < NB * 4; ++i)
+                    for (int i = 0; i < NB * 2; ++i)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) o[m][i][e] *= f;
                     top[m] = nt;
                 }
                 const float ref = top[m] == -INFINITY ? 0.0f : top[m];
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    pr[m][j] = make_float2(exp2_fast(s[m][j].x - ref), exp2_fast(s[m][j].y - ref));
-                    sum[m] += pr[m][j].x + pr[m][j].y;
-                }
+                s[m][0] = exp2_fast(s[m][0] - ref);
+                s[m][1] = exp2_fast(s[m][1] - ref);
+                sum[m] += s[m][0] + s[m][1];
             }
-            // the weighted sum of the values: keys along k, dims along n
-            uint32_t dv[2][NB];
-#pragma unroll
-            for (int j = 0; j < 2; ++j) load_words<NB>(dv[j], tile + NB * 544 + (4 * j + t) * NB * 4);
+        };
+        auto value = [&](const uint8_t *tile, int key0, const float (&s)[NT][2]) {
+            // The weighted sum of the values: dims by keys, keys by rows.
             // A weight p d is a product of FP16 pairs: with p = ph + pl, wh = fp16(ph d) and wl = fp16(pl d + (ph d - wh)),
             // where ph d - wh is exact in one FP16 multiply-add. p is lifted by a power of two that keeps the largest weight
             // below 2^14 (`limit`: a power of two that no scale seen so far passes), so that small values keep 22 bits too; scales
             // below 1/16 are lifted as well.
+            uint32_t dv[2][NB];    // the scales of the keys 2 t + 8 j and the one behind it
+            uint32_t seen[NT][2];  // these pairs of keys, by row g / 2, as masks of halves: a key that is not seen weighs nothing, whatever its scale holds
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                uint32_t raw[NB];
+                load_words<NB>(raw, tile + NB * 544 + (4 * j + t) * NB * 4);
+#pragma unroll
+                for (int b = 0; b < NB; ++b) dv[j][b] = h2(pair_at(raw, b, NB + b));
+#pragma unroll
+                for (int m = 0; m < NT; ++m) seen[m][j] = ~0u;
+            }
+            if (edge(key0)) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int key = key0 + 8 * j + 2 * int(t);
+                    uint32_t any = 0;
+#pragma unroll
+                    for (int m = 0; m < NT; ++m) {
+                        seen[m][j] = (key >= wlow[m] && key <= wpos[m] ? 0x0000ffffu : 0u) | (key + 1 >= wlow[m] && key + 1 <= wpos[m] ? 0xffff0000u : 0u);
+                        any |= seen[m][j];
+                    }
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) dv[j][b] &= any;
+                }
+            }
             half2 big2 = __float2half2_rn(0.0f);
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    if (kMasked) {
-                        uint32_t any = 0;
-#pragma unroll
-                        for (int m = 0; m < MT; ++m) any |= seen[m][j];
-                        const half2 d = pair_at(dv[j], b, NB + b);
-                        big2 = __hmax2(big2, __habs2(as_h2(h2(d) & any)));
-                    } else {
-                        big2 = __hmax2(big2, __habs2(as_h2(dv[j][b])));
-                    }
-                }
+                for (int b = 0; b < NB; ++b) big2 = __hmax2(big2, __habs2(as_h2(dv[j][b])));
             float big = fmaxf(__low2float(big2), __high2float(big2));
             if (__any_sync(~0u, big > limit)) {
 #pragma unroll
@@ -524,9 +623,9 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(const Kv4AttnArgs a,
                 lift = fminf(0x1p14f / (limit * lift_d), 0x1p15f);
                 const float f = lift * lift_d / was;
 #pragma unroll
-                for (int m = 0; m < MT; ++m)
+                for (int m = 0; m < NT; ++m)
 #pragma unroll
-                    for (int i = 0; i < NB * 4; ++i)
+                    for (int i = 0; i < NB * 2; ++i)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) o[m][i][e] *= f;
             }
@@ -537,17 +636,20 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(const Kv4AttnArgs a,
 #pragma unroll
                     for (int b = 0; b < NB; ++b) dv[j][b] = h2(__hmul2(as_h2(dv[j][b]), f));
             }
-            half2 ph[MT][2], pl[MT][2];
+            // Of row g / 2 and the keys 2 t + 8 j, + 1. A lane of an upper column wants ph d, one of a lower column the rest: with
+            // (x, y) = (0, ph) in the one and (ph, pl) in the other both are y d + (x d - fp16(x d)).
+            half2 wx[NT][2], wy[NT][2];
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
+            for (int m = 0; m < NT; ++m)
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    const float x = pr[m][j].x * lift, y = pr[m][j].y * lift;
-                    ph[m][j] = __floats2half2_rn(x, y);
-                    const float2 back = __half22float2(ph[m][j]);
-                    pl[m][j] = __floats2half2_rn(x - back.x, y - back.y);
+                    const float x = s[m][j] * lift;
+                    const half h = __float2half_rn(x);
+                    const uint32_t ph = transpose8(h2(__half2half2(h))), pl = transpose8(h2(__half2half2(__float2half_rn(x - __half2float(h)))));
+                    wx[m][j] = as_h2(g & 1 ? ph : 0u);
+                    wy[m][j] = as_h2(g & 1 ? pl : ph);
                 }
-            const uint32_t sel = (g >> 2) * 0x2222u + 0x4400u;  // byte 2 (g / 4) of two words, each twice
+            const uint32_t sel = (g & 1) * 0x2222u + 0x4400u;  // byte 2 (g % 2) of two words, each twice
 #pragma unroll
             for (int p = 0; p < kPlanes; ++p) {
                 const int nbp = NB - 4 * p < 4 ? NB - 4 * p : 4;
@@ -556,7 +658,7 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(const Kv4AttnArgs a,
                 for (int j = 0; j < 2; ++j)
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        const uint8_t *at = tile + NB * 256 + p * 1024 + (((j * 2 + i) * 4 + (g & 3)) * 4 + t) * nbp * 4;
+                        const uint8_t *at = tile + NB * 256 + p * 1024 + (((j * 2 + i) * 4 + (g >> 1)) * 4 + t) * nbp * 4;
                         if (nbp == 4) load_words<4>(v[j][i], at);
                         if (nbp == 3) load_words<3>(v[j][i], at);
                         if (nbp == 2) load_words<2>(v[j][i], at);
@@ -566,254 +668,266 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(const Kv4AttnArgs a,
                 for (int b = 0; b < 4; ++b) {
                     if (b >= nbp) break;
                     const int bb = 4 * p + b;
-                    uint32_t wa[MT][4];
+                    uint32_t w[NT][2];
 #pragma unroll
-                    for (int m = 0; m < MT; ++m)
+                    for (int j = 0; j < 2; ++j) {
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            uint32_t dd = h2(pair_at(dv[j], bb, NB + bb));
-                            if (kMasked) dd &= seen[m][j];  // a key that is not seen weighs nothing, whatever its scale holds
-                            const half2 wh = __hmul2(ph[m][j], as_h2(dd));
-                            wa[m][2 * j] = h2(wh);
-                            wa[m][2 * j + 1] = h2(__hfma2(pl[m][j], as_h2(dd), __hfma2(ph[m][j], as_h2(dd), __hneg2(wh))));
+                        for (int m = 0; m < NT; ++m) {
+                            const half2 d = as_h2(NT == 1 ? dv[j][bb] : dv[j][bb] & seen[m][j]);
+                            w[m][j] = h2(__hfma2(wy[m][j], d, __hfma2(wx[m][j], d, __hneg2(__hmul2(wx[m][j], d)))));
                         }
+                    }
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
                         const uint32_t b0 = __byte_perm(v[0][0][b], v[0][1][b], sel + x * 0x1111u), b1 = __byte_perm(v[1][0][b], v[1][1][b], sel + x * 0x1111u);
-                        const uint32_t l0 = low_codes(b0), l1 = low_codes(b1), h0 = high_codes(b0), h1 = high_codes(b1);
+                        const uint32_t av[4] = {low_codes(b0), high_codes(b0), low_codes(b1), high_codes(b1)};
 #pragma unroll
-                        for (int m = 0; m < MT; ++m) {
-                            mma16816(o[m][bb * 4 + x * 2], wa[m], l0, l1, o[m][bb * 4 + x * 2]);
-                            mma16816(o[m][bb * 4 + x * 2 + 1], wa[m], h0, h1, o[m][bb * 4 + x * 2 + 1]);
-                        }
+                        for (int m = 0; m < NT; ++m) mma16816(o[m][bb * 2 + x], av, w[m][0], w[m][1], o[m][bb * 2 + x]);
                     }
                 }
             }
         };
 
-        for (unsigned k = 0; k < mine; ++k) {
+        // Tile k's values are taken beside tile k + 1's scores: two chains that do not wait for one another.
+        float s[NT][2];
+        auto arrived = [&](unsigned k) {
             const unsigned slot = (done + k) % S::kSlots, phase = (done + k) / S::kSlots & 1;
-            if (__any_sync(~0u, !mbar_wait(&bars[warp][slot], phase))) {
-                // A copy did not arrive. Let those on their way land (each wait is bounded again); the CTA stops below.
-                for (unsigned i = k; i < ahead; ++i) mbar_wait(&bars[warp][(done + i) % S::kSlots], (done + i) / S::kSlots & 1);
-                late = true;
-                break;
-            }
-            if (present >> slot & 1) {
-                const uint8_t *tile = ring + slot * S::kTile;
-                const int key0 = int(sp.tile0 + t0 + warp + k * kWarps) * int(kTileTokens);
-                if (key0 >= all_low && key0 + int(kTileTokens) - 1 <= all_high) take(tile, key0, std::false_type{});
-                else take(tile, key0, std::true_type{});
+            if (!__any_sync(~0u, !mbar_wait(&bars[warp][slot], phase))) return true;
+            // A copy did not arrive. Let those on their way land (each wait is bounded again); the CTA stops below.
+            for (unsigned i = k; i < ahead; ++i) mbar_wait(&bars[warp][(done + i) % S::kSlots], (done + i) / S::kSlots & 1);
+            late = true;
+            return false;
+        };
+        auto key_of = [&](unsigned k) { return int((pc.tile0 + k * kWarps) * kTileTokens); };
+        auto tile_of = [&](unsigned k) { return ring + (done + k) % S::kSlots * S::kTile; };
+        auto is_there = [&](unsigned k) { return present >> (done + k) % S::kSlots & 1; };
+        if (mine && arrived(0) && is_there(0)) {
+            score(tile_of(0), s);
+            weigh(key_of(0), s);
+        }
+        for (unsigned k = 0; k < mine && !late; ++k) {
+            const bool next = k + 1 < mine && arrived(k + 1) && is_there(k + 1);
+            if (late) break;
+            if (is_there(k)) {
+                if (next) {
+                    float ns[NT][2];
+                    score(tile_of(k + 1), ns);
+                    value(tile_of(k), key_of(k), s);
+                    weigh(key_of(k + 1), ns);
+#pragma unroll
+                    for (int m = 0; m < NT; ++m) s[m][0] = ns[m][0], s[m][1] = ns[m][1];
+                } else {
+                    value(tile_of(k), key_of(k), s);
+                }
+            } else if (next) {
+                score(tile_of(k + 1), s);
+                weigh(key_of(k + 1), s);
             }
             __syncwarp();
-            if (ahead < mine) {  // the slot is free again
+            if (ahead < mine) {  // tile k's slot is free again
                 if (ahead % 32 == 0) look_up(ahead + lane);
-                present = fetch(ahead) ? present | 1u << slot : present & ~(1u << slot);
+                fetch(ahead);
                 ++ahead;
             }
         }
+        const Piece was = pc;
         done += mine;
+        ahead = 0;
+        if (!late) {
+            more = next_piece(pc);
+            if (more) begin_piece();  // the next piece's tiles come while this one's results are joined
+        }
+
+        // the warps' results: [warp][row][dim] (the barrier: all have read the piece before's)
+        __syncthreads();
+        const float drop = 1.0f / (lift * lift_d);
+#pragma unroll
+        for (int m = 0; m < NT; ++m) {
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) sum[m] += __shfl_xor_sync(~0u, sum[m], x);
+            if (g == 0) m_of[warp][m * 4 + t] = top[m], l_of[warp][m * 4 + t] = sum[m];
+            float *to = out + (warp * S::kRows + m * 4 + t) * D + 4 * (g >> 1) + 2 * (g & 1);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {  // two bytes of a word: the low nibbles, then the high ones
+                *reinterpret_cast<float2 *>(to + 32 * b) = make_float2((o[m][2 * b][0] + o[m][2 * b][1]) * drop, (o[m][2 * b + 1][0] + o[m][2 * b + 1][1]) * drop);
+                *reinterpret_cast<float2 *>(to + 32 * b + 16) =
+                    make_float2((o[m][2 * b][2] + o[m][2 * b][3]) * (0.0625f * drop), (o[m][2 * b + 1][2] + o[m][2 * b + 1][3]) * (0.0625f * drop));
+            }
+        }
         if (__syncthreads_or(late)) {
+            // some copy did not arrive: let the others land (each wait is bounded again), and stop
+            for (unsigned i = 0; i < ahead; ++i) mbar_wait(&bars[warp][(done + i) % S::kSlots], (done + i) / S::kSlots & 1);
             if (tid == 0) tell(a.status, kServeWait);
             return;
         }
-
-        // the warps' results, joined in the ring's place: [warp][row][dim]
-        float *out = reinterpret_cast<float *>(smem + S::kQBytes);
-        const float drop = 1.0f / (lift * lift_d);
+        for (unsigned i = tid; i < S::kRows * D / 4; i += kThreads) {
+            const unsigned row = i / (D / 4), dim = i % (D / 4) * 4, at = was.row0 + row;
+            if (at >= was.all) break;
+            float mm = -INFINITY, lv = 0.0f;
+            for (unsigned w = 0; w < kWarps; ++w) mm = fmaxf(mm, m_of[w][row]);
+            const float ref = mm == -INFINITY ? 0.0f : mm;
+            float4 ov = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            sum[m] += __shfl_xor_sync(~0u, sum[m], 1);
-            sum[m] += __shfl_xor_sync(~0u, sum[m], 2);
-            if (t == 0) m_of[warp][m * 8 + g] = top[m], l_of[warp][m * 8 + g] = sum[m];
-            float *to = out + ((warp * MT + m) * 8 + g) * (D + 2);
-#pragma unroll
-            for (int i = 0; i < NB * 4; ++i)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int n = 2 * int(t) + e, b = i / 4, x = i / 2 % 2, h = i & 1;
-                    to[32 * b + 16 * h + 4 * (n & 3) + 2 * (n >> 2) + x] = (o[m][i][e] + o[m][i][2 + e]) * (h ? 0.0625f : 1.0f) * drop;
-                }
-        }
-        __syncthreads();
-        const bool direct = n_split <= 1;
-        if (!direct && item >= plan.max_items) {  // rows counted twice (row starts that overlap): no room
-            if (tid == 0) tell(a.status, kServeRequest);
-        } else {
-            float *part = reinterpret_cast<float *>(a.room) + size_t(item) * plan.rows * D;
-            float2 *stat = reinterpret_cast<float2 *>(reinterpret_cast<float *>(a.room) + size_t(plan.max_items) * plan.rows * D) + size_t(item) * plan.rows;
-            for (unsigned i = tid; i < MT * 8 * D; i += kThreads) {
-                const unsigned row = i / D, dim = i % D;
-                if (row0 + row >= all) break;
-                float mm = -INFINITY;
-                for (unsigned w = 0; w < kWarps; ++w) mm = fmaxf(mm, m_of[w][row]);
-                const float ref = mm == -INFINITY ? 0.0f : mm;
-                float ov = 0.0f, lv = 0.0f;
-                for (unsigned w = 0; w < kWarps; ++w) {
-                    const float f = exp2_fast(m_of[w][row] - ref);
-                    ov += out[((w * MT + row / 8) * 8 + row % 8) * (D + 2) + dim] * f;
-                    lv += l_of[w][row] * f;
-                }
-                if (direct) {
-                    const unsigned at = row0 + row;
-                    a.y[(rq.start + at / per) * a.y_stride + size_t(head * per + at % per) * D + dim] = lv == 0.0f ? 0.0f : ov / lv;
-                } else {
-                    part[row * D + dim] = ov;
-                    if (dim == 0) stat[row] = make_float2(mm, lv);
-                }
+            for (unsigned w = 0; w < kWarps; ++w) {
+                const float f = exp2_fast(m_of[w][row] - ref);
+                const float4 x = *reinterpret_cast<const float4 *>(out + (w * S::kRows + row) * D + dim);
+                ov.x += x.x * f, ov.y += x.y * f, ov.z += x.z * f, ov.w += x.w * f;
+                lv += l_of[w][row] * f;
+            }
+            if (was.slot == kNoSlot) {
+                const float f = 1.0f / lv;
+                float *y = a.y + (was.start + at / per) * a.y_stride + size_t(was.head * per + at % per) * D + dim;
+                y[0] = lv == 0.0f ? 0.0f : ov.x * f, y[1] = lv == 0.0f ? 0.0f : ov.y * f, y[2] = lv == 0.0f ? 0.0f : ov.z * f,
+                y[3] = lv == 0.0f ? 0.0f : ov.w * f;
+            } else {
+                const size_t slot_row = size_t(was.slot) * S::kRows + row;
+                *reinterpret_cast<float4 *>(room.part + slot_row * D + dim) = ov;
+                if (dim == 0) room.stat[slot_row] = make_float2(mm, lv);
             }
         }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncthreads();  // the ring is free for the next item's copies
     }
 }
 
-// Rows whose keys were split: the chunks' maxima, sums and outputs joined. One CTA a row of a unit.
-__global__ void __launch_bounds__(kThreads) kv4_attn_merge_kernel(const Kv4AttnArgs a, const Plan plan) {
-    extern __shared__ unsigned prefix_units[];
-    __shared__ float red[kWarps], factor[kMergeChunk], weight[kMergeChunk], sums[kThreads];
-    __shared__ float4 joined[kThreads];
-    unsigned *prefix = prefix_units, *units = prefix_units + a.n_req + 1;
+// Units that lie in more than one range: the pieces' maxima, sums and outputs joined. Every edge between two ranges has a
+// CTA, which reads what it cuts, and the CTAs of a unit's edges share out its rows and dims. Few pieces: a warp takes 128
+// dims of a row, piece after piece. Many: a CTA takes 32 dims of a row, eight lanes to a piece, so that all loads are on
+// their way at once.
+__global__ void __launch_bounds__(kThreads) kv4_attn_merge_kernel(const Kv4AttnArgs a, const AttnPlan plan) {
+    __shared__ float4 o_of[kWarps][8];
+    __shared__ float2 s_of[kWarps];
     pdl_wait();
     pdl_launch_dependents();
-    const Schedule sched = make_schedule(a, plan, prefix, units);
-    const unsigned dim = a.c.dim, per = a.n_head / a.c.n_kv, total = units[a.n_req];
-    for (unsigned long long ur = blockIdx.x; ur < (unsigned long long)total * plan.rows; ur += gridDim.x) {
-        const unsigned unit = unsigned(ur / plan.rows), row = unsigned(ur % plan.rows);
-        const unsigned r = find(units, a.n_req, unit);
-        const Request rq = request_of(a, r, plan.rows, false);
-        const unsigned head = (unit - units[r]) % a.c.n_kv, group = (unit - units[r]) / a.c.n_kv;
-        const GroupSpan sp = span_of(a, rq, group, plan.rows);
-        const unsigned n_split = (sp.tiles + sched.chunk - 1) / sched.chunk, at = group * plan.rows + row;
-        if (n_split <= 1 || at >= rq.fresh * per) continue;
-        const unsigned first = prefix[r] + group * a.c.n_kv + head, step = rq.groups * a.c.n_kv;
-        if (first + (n_split - 1) * step >= plan.max_items) continue;
-        const size_t gap = size_t(plan.rows) * dim;
-        const float *part = reinterpret_cast<const float *>(a.room) + first * gap + size_t(row) * dim;
-        const float2 *stat = reinterpret_cast<const float2 *>(reinterpret_cast<const float *>(a.room) + plan.max_items * gap) + size_t(first) * plan.rows + row;
-        const size_t part_step = step * gap, stat_step = size_t(step) * plan.rows;
-        float m = -INFINITY;
-        for (unsigned s = threadIdx.x; s < n_split; s += kThreads) m = fmaxf(m, stat[s * stat_step].x);
-        for (unsigned o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-        __syncthreads();
-        if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = m;
-        __syncthreads();
-        for (unsigned w = 0; w < kWarps; ++w) m = fmaxf(m, red[w]);
-        const float ref = m == -INFINITY ? 0.0f : m;
-        // four dims a lane; the groups of lanes that cover the dims share out the chunks, whose factors lie in shared memory
-        const unsigned lanes = dim / 4, groups = kThreads / lanes, mine = threadIdx.x / lanes, d = threadIdx.x % lanes * 4;
-        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        float l = 0.0f;
-        for (unsigned s0 = 0; s0 < n_split; s0 += kMergeChunk) {
-            const unsigned n = n_split - s0 < kMergeChunk ? n_split - s0 : kMergeChunk;
-            __syncthreads();
-            for (unsigned s = threadIdx.x; s < n; s += kThreads) {
-                const float2 x = stat[(s0 + s) * stat_step];
-                const float f = exp2_fast(x.x - ref);
-                factor[s] = f;
-                weight[s] = f * x.y;
-            }
-            __syncthreads();
-            if (mine < groups) {
-#pragma unroll 4
-                for (unsigned s = mine; s < n; s += groups) {
-                    const float4 x = *reinterpret_cast<const float4 *>(part + (s0 + s) * part_step + d);
-                    const float f = factor[s];
-                    o.x += x.x * f, o.y += x.y * f, o.z += x.z * f, o.w += x.w * f;
-                    l += weight[s];
+    const unsigned dim = a.c.dim, per = a.n_head / a.c.n_kv, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    const Room room = room_of(a.room, plan, dim);
+    const unsigned ranges = room.edge[0].ranges < plan.max_ranges ? room.edge[0].ranges : plan.max_ranges;
+    for (unsigned edge = blockIdx.x + 1; edge < ranges; edge += gridDim.x) {
+        const Edge e = room.edge[edge];
+        // (a range that was given up after a wait ran out has left no edge here: whatever lies there is not followed)
+        if (e.n < 2 || e.first >= edge || edge - e.first >= e.n || e.first + e.n > ranges || e.rows > plan.rows || e.head >= a.c.n_kv ||
+            e.start >= a.n_rows || (e.row0 + e.rows - 1) / per >= a.n_rows - e.start)
+            continue;
+        const bool many = e.n >= 16;
+        const unsigned lanes = many ? 8 : 32, chunks = (dim / 4 + lanes - 1) / lanes, share = e.n - 1;
+        unsigned w = edge - e.first - 1;
+        if (!many) w = w * kWarps + warp;
+        for (; w < e.rows * chunks; w += many ? share : share * kWarps) {
+            const unsigned row = w / chunks, d = (w % chunks * lanes + lane % lanes) * 4;
+            const bool in = d < dim;
+            float m = -INFINITY, l = 0.0f;
+            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (unsigned s0 = many ? warp * 4 + lane / 8 : 0; s0 < e.n; s0 += many ? 128 : 8) {
+                float2 x[8];
+                float4 v[8];
+                const unsigned step = many ? 16 : 1;
+#pragma unroll
+                for (unsigned i = 0; i < 8; ++i) {
+                    const unsigned s = s0 + i * step;
+                    const size_t at = ((size_t(e.first + s) * 2 + (s ? 0 : e.slot0)) * plan.rows + row);
+                    x[i] = s < e.n ? room.stat[at] : make_float2(-INFINITY, 0.0f);
+                    v[i] = s < e.n && in ? *reinterpret_cast<const float4 *>(room.part + at * dim + d) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                }
+                float top = m;
+#pragma unroll
+                for (unsigned i = 0; i < 8; ++i) top = fmaxf(top, x[i].x);
+                const float ref = top == -INFINITY ? 0.0f : top, f0 = exp2_fast(m - ref);
+                m = top;
+                l *= f0;
+                o.x *= f0, o.y *= f0, o.z *= f0, o.w *= f0;
+#pragma unroll
+                for (unsigned i = 0; i < 8; ++i) {
+                    const float f = exp2_fast(x[i].x - ref);
+                    l += f * x[i].y;
+                    o.x += v[i].x * f, o.y += v[i].y * f, o.z += v[i].z * f, o.w += v[i].w * f;
                 }
             }
-        }
-        __syncthreads();
-        if (mine < groups) joined[mine * lanes + threadIdx.x % lanes] = o, sums[mine] = l;
-        __syncthreads();
-        if (mine == 0) {
-            for (unsigned i = 1; i < groups; ++i) {
-                const float4 x = joined[i * lanes + threadIdx.x];
-                o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w;
-                l += sums[i];
+            if (many) {  // the pieces' lanes, then the warps
+                float top = m;
+                for (unsigned x = 8; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, x));
+                const float f = exp2_fast(m - (top == -INFINITY ? 0.0f : top));
+                m = top;
+                l *= f;
+                o.x *= f, o.y *= f, o.z *= f, o.w *= f;
+                for (unsigned x = 8; x < 32; x <<= 1)
+                    o.x += __shfl_xor_sync(~0u, o.x, x), o.y += __shfl_xor_sync(~0u, o.y, x), o.z += __shfl_xor_sync(~0u, o.z, x),
+                        o.w += __shfl_xor_sync(~0u, o.w, x), l += __shfl_xor_sync(~0u, l, x);
+                __syncthreads();
+                if (lane < 8) o_of[warp][lane] = o;
+                if (lane == 0) s_of[warp] = make_float2(m, l);
+                __syncthreads();
+                if (warp || lane >= 8) continue;
+                top = -INFINITY;
+                for (unsigned i = 0; i < kWarps; ++i) top = fmaxf(top, s_of[i].x);
+                const float ref = top == -INFINITY ? 0.0f : top;
+                l = 0.0f;
+                o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                for (unsigned i = 0; i < kWarps; ++i) {
+                    const float fi = exp2_fast(s_of[i].x - ref);
+                    const float4 v = o_of[i][lane];
+                    l += s_of[i].y * fi;
+                    o.x += v.x * fi, o.y += v.y * fi, o.z += v.z * fi, o.w += v.w * fi;
+                }
             }
-            const float f = l == 0.0f ? 0.0f : 1.0f / l;
-            float *y = a.y + (rq.start + at / per) * a.y_stride + size_t(head * per + at % per) * dim + d;
+            if (!in) continue;
+            const unsigned at = e.row0 + row;
+            const float f = 1.0f / l;
+            float *y = a.y + (e.start + at / per) * a.y_stride + size_t(e.head * per + at % per) * dim + d;
             y[0] = l == 0.0f ? 0.0f : o.x * f, y[1] = l == 0.0f ? 0.0f : o.y * f, y[2] = l == 0.0f ? 0.0f : o.z * f, y[3] = l == 0.0f ? 0.0f : o.w * f;
         }
     }
 }
 
-template <int NB, int MT>
-cudaError_t launch_tiles(const Kv4AttnArgs &a, const Plan &plan, unsigned sms, cudaStream_t st) {
-    using S = Shape<NB, MT>;
-    const size_t smem = S::kSmem + (size_t(a.n_req) + 1) * 4;
-    static std::mutex mu;
-    static int resident[64] = {};  // CTAs an SM takes, by device
-    int dev = 0, ctas = 0;
-    cudaError_t e = cudaGetDevice(&dev);
+template <int NB, int NT>
+cudaError_t launch_tiles(const Kv4AttnArgs &a, const AttnPlan &plan, unsigned grid, cudaStream_t st) {
+    using S = Shape<NB, NT>;
+    const cudaError_t e = ensure_smem_attr(reinterpret_cast<const void *>(kv4_attn_kernel<NB, NT>), S::kSmem + int(kAttnMaxReq + 1) * 4);
     if (e != cudaSuccess) return e;
-    {
-        std::lock_guard<std::mutex> lock(mu);
-        if (dev < 64) ctas = resident[dev];
-        if (!ctas) {
-            e = cudaFuncSetAttribute(kv4_attn_kernel<NB, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem + int(kAttnMaxReq + 1) * 4);
-            if (e != cudaSuccess) return e;
-            e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&ctas, kv4_attn_kernel<NB, MT>, kThreads, S::kSmem + 1024);
-            if (e != cudaSuccess) return e;
-            if (ctas < 1) ctas = 1;
-            if (dev < 64) resident[dev] = ctas;
-        }
-    }
-    const unsigned grid = sms * unsigned(ctas);
-    return launch_pdl(kv4_attn_kernel<NB, MT>, dim3(grid < plan.max_items ? grid : plan.max_items), dim3(kThreads), smem, st, a, plan);
+    return launch_pdl(kv4_attn_kernel<NB, NT>, dim3(grid), dim3(kThreads), S::kSmem + (size_t(a.n_req) + 1) * 4, st, a, plan);
 }
 
-Plan plan_of(const Kv4AttnArgs &a, unsigned sms) {
-    Plan p;
+AttnPlan plan_of(const Kv4AttnArgs &a, unsigned sms) {
+    AttnPlan p;
     const unsigned per = a.n_head / a.c.n_kv;
-    p.rows = a.c.dim <= 128 && (unsigned long long)a.max_q * per > 8 ? 16 : 8;
-    p.target = sms * 4;
-    // the most units there can be, and the items: `target`, or a chunk's worth each, and a rest for each unit
+    const unsigned sets = (unsigned long long)a.max_q * per > 4 ? 2 : 1;
+    p.rows = 4 * sets;
+    p.grid = sms * (a.c.dim / 32 * sets <= 8 ? TC : 2);  // as many as run at once
+    // the most units there can be, and the line's length
     const unsigned long long q = a.max_q < a.n_rows ? a.max_q : a.n_rows, rows = (unsigned long long)a.n_rows * per;
     unsigned long long groups = rows / p.rows + (a.n_req < a.n_rows ? a.n_req : a.n_rows);
     const unsigned long long each = (q * per + p.rows - 1) / p.rows * a.n_req;
     if (each < groups) groups = each;
-    const unsigned long long tiles = groups * a.c.n_kv * ((a.max_kv + kTileTokens - 1) / kTileTokens);
-    const unsigned long long by_chunk = tiles / kMaxChunkTiles;
-    unsigned long long items = groups * a.c.n_kv + (by_chunk > p.target ? by_chunk : p.target);
-    if (tiles / kWarps + groups * a.c.n_kv < items) items = tiles / kWarps + groups * a.c.n_kv;
-    p.max_items = items < 0x7fffffffull ? unsigned(items) : 0x7fffffffu;
+    const unsigned long long units = groups * a.c.n_kv, line = units * ((a.max_kv + kTileTokens - 1) / kTileTokens + kUnitCost);
+    if ((line + kWarps - 1) / kWarps < p.grid) p.grid = unsigned((line + kWarps - 1) / kWarps);
+    const unsigned long long turns = (line + (unsigned long long)p.grid * kMaxRange - 1) / ((unsigned long long)p.grid * kMaxRange);
+    p.max_ranges = unsigned(turns * p.grid);
+    p.fits = line < 0x80000000ull;
     return p;
 }
 
 }  // namespace
 
 size_t kv4_attn_room(const Kv4AttnArgs &a, unsigned sms) {
-    const Plan p = plan_of(a, sms);
-    return size_t(p.max_items) * p.rows * (a.c.dim * 4 + 8);
+    const AttnPlan p = plan_of(a, sms);
+    if (!p.fits) return 0;
+    return size_t(p.max_ranges) * (2 * p.rows * (a.c.dim * 4 + 8) + sizeof(Edge));
 }
-unsigned kv4_attn_launches(const Kv4AttnArgs &a, unsigned) { return a.max_kv > kWarps * kTileTokens ? 2 : 1; }
+unsigned kv4_attn_launches(const Kv4AttnArgs &a, unsigned sms) { return plan_of(a, sms).max_ranges > 1 ? 2 : 1; }
 
 cudaError_t launch_kv4_attn(const Kv4AttnArgs &a, unsigned sms, cudaStream_t st) {
-    const Plan p = plan_of(a, sms);
+    const AttnPlan p = plan_of(a, sms);
     const unsigned nb = a.c.dim / 32;
     cudaError_t e = cudaErrorInvalidValue;
-    if (p.rows == 16) {
-        if (nb == 1) e = launch_tiles<1, 2>(a, p, sms, st);
-        if (nb == 2) e = launch_tiles<2, 2>(a, p, sms, st);
-        if (nb == 3) e = launch_tiles<3, 2>(a, p, sms, st);
-        if (nb == 4) e = launch_tiles<4, 2>(a, p, sms, st);
-    } else {
-        if (nb == 1) e = launch_tiles<1, 1>(a, p, sms, st);
-        if (nb == 2) e = launch_tiles<2, 1>(a, p, sms, st);
-        if (nb == 3) e = launch_tiles<3, 1>(a, p, sms, st);
-        if (nb == 4) e = launch_tiles<4, 1>(a, p, sms, st);
-        if (nb == 5) e = launch_tiles<5, 1>(a, p, sms, st);
-        if (nb == 6) e = launch_tiles<6, 1>(a, p, sms, st);
-        if (nb == 7) e = launch_tiles<7, 1>(a, p, sms, st);
-        if (nb == 8) e = launch_tiles<8, 1>(a, p, sms, st);
+#define B200Q_TILES(NB)                                                       \
+    case NB:                                                                 \
+        e = p.rows == 4 ? launch_tiles<NB, 1>(a, p, p.grid, st) : launch_tiles<NB, 2>(a, p, p.grid, st); \
+        break;
+    switch (nb) {
+        B200Q_TILES(1) B200Q_TILES(2) B200Q_TILES(3) B200Q_TILES(4) B200Q_TILES(5) B200Q_TILES(6) B200Q_TILES(7) B200Q_TILES(8)
     }
-    // up to 64 keys are never split
-    if (e != cudaSuccess || kv4_attn_launches(a, sms) == 1) return e;
-    const unsigned long long rows = (unsigned long long)p.max_items * p.rows;
-    return launch_pdl(kv4_attn_merge_kernel, dim3(unsigned(rows < sms * 16ull ? rows : sms * 16ull)), dim3(kThreads), (size_t(a.n_req) + 1) * 8, st, a, p);
+#undef B200Q_TILES
+    if (e != cudaSuccess) return e;
+    if (p.max_ranges == 1) return e;  // nothing lies in two ranges
+    const unsigned edges = p.max_ranges - 1;
+    return launch_pdl(kv4_attn_merge_kernel, dim3(edges < sms * 8 ? edges : sms * 8), dim3(kThreads), 0, st, a, p);
 }
 
 }  // namespace b200q

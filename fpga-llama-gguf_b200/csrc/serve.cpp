@@ -348,6 +348,7 @@ B200Q_API int b200q_kv4_attn(int device, const b200q_kv4_pool *pool, const float
     if (!c.ok() || n_rows == 0) return c.rc();
     Kv4AttnArgs a = attn_shape(pool, n_rows, n_head, n_req, max_q, max_kv);
     const size_t room = kv4_attn_room(a, c.sms());
+    c.need(room != 0, "n_rows, n_req and max_kv allow for more than 2^31 tiles of work");
     if (workspace_bytes < room) c.refuse("the workspace holds %zu bytes, %zu are needed", workspace_bytes, room);
     c.memory("pool", pool->base, bytes, 16);
     c.memory("q", q, rows_extent(n_rows, q_stride, q_width), 4);
