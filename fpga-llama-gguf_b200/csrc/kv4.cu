@@ -14,9 +14,55 @@ __device__ __forceinline__ void tell(uint32_t *status, unsigned bit) {
 
 // ---- block_map ------------------------------------------------------------------------------------------------------
 // Request r's new tokens take positions past .. past + new - 1. Blocks ceil(past / page) .. ceil(kv / page) - 1 of its
-// table row come from the free list in request order: two exclusive sums over the requests (rows, fresh pages), then one
-// slot a row. A single CTA: the work is two short sums, and rows are a few bytes each.
-__global__ void __launch_bounds__(1024) block_map_kernel(const BlockMapArgs a) {
+// table row come from the free list in request order: two exclusive sums over the requests (rows, fresh pages), which one
+// CTA forms, then one slot a row. Latency is all that counts in the sums; the rows are 8 bytes each, so up to kMapRows of
+// them the same CTA writes (one launch), more are shared out by a second kernel.
+constexpr unsigned kMapRows = 4096;
+
+// rows j0 .. j0 + 3: each one's request is found once, by bisection, and then followed
+__device__ __forceinline__ void map_rows(const BlockMapArgs &a, unsigned j0) {
+    const unsigned rows = a.q_start[a.n_req];
+    unsigned slot[4], pos[4];
+    unsigned r = 0;
+    if (j0 < rows) {
+        unsigned hi = a.n_req;  // the last request that starts at or before row j0
+        while (hi - r > 1) {
+            const unsigned mid = (r + hi) / 2;
+            if (a.q_start[mid] <= j0) r = mid;
+            else hi = mid;
+        }
+    }
+    unsigned next = j0 < rows ? a.q_start[r + 1] : 0, start = j0 < rows ? a.q_start[r] : 0, past = j0 < rows ? a.past[r] : 0;
+    unsigned block = ~0u, page = kNoSlot;
+#pragma unroll
+    for (unsigned i = 0; i < 4; ++i) {
+        const unsigned j = j0 + i;
+        slot[i] = kNoSlot;
+        pos[i] = 0;
+        if (j >= rows) continue;
+        while (next <= j) {
+            start = next;
+            ++r;
+            next = a.q_start[r + 1];
+            past = a.past[r];
+            block = ~0u;
+        }
+        const unsigned long long p = (unsigned long long)past + (j - start);
+        if (p >= (unsigned long long)a.stride * a.page) continue;
+        pos[i] = unsigned(p);
+        const unsigned b = pos[i] / a.page;
+        if (b != block) page = a.table[size_t(r) * a.stride + b], block = b;
+        if (page != kNoSlot) slot[i] = page * a.page + (pos[i] - b * a.page);
+    }
+    if (j0 + 4 <= a.n_rows && ((reinterpret_cast<uintptr_t>(a.slots) | reinterpret_cast<uintptr_t>(a.positions)) & 15) == 0) {
+        *reinterpret_cast<uint4 *>(a.slots + j0) = make_uint4(slot[0], slot[1], slot[2], slot[3]);
+        *reinterpret_cast<uint4 *>(a.positions + j0) = make_uint4(pos[0], pos[1], pos[2], pos[3]);
+    } else {
+        for (unsigned i = 0; i < 4 && j0 + i < a.n_rows; ++i) a.slots[j0 + i] = slot[i], a.positions[j0 + i] = pos[i];
+    }
+}
+
+__global__ void __launch_bounds__(1024) block_map_kernel(const BlockMapArgs a, bool rows_too) {
     __shared__ unsigned long long warp_rows[32], warp_need[32];
     __shared__ unsigned long long done_rows, done_need;
     pdl_wait();
@@ -25,21 +71,20 @@ __global__ void __launch_bounds__(1024) block_map_kernel(const BlockMapArgs a) {
     const unsigned long long cap = (unsigned long long)a.stride * a.page;
     const unsigned cursor = *a.cursor_in;
     if (tid == 0) done_rows = done_need = 0;
-    __syncthreads();
-    for (unsigned r0 = 0; r0 < a.n_req; r0 += 1024) {
+    for (unsigned r0 = 0; r0 < a.n_req; r0 += blockDim.x) {
         const unsigned r = r0 + tid;
-        unsigned long long past = 0, fresh = 0, first = 0, last = 0;
+        unsigned fresh = 0, first = 0, last = 0;
         if (r < a.n_req) {
-            past = a.past[r];
+            const unsigned past = a.past[r];
             fresh = a.fresh[r];
-            unsigned long long kv = past + fresh;
+            unsigned long long kv = (unsigned long long)past + fresh;
             if (kv > cap) {
                 kv = cap;
                 tell(a.status, kServeShort);
             }
             a.kv_len[r] = unsigned(kv);
-            first = (past + a.page - 1) / a.page;
-            last = (kv + a.page - 1) / a.page;
+            first = past / a.page + (past % a.page != 0);
+            last = unsigned(kv) / a.page + (unsigned(kv) % a.page != 0);
             if (last < first) last = first;
         }
         unsigned long long rows = fresh, need = last - first;
@@ -47,51 +92,46 @@ __global__ void __launch_bounds__(1024) block_map_kernel(const BlockMapArgs a) {
             const unsigned long long x = __shfl_up_sync(~0u, rows, o), y = __shfl_up_sync(~0u, need, o);
             if (lane >= o) rows += x, need += y;
         }
+        __syncthreads();  // the sums of the turn before are read, done_* written
         if (lane == 31) warp_rows[warp] = rows, warp_need[warp] = need;
         __syncthreads();
         unsigned long long row0 = done_rows + rows - fresh, need0 = done_need + need - (last - first);
-        for (unsigned w = 0; w < warp; ++w) row0 += warp_rows[w], need0 += warp_need[w];
+        if (warp) {  // the warps before this one: a lane each, then added up
+            unsigned long long x = lane < warp ? warp_rows[lane] : 0, y = lane < warp ? warp_need[lane] : 0;
+            for (unsigned o = 16; o; o >>= 1) x += __shfl_xor_sync(~0u, x, o), y += __shfl_xor_sync(~0u, y, o);
+            row0 += x, need0 += y;
+        }
         if (r < a.n_req) {
             a.q_start[r] = unsigned(row0);
-            for (unsigned long long b = first; b < last; ++b) {
+            for (unsigned b = first; b < last; ++b) {
                 const unsigned long long f = cursor + need0 + (b - first);
                 a.table[size_t(r) * a.stride + b] = f < a.n_free ? a.free_pages[f] : kNoSlot;
             }
             if (last > first && cursor + need0 + (last - first) > a.n_free) tell(a.status, kServeShort);
         }
         __syncthreads();
-        if (tid == 1023) {
+        if (tid == blockDim.x - 1) {
             done_rows = row0 + fresh;
             done_need = need0 + (last - first);
         }
-        __syncthreads();
     }
+    __syncthreads();
     if (tid == 0) {
         a.q_start[a.n_req] = unsigned(done_rows);
         const unsigned long long c = cursor + done_need;
         *a.cursor_out = unsigned(c < a.n_free ? c : (cursor < a.n_free ? a.n_free : cursor));
         if (done_rows > a.n_rows) tell(a.status, kServeRequest);
     }
+    if (!rows_too) return;
     __syncthreads();
-    for (unsigned j = tid; j < a.n_rows; j += 1024) {
-        unsigned slot = kNoSlot, pos = 0;
-        if (j < done_rows) {
-            unsigned lo = 0, hi = a.n_req;  // the last request that starts at or before row j
-            while (hi - lo > 1) {
-                const unsigned mid = (lo + hi) / 2;
-                if (a.q_start[mid] <= j) lo = mid;
-                else hi = mid;
-            }
-            const unsigned long long p = (unsigned long long)a.past[lo] + (j - a.q_start[lo]);
-            if (p < cap) {
-                pos = unsigned(p);
-                const unsigned page = a.table[size_t(lo) * a.stride + pos / a.page];
-                if (page != kNoSlot) slot = page * a.page + pos % a.page;
-            }
-        }
-        a.slots[j] = slot;
-        a.positions[j] = pos;
-    }
+    for (unsigned j = tid * 4; j < a.n_rows; j += blockDim.x * 4) map_rows(a, j);
+}
+
+__global__ void __launch_bounds__(256) map_rows_kernel(const BlockMapArgs a) {
+    pdl_wait();
+    pdl_launch_dependents();
+    const unsigned j = (blockIdx.x * 256 + threadIdx.x) * 4;
+    if (j < a.n_rows) map_rows(a, j);
 }
 
 // ---- kv4_store / kv4_load -------------------------------------------------------------------------------------------
@@ -103,79 +143,131 @@ __device__ __forceinline__ uint8_t *tile_of(const Kv4View &c, unsigned slot, uns
     return c.base + ((size_t(page) * c.n_kv + head) * (c.page / kTileTokens) + t) * kv4_tile_bytes(c.dim);
 }
 
+// A thread stays with its values of its block and goes down the rows, kRowsTurn at a time, so that what places them in a
+// row is worked out once and several rows' loads are on their way together.
+constexpr unsigned kRowsTurn = 4;
+
+struct RowPlace {
+    unsigned head, b, l;  // KV head, block of the head, lane of the block
+    bool is_v, real;
+    size_t in_row;        // of the thread's values, in floats
+};
+__device__ __forceinline__ RowPlace row_place(const Kv4RowsArgs &a) {
+    const unsigned nb = a.c.dim / 32, half = a.c.n_kv * nb, i = blockIdx.x * 256 + threadIdx.x, blk = i / 8;
+    RowPlace p;
+    p.real = blk < 2 * half;
+    p.is_v = blk >= half;
+    const unsigned hb = p.is_v ? blk - half : blk;
+    p.l = i % 8;
+    p.head = hb / nb;
+    p.b = hb % nb;
+    p.in_row = size_t(hb) * 32 + p.l * 4;
+    return p;
+}
+
+template <bool kWide>  // rows on 16 bytes
 __global__ void __launch_bounds__(256) kv4_store_kernel(const Kv4RowsArgs a) {
     pdl_wait();
     pdl_launch_dependents();
-    const unsigned nb = a.c.dim / 32, per_row = a.c.n_kv * nb * 2;  // blocks of a token: K's, then V's
-    const unsigned long long total = (unsigned long long)a.n * per_row * 8;
-    for (unsigned long long i = (unsigned long long)blockIdx.x * 256 + threadIdx.x; i < (total + 31) / 32 * 32;
-         i += (unsigned long long)gridDim.x * 256) {
-        const bool real = i < total;
-        const unsigned long long blk = real ? i / 8 : 0;
-        const unsigned l = unsigned(i % 8), row = unsigned(blk / per_row), in_row = unsigned(blk % per_row);
-        const bool is_v = in_row >= per_row / 2;
-        const unsigned hb = is_v ? in_row - per_row / 2 : in_row, head = hb / nb, b = hb % nb;
-        const float *src = (is_v ? a.v + row * a.v_stride : a.k + row * a.k_stride) + hb * 32 + l * 4;
-        float x[4];
-        for (unsigned e = 0; e < 4; ++e) x[e] = real ? src[e] : 0.0f;
-        float best = 0.0f, amax = 0.0f;
-        bool bad = false;
-        for (unsigned e = 0; e < 4; ++e) {
-            bad = bad || !(fabsf(x[e]) <= 3.402823466e38f);
-            if (fabsf(x[e]) > amax) amax = fabsf(x[e]), best = x[e];
+    const RowPlace p = row_place(a);
+    const unsigned nb = a.c.dim / 32;
+    const float *from = (p.is_v ? a.v : a.k) + p.in_row;
+    const size_t stride = p.is_v ? a.v_stride : a.k_stride;
+    for (unsigned row0 = blockIdx.y * kRowsTurn; row0 < a.n; row0 += gridDim.y * kRowsTurn) {
+        float x[kRowsTurn][4];
+        unsigned slots[kRowsTurn];
+#pragma unroll
+        for (unsigned i = 0; i < kRowsTurn; ++i) {
+            const bool in = p.real && row0 + i < a.n;
+            slots[i] = in ? a.slots[row0 + i] : kNoSlot;
+            const float *src = from + (row0 + i) * stride;
+            if (kWide && in) {
+                const float4 v = __ldcs(reinterpret_cast<const float4 *>(src));
+                x[i][0] = v.x, x[i][1] = v.y, x[i][2] = v.z, x[i][3] = v.w;
+            } else {
+                for (unsigned e = 0; e < 4; ++e) x[i][e] = in ? src[e] : 0.0f;
+            }
         }
-        for (unsigned o = 1; o < 8; o <<= 1) {
-            const float m = __shfl_xor_sync(~0u, amax, o), v = __shfl_xor_sync(~0u, best, o);
-            bad = __shfl_xor_sync(~0u, int(bad), o) || bad;
-            if (m > amax || (m == amax && (l & o))) amax = m, best = v;  // the lower lanes' value on ties
+#pragma unroll
+        for (unsigned i = 0; i < kRowsTurn; ++i) {
+            float best = 0.0f, amax = 0.0f;
+            bool bad = false;
+#pragma unroll
+            for (unsigned e = 0; e < 4; ++e) {
+                bad = bad || !(fabsf(x[i][e]) <= 3.402823466e38f);
+                if (fabsf(x[i][e]) > amax) amax = fabsf(x[i][e]), best = x[i][e];
+            }
+#pragma unroll
+            for (unsigned o = 1; o < 8; o <<= 1) {
+                const float v = __shfl_xor_sync(~0u, best, o);
+                if (fabsf(v) > amax || (fabsf(v) == amax && (p.l & o))) best = v;  // the lower lanes' value on ties
+                amax = fabsf(best);
+            }
+            bad = __ballot_sync(~0u, bad) >> (threadIdx.x & 24) & 0xff;
+            const float d = best * -0.125f, inv = d != 0.0f ? fdiv(1.0f, d) : 0.0f;
+            uint32_t half = 0;
+#pragma unroll
+            for (unsigned e = 0; e < 4; ++e) {
+                const int q = bad ? 8 : int(fadd(fmul(x[i][e], inv), 8.5f));
+                half |= uint32_t(q < 15 ? (q < 0 ? 0 : q) : 15) << (8 * e);
+            }
+            const uint32_t high = __shfl_down_sync(~0u, half, 4);
+            const unsigned slot = slots[i];
+            if (slot == kNoSlot) continue;
+            if (slot / a.c.page >= a.c.n_pages) {
+                tell(a.status, kServeSlot);
+                continue;
+            }
+            uint8_t *tile = tile_of(a.c, slot, p.head);
+            const unsigned t = slot % a.c.page % kTileTokens;
+            if (p.l < 4)
+                *reinterpret_cast<uint32_t *>(tile + (p.is_v ? kv4_v_word(nb, t, p.b, p.l) : kv4_k_word(nb, t, p.b, p.l))) = half | high << 4;
+            else if (p.l == 4)
+                *reinterpret_cast<uint16_t *>(tile + (p.is_v ? kv4_v_scale(nb, t, p.b) : kv4_k_scale(nb, t, p.b))) =
+                    bad ? uint16_t(0x7e00) : float_to_half_bits(d);
         }
-        const float d = best * -0.125f, inv = d != 0.0f ? fdiv(1.0f, d) : 0.0f;
-        uint32_t half = 0;
-        for (unsigned e = 0; e < 4; ++e) {
-            const int q = bad ? 8 : int(fadd(fmul(x[e], inv), 8.5f));
-            half |= uint32_t(q < 15 ? (q < 0 ? 0 : q) : 15) << (8 * e);
-        }
-        const uint32_t high = __shfl_down_sync(~0u, half, 4);
-        if (!real) continue;
-        const unsigned slot = a.slots[row];
-        if (slot == kNoSlot) continue;
-        if (slot / a.c.page >= a.c.n_pages) {
-            tell(a.status, kServeSlot);
-            continue;
-        }
-        uint8_t *tile = tile_of(a.c, slot, head);
-        const unsigned t = slot % a.c.page % kTileTokens;
-        if (l < 4)
-            *reinterpret_cast<uint32_t *>(tile + (is_v ? kv4_v_word(nb, t, b, l) : kv4_k_word(nb, t, b, l))) = half | high << 4;
-        else if (l == 4)
-            *reinterpret_cast<uint16_t *>(tile + (is_v ? kv4_v_scale(nb, t, b) : kv4_k_scale(nb, t, b))) =
-                bad ? uint16_t(0x7e00) : float_to_half_bits(d);
     }
 }
 
+template <bool kWide>
 __global__ void __launch_bounds__(256) kv4_load_kernel(const Kv4RowsArgs a) {
     pdl_wait();
     pdl_launch_dependents();
-    const unsigned nb = a.c.dim / 32, per_row = a.c.n_kv * nb * 2;
-    const unsigned long long total = (unsigned long long)a.n * per_row * 8;
-    for (unsigned long long i = (unsigned long long)blockIdx.x * 256 + threadIdx.x; i < total;
-         i += (unsigned long long)gridDim.x * 256) {
-        const unsigned long long blk = i / 8;
-        const unsigned l = unsigned(i % 8), row = unsigned(blk / per_row), in_row = unsigned(blk % per_row);
-        const bool is_v = in_row >= per_row / 2;
-        const unsigned hb = is_v ? in_row - per_row / 2 : in_row, head = hb / nb, b = hb % nb;
-        const unsigned slot = a.slots[row];
-        if (slot == kNoSlot) continue;
-        if (slot / a.c.page >= a.c.n_pages) {
-            tell(a.status, kServeSlot);
-            continue;
+    const RowPlace p = row_place(a);
+    if (!p.real) return;
+    const unsigned nb = a.c.dim / 32, w = p.l & 3;
+    float *to = (p.is_v ? a.v : a.k) + p.in_row;
+    const size_t stride = p.is_v ? a.v_stride : a.k_stride;
+    for (unsigned row0 = blockIdx.y * kRowsTurn; row0 < a.n; row0 += gridDim.y * kRowsTurn) {
+        unsigned slots[kRowsTurn];
+        uint32_t word[kRowsTurn];
+        uint16_t scale[kRowsTurn];
+#pragma unroll
+        for (unsigned i = 0; i < kRowsTurn; ++i) slots[i] = row0 + i < a.n ? a.slots[row0 + i] : kNoSlot;
+#pragma unroll
+        for (unsigned i = 0; i < kRowsTurn; ++i) {
+            if (slots[i] != kNoSlot && slots[i] / a.c.page >= a.c.n_pages) {
+                tell(a.status, kServeSlot);
+                slots[i] = kNoSlot;
+            }
+            if (slots[i] == kNoSlot) continue;
+            const uint8_t *tile = tile_of(a.c, slots[i], p.head);
+            const unsigned t = slots[i] % a.c.page % kTileTokens;
+            word[i] = *reinterpret_cast<const uint32_t *>(tile + (p.is_v ? kv4_v_word(nb, t, p.b, w) : kv4_k_word(nb, t, p.b, w)));
+            scale[i] = *reinterpret_cast<const uint16_t *>(tile + (p.is_v ? kv4_v_scale(nb, t, p.b) : kv4_k_scale(nb, t, p.b)));
         }
-        const uint8_t *tile = tile_of(a.c, slot, head);
-        const unsigned t = slot % a.c.page % kTileTokens, w = l & 3;
-        const uint32_t word = *reinterpret_cast<const uint32_t *>(tile + (is_v ? kv4_v_word(nb, t, b, w) : kv4_k_word(nb, t, b, w)));
-        const float d = half_bits_to_float(*reinterpret_cast<const uint16_t *>(tile + (is_v ? kv4_v_scale(nb, t, b) : kv4_k_scale(nb, t, b))));
-        float *dst = (is_v ? a.v + row * a.v_stride : a.k + row * a.k_stride) + hb * 32 + l * 4;
-        for (unsigned e = 0; e < 4; ++e) dst[e] = fmul(float(int(word >> (8 * e + (l & 4)) & 15) - 8), d);
+#pragma unroll
+        for (unsigned i = 0; i < kRowsTurn; ++i) {
+            if (slots[i] == kNoSlot) continue;
+            const float d = half_bits_to_float(scale[i]);
+            float x[4];
+#pragma unroll
+            for (unsigned e = 0; e < 4; ++e) x[e] = fmul(float(int(word[i] >> (8 * e + (p.l & 4)) & 15) - 8), d);
+            float *dst = to + (row0 + i) * stride;
+            if (kWide) __stcs(reinterpret_cast<float4 *>(dst), make_float4(x[0], x[1], x[2], x[3]));
+            else
+                for (unsigned e = 0; e < 4; ++e) dst[e] = x[e];
+        }
     }
 }
 
@@ -235,19 +327,26 @@ __global__ void __launch_bounds__(128) kv4_reorder_kernel(const Kv4ReorderArgs a
 }  // namespace
 
 cudaError_t launch_block_map(const BlockMapArgs &a, cudaStream_t st) {
-    return launch_pdl(block_map_kernel, dim3(1), dim3(1024), 0, st, a);
+    const bool one = a.n_rows <= kMapRows;
+    const unsigned most = one && a.n_rows / 4 > a.n_req ? a.n_rows / 4 : a.n_req, threads = most <= 128 ? 128 : most <= 512 ? 512 : 1024;
+    const cudaError_t e = launch_pdl(block_map_kernel, dim3(1), dim3(threads), 0, st, a, one);
+    if (one || e != cudaSuccess) return e;
+    return launch_pdl(map_rows_kernel, dim3((a.n_rows + 1023) / 1024), dim3(256), 0, st, a);
 }
 
+// x: the values of a row; y: the rows, as many at a time as fill the GPU a few times over
 static dim3 rows_grid(const Kv4RowsArgs &a) {
-    const unsigned long long threads = (unsigned long long)a.n * a.c.n_kv * (a.c.dim / 32) * 16;
-    const unsigned long long g = (threads + 255) / 256;
-    return dim3(unsigned(g < 148 * 8 ? g : 148 * 8));
+    const unsigned x = (a.c.n_kv * (a.c.dim / 32) * 16 + 255) / 256, turns = (a.n + kRowsTurn - 1) / kRowsTurn, y = 148 * 16 / x + 1;
+    return dim3(x, turns < y ? turns : y);
+}
+static bool wide_rows(const Kv4RowsArgs &a) {
+    return ((reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) | a.k_stride * 4 | a.v_stride * 4) & 15) == 0;
 }
 cudaError_t launch_kv4_store(const Kv4RowsArgs &a, cudaStream_t st) {
-    return launch_pdl(kv4_store_kernel, rows_grid(a), dim3(256), 0, st, a);
+    return launch_pdl(wide_rows(a) ? kv4_store_kernel<true> : kv4_store_kernel<false>, rows_grid(a), dim3(256), 0, st, a);
 }
 cudaError_t launch_kv4_load(const Kv4RowsArgs &a, cudaStream_t st) {
-    return launch_pdl(kv4_load_kernel, rows_grid(a), dim3(256), 0, st, a);
+    return launch_pdl(wide_rows(a) ? kv4_load_kernel<true> : kv4_load_kernel<false>, rows_grid(a), dim3(256), 0, st, a);
 }
 
 cudaError_t launch_kv4_reorder(const Kv4ReorderArgs &a, cudaStream_t st) {

@@ -92,8 +92,16 @@ class Call {
     void check_memory() {
         if (!ok()) return;
         static AttrFn attr = entry();
+        CUdeviceptr start_of[kMaxExtents];
+        size_t size_of[kMaxExtents];
+        unsigned n_known = 0;
         for (unsigned i = 0; i < n_ && ok(); ++i) {
             const Extent &x = ext_[i];
+            const CUdeviceptr p = reinterpret_cast<CUdeviceptr>(x.p);
+            bool known = false;  // inside an allocation that an earlier pointer of this call lies in
+            for (unsigned j = 0; j < n_known && !known; ++j)
+                known = p >= start_of[j] && p - start_of[j] <= size_of[j] && x.bytes <= size_of[j] - (p - start_of[j]);
+            if (known) continue;
             int type = 0, ordinal = -1, managed = 0;
             CUdeviceptr start = 0;
             size_t size = 0;
@@ -101,13 +109,14 @@ class Call {
                                            CU_POINTER_ATTRIBUTE_IS_MANAGED, CU_POINTER_ATTRIBUTE_RANGE_START_ADDR,
                                            CU_POINTER_ATTRIBUTE_RANGE_SIZE};
             void *to[5] = {&type, &ordinal, &managed, &start, &size};
-            const CUdeviceptr p = reinterpret_cast<CUdeviceptr>(x.p);
             if (!attr || attr(5, what, to, p) != CUDA_SUCCESS || (type != CU_MEMORYTYPE_DEVICE && !managed))
                 refuse("%s is not device memory (it must be device memory of device %d)", x.name, device_);
             else if (!managed && ordinal != device_)
                 refuse("%s is device memory of device %d, not of device %d", x.name, ordinal, device_);
             else if (p < start || p - start > size || x.bytes > size - (p - start))
                 refuse("%s + %zu bytes runs past the end of its allocation", x.name, x.bytes);
+            start_of[n_known] = start;
+            size_of[n_known++] = size;
         }
         for (unsigned i = 0; i < n_ && ok(); ++i)
             for (unsigned j = 0; j < n_; ++j) {
