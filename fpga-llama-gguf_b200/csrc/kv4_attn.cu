@@ -33,6 +33,10 @@ constexpr unsigned kWarps = 4, kThreads = kWarps * 32;
 #endif
 constexpr unsigned kUnitCost = UC;        // what a unit costs besides its tiles (its queries, its joined output), in tiles
 constexpr unsigned kMaxRange = 1024;     // a warp adds at most 256 tiles into its accumulators before they are joined in FP32
+#ifndef PW
+#define PW 6144
+#endif
+constexpr unsigned kPromptRows = 64, kPromptWork = PW;
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ void tell(uint32_t *status, unsigned bit) {
@@ -43,6 +47,7 @@ struct AttnPlan {
     unsigned grid = 0;        // CTAs
     unsigned max_ranges = 0;  // ranges the workspace holds partial results for
     unsigned rows = 4;        // query rows (token, head) of a unit
+    unsigned most_rows = ~0u; // requests with more rows are the prompt kernel's
     bool fits = true;         // the line's places fit 32 bits
 };
 
@@ -57,14 +62,15 @@ struct Request {
     unsigned start = 0, fresh = 0, len = 0, groups = 0, span = 0;  // span: tiles that a group of rows sees at most
 };
 
-__device__ __forceinline__ Request request_of(const Kv4AttnArgs &a, unsigned r, unsigned rows, bool report) {
+__device__ __forceinline__ Request request_of(const Kv4AttnArgs &a, unsigned r, const AttnPlan &plan, bool report) {
     Request q;
     const unsigned s = a.q_start[r], e = a.q_start[r + 1], len = a.kv_len[r];
     if (s > e || e > a.n_rows || e - s > a.max_q || len > a.max_kv) {
         if (report) tell(a.status, kServeRequest);
         return q;
     }
-    const unsigned group = a.n_head / a.c.n_kv;
+    const unsigned group = a.n_head / a.c.n_kv, rows = plan.rows;
+    if ((unsigned long long)(e - s) * group > plan.most_rows) return q;
     q.start = s;
     q.fresh = e - s;
     q.len = len;
@@ -99,7 +105,7 @@ __device__ Schedule make_schedule(const Kv4AttnArgs &a, const AttnPlan &plan, un
     unsigned line = 0;
     for (unsigned r = r0; r < r1; ++r) {
         before[r] = line;
-        if (r < broken) line += line_of(a, request_of(a, r, plan.rows, blockIdx.x == 0));
+        if (r < broken) line += line_of(a, request_of(a, r, plan, blockIdx.x == 0));
         else if (blockIdx.x == 0) tell(a.status, kServeRequest);
     }
     unsigned ls = line;
@@ -332,7 +338,7 @@ __global__ void __launch_bounds__(kThreads, Shape<NB, NT>::kCtas) kv4_attn_kerne
             }
             if (fresh_range) req = find(before, a.n_req, from);
             while (before[req + 1] <= at_line) ++req;
-            const Request rq = request_of(a, req, plan.rows, false);
+            const Request rq = request_of(a, req, plan, false);
             const unsigned length = rq.span + kUnitCost, unit = (at_line - before[req]) / length, begin = before[req] + unit * length;
             const unsigned u0 = at_line - begin, u1 = (to - begin < length ? to - begin : length);
             const GroupSpan sp = span_of(a, rq, unit / a.c.n_kv, plan.rows);
@@ -889,6 +895,7 @@ AttnPlan plan_of(const Kv4AttnArgs &a, unsigned sms) {
     const unsigned per = a.n_head / a.c.n_kv;
     const unsigned sets = (unsigned long long)a.max_q * per > 4 ? 2 : 1;
     p.rows = 4 * sets;
+    if ((unsigned long long)a.max_q * per >= kPromptRows && (unsigned long long)a.n_rows * a.n_head >= kPromptWork) p.most_rows = kPromptRows - 1;
     p.grid = sms * (a.c.dim / 32 * sets <= 8 ? TC : 2);  // as many as run at once
     // the most units there can be, and the line's length
     const unsigned long long q = a.max_q < a.n_rows ? a.max_q : a.n_rows, rows = (unsigned long long)a.n_rows * per;
@@ -910,7 +917,10 @@ size_t kv4_attn_room(const Kv4AttnArgs &a, unsigned sms) {
     if (!p.fits) return 0;
     return size_t(p.max_ranges) * (2 * p.rows * (a.c.dim * 4 + 8) + sizeof(Edge));
 }
-unsigned kv4_attn_launches(const Kv4AttnArgs &a, unsigned sms) { return plan_of(a, sms).max_ranges > 1 ? 2 : 1; }
+unsigned kv4_attn_launches(const Kv4AttnArgs &a, unsigned sms) {
+    const AttnPlan p = plan_of(a, sms);
+    return (p.max_ranges > 1 ? 2 : 1) + (p.most_rows != ~0u);
+}
 
 cudaError_t launch_kv4_attn(const Kv4AttnArgs &a, unsigned sms, cudaStream_t st) {
     const AttnPlan p = plan_of(a, sms);
@@ -925,9 +935,12 @@ cudaError_t launch_kv4_attn(const Kv4AttnArgs &a, unsigned sms, cudaStream_t st)
     }
 #undef B200Q_TILES
     if (e != cudaSuccess) return e;
-    if (p.max_ranges == 1) return e;  // nothing lies in two ranges
-    const unsigned edges = p.max_ranges - 1;
-    return launch_pdl(kv4_attn_merge_kernel, dim3(edges < sms * 8 ? edges : sms * 8), dim3(kThreads), 0, st, a, p);
+    if (p.max_ranges > 1) {  // (else nothing lies in two ranges)
+        const unsigned edges = p.max_ranges - 1;
+        e = launch_pdl(kv4_attn_merge_kernel, dim3(edges < sms * 8 ? edges : sms * 8), dim3(kThreads), 0, st, a, p);
+    }
+    if (e != cudaSuccess || p.most_rows == ~0u) return e;
+    return launch_kv4_prompt(a, p.most_rows + 1, st);
 }
 
 }  // namespace b200q

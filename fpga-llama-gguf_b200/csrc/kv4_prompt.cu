@@ -1,0 +1,426 @@
+// Attention over the paged 4-bit cache for prompts: requests with many rows, on the fifth-generation tensor cores.
+//
+// A CTA takes 128 query rows (token, head of the group) of one KV head and goes over the keys 64 at a time, with FP32
+// sums and outputs as in kv4_attn.cu:
+//   S = Q K^T        FP32 accuracy from FP16 products: q = qh + ql (22 bits; rows scaled by a power of two), and a value of
+//                    the cache is d (c - 8), 15 bits, so kh + kl holds it exactly: S = qh kh + ql kh + qh kl
+//                    (what ql kl would add is below 2^-22 of a product)
+//   P = 2^(s - m)    the running maximum m of a row moves only when a score passes it
+//   O += P V         the same way: ph vh + pl vh + ph vl, in tensor memory over all keys
+// K and V rows are scaled by a power of two each (the key's largest d becomes 1/2 to 1), so that FP16 holds them whatever
+// their magnitude. K's comes back in as a factor of the key's column of S; V's, e_t, moves into the weight:
+// w_t = 2^(s_t + log2 e_t - m), and the sum of the weights takes w_t / e_t.
+//
+// Operands: qh, kh, kl, vh, vl in shared memory (no swizzle; K is K-major, V MN-major, both written 16 bytes = 8 dims of a
+// key at a time by the same code), ql and P in tensor memory. In a step all 8 warps
+//   unpack V    while the tensor cores form S
+//   soften      S from tensor memory, P back (lane = row; two warps share a row's 64 keys)
+//   unpack the next K    while the tensor cores add P V
+// and a bulk copy brings the next raw tiles as soon as V is unpacked.
+// Bound: per step 128 x 64 x D x 6 products; at D 256 shared memory (the operands' 320 KB and the unpacked tiles' 128 KB at
+// 128 bytes a cycle) is about as long as the tensor cores' work.
+#include <cuda_runtime.h>
+
+#include "common.cuh"
+#include "kv4.cuh"
+#include "launch.h"
+#include "serve.h"
+#include "tcgen05.cuh"
+
+namespace b200q {
+namespace {
+
+constexpr unsigned kRows = 128, kKeys = 64, kThreads = 256;
+constexpr unsigned kBadMax = 96;  // values that are not numbers, remembered by (key, block)
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ void tell(uint32_t *status, unsigned bit) {
+    if (status) atomicOr(status, bit);
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t h2(half2 x) { return *reinterpret_cast<uint32_t *>(&x); }
+__device__ __forceinline__ half2 as_h2(uint32_t x) { return *reinterpret_cast<half2 *>(&x); }
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float(unsigned(127 + e) << 23); }
+
+template <int NB>
+struct Prompt {
+    static constexpr int D = NB * 32, kTile = NB * 576;
+    static constexpr int kQ = kRows * D * 2, kPart = kKeys * D * 2;
+    static constexpr int kRaw = kQ + 4 * kPart, kSmem = kRaw + 4 * kTile;
+    static constexpr unsigned kS = D, kP = D + 64, kQl = D + 128, kNeed = D + 128 + D / 2;  // columns of tensor memory
+    static constexpr unsigned kCols = kNeed <= 256 ? 256 : 512;
+    static_assert(kNeed <= 512 && kSmem <= 216 * 1024);
+};
+
+template <int NB>
+__global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnArgs a, unsigned least_rows) {
+    using S = Prompt<NB>;
+    constexpr int D = S::D;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    __shared__ uint64_t bar_s, bar_o, bar_raw;
+    __shared__ uint32_t tm_base;
+    __shared__ __align__(16) float k_scale[kKeys], v_log[kKeys], v_inv[kKeys];  // read four at a time
+    __shared__ float row_top[2][kRows];
+    __shared__ unsigned present, n_bad, bad[kBadMax];
+    const unsigned tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const unsigned per = a.n_head / a.c.n_kv, head = blockIdx.x % a.c.n_kv, req = blockIdx.x / a.c.n_kv, row0 = (gridDim.y - 1 - blockIdx.y) * kRows;
+    pdl_wait();
+    pdl_launch_dependents();
+
+    // the request (left out, as kv4_attn.cu says, when its rows or lengths lie outside the bounds)
+    bool broken = false;
+    for (unsigned i = tid; i <= req; i += kThreads) broken = broken || a.q_start[i] > a.q_start[i + 1];
+    if (__syncthreads_or(broken)) return;
+    const unsigned start = a.q_start[req], end = a.q_start[req + 1], len = a.kv_len[req], all = (end - start) * per;
+    if (end > a.n_rows || end - start > a.max_q || len > a.max_kv || all < least_rows || row0 >= all) return;
+    const int base = int(len) - int(end - start);
+    const unsigned last = row0 + kRows < all ? row0 + kRows - 1 : all - 1;
+    const int hi = base + int(last / per), first_pos = base + int(row0 / per);
+    const int lo = a.window && first_pos >= 0 && unsigned(first_pos) + 1 > a.window ? first_pos + 1 - int(a.window) : 0;
+
+    // this thread's row (lane of tensor memory), and its half of the keys or dims
+    const unsigned quarter = warp & 3, half_ = warp >> 2, row = quarter * 32 + lane, at_row = row0 + row;
+    const bool real = at_row < all;
+    const int pos = real ? base + int(at_row / per) : -1;
+    const int low = a.window && pos >= 0 && unsigned(pos) + 1 > a.window ? pos + 1 - int(a.window) : 0;
+    float *y = a.y + (start + (real ? at_row / per : 0)) * a.y_stride + size_t(head * per + (real ? at_row % per : 0)) * D;
+    if (hi < 0) {  // no row of the tile sees anything
+        if (real)
+            for (unsigned d = 0; d < D / 2; ++d) y[half_ * (D / 2) + d] = 0.0f;
+        return;
+    }
+    const unsigned step0 = unsigned(lo) / kKeys, steps = unsigned(hi) / kKeys + 1 - step0;
+
+    if (warp == 0) tm_alloc(&tm_base, S::kCols);
+    if (tid == 0) {
+        mbar_init(&bar_s, 1);
+        mbar_init(&bar_o, 1);
+        mbar_init(&bar_raw, 1);
+        mbar_fence_init();
+        n_bad = 0;
+    }
+    tm_fence_before();
+    __syncthreads();
+    tm_fence_after();
+    const uint32_t tm = tm_base, tm_lane = tm + (quarter * 32 << 16);
+    uint8_t *const kh = smem + S::kQ, *const kl = kh + S::kPart, *const vh = kl + S::kPart, *const vl = vh + S::kPart, *const raw = smem + S::kRaw;
+
+    // the raw tiles of step j (warp 0): a bulk copy each, those behind the last key or without a page left out
+    const unsigned tiles_per_page = a.c.page / kTileTokens;
+    auto fetch = [&](unsigned j) {
+        const unsigned tile = (step0 + j) * (kKeys / kTileTokens) + lane;
+        const uint8_t *src = nullptr;
+        if (lane < kKeys / kTileTokens && int(tile * kTileTokens) <= hi) {
+            const unsigned page = a.table[size_t(req) * a.stride + tile / tiles_per_page];
+            if (page < a.c.n_pages)
+                src = a.c.base + ((size_t(page) * a.c.n_kv + head) * tiles_per_page + tile % tiles_per_page) * S::kTile;
+            else tell(a.status, kServePage);
+        }
+        const unsigned there = __ballot_sync(~0u, src != nullptr);
+        if (lane == 0) {
+            present = there;
+            mbar_expect_tx(&bar_raw, __popc(there) * S::kTile);
+        }
+        __syncwarp();
+        if (src)
+            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                             smem_addr(raw + lane * S::kTile)),
+                         "l"(src), "r"(S::kTile), "r"(smem_addr(&bar_raw))
+                         : "memory");
+    };
+    if (warp == 0) fetch(0);
+
+    // Q: rows scaled to below 2^11; the upper parts to shared memory, the lower ones to tensor memory
+    float row_scale;
+    {
+        const float *q = a.q + (start + (real ? at_row / per : 0)) * a.q_stride + (head * per + (real ? at_row % per : 0)) * a.q_head_stride;
+        const bool wide = ((reinterpret_cast<uintptr_t>(a.q) | a.q_stride * 4 | a.q_head_stride * 4) & 15) == 0;
+        auto load4 = [&](unsigned d) {
+            if (!real) return make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (wide) return *reinterpret_cast<const float4 *>(q + d);
+            return make_float4(q[d], q[d + 1], q[d + 2], q[d + 3]);
+        };
+        float top = 0.0f;
+        for (unsigned d = half_ * (D / 2); d < (half_ + 1) * (D / 2); d += 4) {
+            const float4 v = load4(d);
+            top = fmaxf(top, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+        }
+        row_top[half_][row] = top;
+        __syncthreads();
+        top = fmaxf(row_top[0][row], row_top[1][row]);
+        int ex = int(__float_as_uint(top) >> 23) - 127 - 10;
+        ex = ex < -110 ? -110 : ex > 110 ? 110 : ex;
+        row_scale = a.scale * kLog2e * pow2(ex);
+        const float down = pow2(-ex);
+        for (unsigned d = half_ * (D / 2); d < (half_ + 1) * (D / 2); d += 16) {
+            uint32_t low_part[8];
+#pragma unroll
+            for (unsigned g = 0; g < 2; ++g) {
+                uint32_t up[4];
+#pragma unroll
+                for (unsigned e = 0; e < 2; ++e) {
+                    const float4 v = load4(d + g * 8 + e * 4);
+                    const half2 x = __floats2half2_rn(v.x * down, v.y * down), z = __floats2half2_rn(v.z * down, v.w * down);
+                    const float2 bx = __half22float2(x), bz = __half22float2(z);
+                    up[2 * e] = h2(x), up[2 * e + 1] = h2(z);
+                    low_part[g * 4 + 2 * e] = h2(__floats2half2_rn(v.x * down - bx.x, v.y * down - bx.y));
+                    low_part[g * 4 + 2 * e + 1] = h2(__floats2half2_rn(v.z * down - bz.x, v.w * down - bz.y));
+                }
+                *reinterpret_cast<uint4 *>(smem + row / 8 * (D * 16) + (d / 8 + g) * 128 + row % 8 * 16) = make_uint4(up[0], up[1], up[2], up[3]);
+            }
+            tm_store8(tm_lane + S::kQl + d / 2, low_part);
+        }
+        tm_wait_store();
+    }
+
+    // Raw tiles to FP16 pairs of operands. A warp takes 8 keys, a lane a key and every fourth block.
+    const unsigned key = warp * 8 + lane % 8, token = key % kTileTokens;
+    const uint8_t *const my_tile = raw + key / kTileTokens * S::kTile;
+    auto unpack = [&](unsigned j, bool is_v, uint8_t *up, uint8_t *down) {
+        const int at = int((step0 + j) * kKeys + key);
+        const bool hidden = at > hi || !(present >> key / kTileTokens & 1);
+        half d[(NB + 3) / 4];
+        float top = 0.0f;
+#pragma unroll
+        for (int p = 0; p < (NB + 3) / 4; ++p) {
+            const unsigned b = p * 4 + lane / 8;
+            d[p] = __float2half_rn(0.0f);
+            if (b < NB && !hidden) {
+                d[p] = *reinterpret_cast<const half *>(my_tile + (is_v ? NB * 544 : NB * 512) + (token * NB + b) * 2);
+                if (is_v && !(fabsf(__half2float(d[p])) <= 65504.0f)) {  // set apart, lest it reach rows that do not see the key
+                    const unsigned n = atomicAdd(&n_bad, 1u);
+                    if (n < kBadMax) bad[n] = unsigned(at) * 8 + b;
+                    d[p] = __float2half_rn(0.0f);
+                }
+                top = fmaxf(top, fabsf(__half2float(d[p])));
+            }
+        }
+        top = fmaxf(top, __shfl_xor_sync(~0u, top, 8));
+        top = fmaxf(top, __shfl_xor_sync(~0u, top, 16));
+        const int e = top == 0.0f ? 0 : int(__float_as_uint(fminf(top, 65504.0f)) >> 23) - 126;  // top / 2^e is below 1
+        if (lane < 8) {
+            if (is_v) v_log[key] = hidden ? -INFINITY : float(e), v_inv[key] = pow2(-e);
+            else k_scale[key] = pow2(e);
+        }
+#pragma unroll
+        for (int p = 0; p < (NB + 3) / 4; ++p) {
+            const int nbp = NB - 4 * p < 4 ? NB - 4 * p : 4;
+            const unsigned bq = lane / 8, b = p * 4 + bq;
+            if (int(bq) >= nbp) continue;
+            const half2 dd = __half2half2(__float2half_rn(__half2float(d[p]) * pow2(-e)));
+            const uint8_t *words = my_tile + p * 1024 + (is_v ? NB * 256 + ((token / 8 * 2 + token % 2) * 16 + token / 2 % 4) * nbp * 4 : token * 16 * nbp) + bq * 4;
+            const unsigned word_step = is_v ? 16 * nbp : 4 * nbp;
+            uint8_t *const to = up + warp * (D * 16) + b * 512 + lane % 8 * 16, *const to_low = down + (to - up);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                uint32_t hi_of[2][4], lo_of[2][4];  // low nibbles' 8 dims, high nibbles' 8 dims
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const uint32_t w = hidden ? 0x88888888u : *reinterpret_cast<const uint32_t *>(words + (2 * u + i) * word_step);
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const uint32_t pair = __byte_perm(w, 0u, x ? 0x4342 : 0x4140);  // two bytes, 16 bits apart
+#pragma unroll
+                        for (int n = 0; n < 2; ++n) {
+                            const half2 c = __hsub2(as_h2((pair >> (4 * n) & 0x000f000fu) | 0x64006400u), as_h2(0x64086408u));
+                            const half2 v = __hmul2(c, dd);
+                            hi_of[n][2 * i + x] = h2(v);
+                            lo_of[n][2 * i + x] = h2(__hfma2(c, dd, __hneg2(v)));
+                        }
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    *reinterpret_cast<uint4 *>(to + (2 * n + u) * 128) = make_uint4(hi_of[n][0], hi_of[n][1], hi_of[n][2], hi_of[n][3]);
+                    *reinterpret_cast<uint4 *>(to_low + (2 * n + u) * 128) = make_uint4(lo_of[n][0], lo_of[n][1], lo_of[n][2], lo_of[n][3]);
+                }
+            }
+        }
+    };
+    auto hand_over = [&] {  // what this thread wrote, to the tensor cores
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        tm_fence_before();
+    };
+
+    bool fail = !mbar_wait(&bar_raw, 0);
+    if (!fail) unpack(0, false, kh, kl);
+    hand_over();
+    fail = __syncthreads_or(fail);
+    const uint32_t q_at = smem_addr(smem), kh_at = smem_addr(kh), kl_at = smem_addr(kl), vh_at = smem_addr(vh), vl_at = smem_addr(vl);
+    float top = -INFINITY, sum = 0.0f;
+    unsigned j = 0;
+    for (; j < steps && !fail; ++j) {
+        if (tid == 0) {
+            tm_fence_after();
+            constexpr uint32_t kind = tm_f16(kKeys, false);
+#pragma unroll 1
+            for (unsigned k = 0; k < D / 16; ++k) {
+                const uint64_t q = tm_operand(q_at + k * 256, 128, D * 16), kk = tm_operand(kh_at + k * 256, 128, D * 16);
+                tm_mma(tm + S::kS, q, kk, kind, k != 0);
+                tm_mma(tm + S::kS, q, tm_operand(kl_at + k * 256, 128, D * 16), kind, true);
+                tm_mma_t(tm + S::kS, tm + S::kQl + k * 8, kk, kind, true);
+            }
+            tm_commit(&bar_s);
+        }
+        if (j) fail = !mbar_wait(&bar_o, (j - 1) & 1);  // P and V are free
+        if (!fail) unpack(j, true, vh, vl);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // (the raw tiles are read: the next copies may come)
+        if ((fail = __syncthreads_or(fail))) break;
+        if (warp == 0 && j + 1 < steps) fetch(j + 1);
+
+        // scores of the row and 32 keys, in powers of two
+        fail = !mbar_wait(&bar_s, j & 1);
+        tm_fence_after();
+        uint32_t s[32];
+        tm_load32(tm_lane + S::kS + half_ * 32, s);
+        const int key0 = int((step0 + j) * kKeys + half_ * 32);
+        float mx = -INFINITY;
+        const bool edge = __any_sync(~0u, key0 < low || key0 + 31 > pos);
+#pragma unroll
+        for (unsigned i = 0; i < 32; i += 4) {
+            const float4 ks = *reinterpret_cast<const float4 *>(k_scale + half_ * 32 + i), vg = *reinterpret_cast<const float4 *>(v_log + half_ * 32 + i);
+            const float f[4] = {ks.x, ks.y, ks.z, ks.w}, g[4] = {vg.x, vg.y, vg.z, vg.w};
+#pragma unroll
+            for (unsigned e = 0; e < 4; ++e) {
+                float t = fmaf(__uint_as_float(s[i + e]) * f[e], row_scale, g[e]);
+                if (edge && (key0 + int(i + e) < low || key0 + int(i + e) > pos)) t = -INFINITY;
+                if (g[e] == -INFINITY) t = -INFINITY;
+                mx = fmaxf(mx, t);
+                s[i + e] = __float_as_uint(t);
+            }
+        }
+        row_top[half_][row] = mx;
+        if ((fail = __syncthreads_or(fail))) break;
+        mx = fmaxf(mx, row_top[half_ ^ 1][row]);
+        if (__any_sync(~0u, mx > top)) {  // a higher maximum: 4 above the score, so that it moves seldom
+            const float nt = mx > top ? mx + 4.0f : top, f = top == nt ? 1.0f : exp2_fast(top - nt);
+            sum *= f;
+            top = nt;
+            if (j) {
+                for (unsigned c = half_ * (D / 2); c < (half_ + 1) * (D / 2); c += 16) {
+                    uint32_t o[16];
+                    tm_load16(tm_lane + c, o);
+#pragma unroll
+                    for (unsigned e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                    tm_store16(tm_lane + c, o);
+                }
+            }
+        }
+        const float ref = top == -INFINITY ? 0.0f : top;
+        uint32_t ph[16], pl[16];
+#pragma unroll
+        for (unsigned i = 0; i < 32; i += 4) {
+            const float4 vi = *reinterpret_cast<const float4 *>(v_inv + half_ * 32 + i);
+            const float g[4] = {vi.x, vi.y, vi.z, vi.w};
+            float w[4];
+#pragma unroll
+            for (unsigned e = 0; e < 4; ++e) {
+                w[e] = exp2_fast(__uint_as_float(s[i + e]) - ref);
+                sum = fmaf(w[e], g[e], sum);
+                w[e] *= 0x1p14f;
+            }
+#pragma unroll
+            for (unsigned e = 0; e < 4; e += 2) {
+                const half2 h = __floats2half2_rn(w[e], w[e + 1]);
+                const float2 b = __half22float2(h);
+                ph[(i + e) / 2] = h2(h);
+                pl[(i + e) / 2] = h2(__floats2half2_rn(w[e] - b.x, w[e + 1] - b.y));
+            }
+        }
+        tm_store16(tm_lane + S::kP + half_ * 16, ph);
+        tm_store16(tm_lane + S::kP + 32 + half_ * 16, pl);
+        tm_wait_store();
+        hand_over();
+        __syncthreads();
+        if (tid == 0) {
+            tm_fence_after();
+            constexpr uint32_t kind = tm_f16(D, true);
+#pragma unroll 1
+            for (unsigned k = 0; k < kKeys / 16; ++k) {
+                const uint64_t v = tm_operand(vh_at + k * (D * 32), D * 16, 128);
+                tm_mma_t(tm, tm + S::kP + k * 8, v, kind, j || k);
+                tm_mma_t(tm, tm + S::kP + k * 8, tm_operand(vl_at + k * (D * 32), D * 16, 128), kind, true);
+                tm_mma_t(tm, tm + S::kP + 32 + k * 8, v, kind, true);
+            }
+            tm_commit(&bar_o);
+        }
+        if (j + 1 < steps) {
+            fail = !mbar_wait(&bar_raw, (j + 1) & 1);
+            if (!fail) unpack(j + 1, false, kh, kl);
+            hand_over();
+            fail = __syncthreads_or(fail);
+        }
+    }
+    if (!fail) fail = !mbar_wait(&bar_o, (steps - 1) & 1);
+    tm_fence_after();
+    row_top[half_][row] = sum;
+    if (__syncthreads_or(fail)) {
+        // some wait ran out: say so, let what is on its way land (each wait is bounded again), and give back what is held
+        if (tid == 0) {
+            tell(a.status, kServeWait);
+            for (unsigned i = 0; i < 2; ++i) mbar_wait(&bar_raw, i), mbar_wait(&bar_s, i), mbar_wait(&bar_o, i);
+        }
+    } else {
+        sum = row_top[0][row] + row_top[1][row];
+        const float f = sum == 0.0f ? 0.0f : 0x1p-14f / sum;
+        // a value that is not a number makes its block's dims so, in the rows that see it
+        unsigned nan_blocks = 0;
+        const unsigned nb = n_bad < kBadMax ? n_bad : kBadMax;
+        for (unsigned i = 0; i < nb; ++i)
+            if (int(bad[i] / 8) >= low && int(bad[i] / 8) <= pos) nan_blocks |= 1u << bad[i] % 8;
+        if (n_bad > kBadMax && pos >= 0) nan_blocks = ~0u;  // more than are remembered
+        const bool wide = ((reinterpret_cast<uintptr_t>(a.y) | a.y_stride * 4) & 15) == 0;
+        for (unsigned c = half_ * (D / 2); c < (half_ + 1) * (D / 2); c += 16) {
+            uint32_t o[16];
+            tm_load16(tm_lane + c, o);
+            if (!real) continue;
+            float v[16];
+#pragma unroll
+            for (unsigned e = 0; e < 16; ++e) v[e] = nan_blocks >> c / 32 & 1 ? __uint_as_float(0x7fc00000u) : sum == 0.0f ? 0.0f : __uint_as_float(o[e]) * f;
+            if (wide) {
+#pragma unroll
+                for (unsigned e = 0; e < 16; e += 4) *reinterpret_cast<float4 *>(y + c + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+            } else {
+#pragma unroll
+                for (unsigned e = 0; e < 16; ++e) y[c + e] = v[e];
+            }
+        }
+    }
+    tm_fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        tm_fence_after();
+        tm_free(tm, S::kCols);
+    }
+}
+
+template <int NB>
+cudaError_t launch_prompt(const Kv4AttnArgs &a, unsigned least_rows, cudaStream_t st) {
+    using S = Prompt<NB>;
+    const cudaError_t e = ensure_smem_attr(reinterpret_cast<const void *>(kv4_prompt_kernel<NB>), S::kSmem);
+    if (e != cudaSuccess) return e;
+    const unsigned long long rows = (unsigned long long)(a.max_q < a.n_rows ? a.max_q : a.n_rows) * (a.n_head / a.c.n_kv);
+    return launch_pdl(kv4_prompt_kernel<NB>, dim3(a.c.n_kv * a.n_req, unsigned((rows + kRows - 1) / kRows)), dim3(kThreads), S::kSmem, st, a, least_rows);
+}
+
+}  // namespace
+
+cudaError_t launch_kv4_prompt(const Kv4AttnArgs &a, unsigned least_rows, cudaStream_t st) {
+    switch (a.c.dim / 32) {
+    case 1: return launch_prompt<1>(a, least_rows, st);
+    case 2: return launch_prompt<2>(a, least_rows, st);
+    case 3: return launch_prompt<3>(a, least_rows, st);
+    case 4: return launch_prompt<4>(a, least_rows, st);
+    case 5: return launch_prompt<5>(a, least_rows, st);
+    case 6: return launch_prompt<6>(a, least_rows, st);
+    case 7: return launch_prompt<7>(a, least_rows, st);
+    case 8: return launch_prompt<8>(a, least_rows, st);
+    }
+    return cudaErrorInvalidValue;
+}
+
+}  // namespace b200q

@@ -245,7 +245,7 @@ void check_attn(Call &c, const b200q_kv4_pool *pool, unsigned n_rows, unsigned n
     c.need(n_req >= 1 && n_req <= kMaxAttnReq, "n_req is not 1 to 4096");
     c.need(n_rows <= (1u << 24), "n_rows is over 2^24");
     c.need(max_q >= 1 && max_q <= (1u << 24), "max_q is not 1 to 2^24");
-    c.need(max_kv >= 1 && max_kv <= (1u << 30), "max_kv is not 1 to 2^30");
+    c.need(max_kv >= 1 && max_kv <= (1u << 28), "max_kv is not 1 to 2^28");
 }
 
 Kv4AttnArgs attn_shape(const b200q_kv4_pool *pool, unsigned n_rows, unsigned n_head, unsigned n_req, unsigned max_q, unsigned max_kv) {

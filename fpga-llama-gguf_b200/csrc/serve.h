@@ -87,6 +87,8 @@ cudaError_t launch_kv4_store(const Kv4RowsArgs &a, cudaStream_t st);
 cudaError_t launch_kv4_load(const Kv4RowsArgs &a, cudaStream_t st);
 size_t kv4_attn_room(const Kv4AttnArgs &a, unsigned sms);  // 0: more work than one launch takes
 cudaError_t launch_kv4_attn(const Kv4AttnArgs &a, unsigned sms, cudaStream_t st);
+// requests of least_rows (token, head of the group) rows or more, on tcgen05; the others are left out
+cudaError_t launch_kv4_prompt(const Kv4AttnArgs &a, unsigned least_rows, cudaStream_t st);
 size_t beam_select_room(const BeamSelectArgs &a);
 cudaError_t launch_beam_select(const BeamSelectArgs &a, cudaStream_t st);
 cudaError_t launch_beam_reorder(const BeamReorderArgs &a, cudaStream_t st);
