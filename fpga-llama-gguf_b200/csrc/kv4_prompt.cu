@@ -12,13 +12,12 @@
 // w_t = 2^(s_t + log2 e_t - m), and the sum of the weights takes w_t / e_t.
 //
 // Operands: qh, kh, kl, vh, vl in shared memory (no swizzle; K is K-major, V MN-major, both written 16 bytes = 8 dims of a
-// key at a time by the same code), ql and P in tensor memory. In a step all 8 warps
+// key at a time by the same code), ql and P in tensor memory. kl lies behind kh, so that one product of N 128 forms qh kh and
+// qh kl side by side and qh, whose reads bound the products of N 64, is read once for both. In a step 8 warps
 //   unpack V    while the tensor cores form S
-//   soften      S from tensor memory, P back (lane = row; two warps share a row's 64 keys)
+//   soften      S from tensor memory, P back into its place (lane = row; two warps share a row's 64 keys)
 //   unpack the next K    while the tensor cores add P V
-// and a bulk copy brings the next raw tiles as soon as V is unpacked.
-// Bound: per step 128 x 64 x D x 6 products; at D 256 shared memory (the operands' 320 KB and the unpacked tiles' 128 KB at
-// 128 bytes a cycle) is about as long as the tensor cores' work.
+// A ninth warp issues the products (which holds it up while the tensor cores are busy) and the raw tiles' bulk copies.
 #include <cuda_runtime.h>
 
 #include "common.cuh"
@@ -30,7 +29,7 @@
 namespace b200q {
 namespace {
 
-constexpr unsigned kRows = 128, kKeys = 64, kThreads = 256;
+constexpr unsigned kRows = 128, kKeys = 64, kWork = 256, kThreads = kWork + 32;  // 8 warps, and one that issues products and copies
 constexpr unsigned kBadMax = 96;  // values that are not numbers, remembered by (key, block)
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -51,17 +50,33 @@ struct Prompt {
     static constexpr int D = NB * 32, kTile = NB * 576;
     static constexpr int kQ = kRows * D * 2, kPart = kKeys * D * 2;
     static constexpr int kRaw = kQ + 4 * kPart, kSmem = kRaw + 4 * kTile;
-    static constexpr unsigned kS = D, kP = D + 64, kQl = D + 128, kNeed = D + 128 + D / 2;  // columns of tensor memory
+    // columns of tensor memory: O, S (qh kh + ql kh, then qh kl; P takes the place of the former, 32 keys' upper and lower
+    // parts by 16 columns), ql
+    static constexpr unsigned kS = D, kQl = D + 128, kNeed = D + 128 + D / 2;
     static constexpr unsigned kCols = kNeed <= 256 ? 256 : 512;
     static_assert(kNeed <= 512 && kSmem <= 216 * 1024);
 };
+
+__device__ __forceinline__ void work_sync() { asm volatile("barrier.cta.sync 1, %0;" ::"n"(kWork) : "memory"); }
+__device__ __forceinline__ bool work_sync_or(bool x) {
+    uint32_t y;
+    asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n barrier.cta.red.or.pred q, 1, %2, p;\n selp.u32 %0, 1, 0, q;\n}"
+                 : "=r"(y)
+                 : "r"(uint32_t(x)), "n"(kWork)
+                 : "memory");
+    return y;
+}
+__device__ __forceinline__ void arrive(uint64_t *bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
 
 template <int NB>
 __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnArgs a, unsigned least_rows) {
     using S = Prompt<NB>;
     constexpr int D = S::D;
     extern __shared__ __align__(1024) uint8_t smem[];
-    __shared__ uint64_t bar_s, bar_o, bar_raw;
+    // S formed, P V added, raw tiles there; K unpacked, V unpacked (and the raw tiles read), P stored: an arrival a warp
+    __shared__ uint64_t bar_s, bar_o, bar_raw, bar_k, bar_v, bar_p;
     __shared__ uint32_t tm_base;
     __shared__ __align__(16) float k_scale[kKeys], v_log[kKeys], v_inv[kKeys];  // read four at a time
     __shared__ float row_top[2][kRows];
@@ -83,13 +98,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnAr
     const int lo = a.window && first_pos >= 0 && unsigned(first_pos) + 1 > a.window ? first_pos + 1 - int(a.window) : 0;
 
     // this thread's row (lane of tensor memory), and its half of the keys or dims
-    const unsigned quarter = warp & 3, half_ = warp >> 2, row = quarter * 32 + lane, at_row = row0 + row;
+    const unsigned quarter = warp & 3, half_ = warp >> 2 & 1, row = quarter * 32 + lane, at_row = row0 + row;
     const bool real = at_row < all;
     const int pos = real ? base + int(at_row / per) : -1;
     const int low = a.window && pos >= 0 && unsigned(pos) + 1 > a.window ? pos + 1 - int(a.window) : 0;
     float *y = a.y + (start + (real ? at_row / per : 0)) * a.y_stride + size_t(head * per + (real ? at_row % per : 0)) * D;
     if (hi < 0) {  // no row of the tile sees anything
-        if (real)
+        if (real && warp < kWork / 32)
             for (unsigned d = 0; d < D / 2; ++d) y[half_ * (D / 2) + d] = 0.0f;
         return;
     }
@@ -100,6 +115,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnAr
         mbar_init(&bar_s, 1);
         mbar_init(&bar_o, 1);
         mbar_init(&bar_raw, 1);
+        mbar_init(&bar_k, kWork / 32);
+        mbar_init(&bar_v, kWork / 32);
+        mbar_init(&bar_p, kWork / 32);
         mbar_fence_init();
         n_bad = 0;
     }
@@ -109,31 +127,70 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnAr
     const uint32_t tm = tm_base, tm_lane = tm + (quarter * 32 << 16);
     uint8_t *const kh = smem + S::kQ, *const kl = kh + S::kPart, *const vh = kl + S::kPart, *const vl = vh + S::kPart, *const raw = smem + S::kRaw;
 
-    // the raw tiles of step j (warp 0): a bulk copy each, those behind the last key or without a page left out
-    const unsigned tiles_per_page = a.c.page / kTileTokens;
-    auto fetch = [&](unsigned j) {
-        const unsigned tile = (step0 + j) * (kKeys / kTileTokens) + lane;
-        const uint8_t *src = nullptr;
-        if (lane < kKeys / kTileTokens && int(tile * kTileTokens) <= hi) {
-            const unsigned page = a.table[size_t(req) * a.stride + tile / tiles_per_page];
-            if (page < a.c.n_pages)
-                src = a.c.base + ((size_t(page) * a.c.n_kv + head) * tiles_per_page + tile % tiles_per_page) * S::kTile;
-            else tell(a.status, kServePage);
+    const uint32_t q_at = smem_addr(smem), kh_at = smem_addr(kh), vh_at = smem_addr(vh), vl_at = smem_addr(vl);
+    bool fail = false;
+    if (warp == kWork / 32) {
+        // the warp that issues: raw tiles (a bulk copy each, those behind the last key or without a page left out) and products
+        const unsigned tiles_per_page = a.c.page / kTileTokens;
+        const uint8_t *src;
+        auto look_up = [&](unsigned j) {
+            const unsigned tile = (step0 + j) * (kKeys / kTileTokens) + lane;
+            src = nullptr;
+            if (j < steps && lane < kKeys / kTileTokens && int(tile * kTileTokens) <= hi) {
+                const unsigned page = a.table[size_t(req) * a.stride + tile / tiles_per_page];
+                if (page < a.c.n_pages)
+                    src = a.c.base + ((size_t(page) * a.c.n_kv + head) * tiles_per_page + tile % tiles_per_page) * S::kTile;
+                else tell(a.status, kServePage);
+            }
+        };
+        auto fetch = [&] {
+            const unsigned there = __ballot_sync(~0u, src != nullptr);
+            if (lane == 0) {
+                present = there;
+                mbar_expect_tx(&bar_raw, __popc(there) * S::kTile);
+            }
+            __syncwarp();
+            if (src)
+                asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                                 smem_addr(raw + lane * S::kTile)),
+                             "l"(src), "r"(S::kTile), "r"(smem_addr(&bar_raw))
+                             : "memory");
+        };
+        auto reached = [&](uint64_t *bar, unsigned phase) { return __all_sync(~0u, mbar_wait(bar, phase & 1)); };
+        look_up(0);
+        fetch();
+        for (unsigned j = 0; j < steps && !fail; ++j) {
+            look_up(j + 1);
+            if ((fail = !reached(&bar_k, j) || (j && !reached(&bar_o, j - 1)))) break;  // (S takes P's place)
+            tm_fence_after();
+            if (lane == 0) {
+#pragma unroll 1
+                for (unsigned k = 0; k < D / 16; ++k) {
+                    const uint64_t kk = tm_operand(kh_at + k * 256, 128, D * 16);
+                    tm_mma(tm + S::kS, tm_operand(q_at + k * 256, 128, D * 16), kk, tm_f16(2 * kKeys, false), k != 0);
+                    tm_mma_t(tm + S::kS, tm + S::kQl + k * 8, kk, tm_f16(kKeys, false), true);
+                }
+                tm_commit(&bar_s);
+            }
+            __syncwarp();
+            if ((fail = !reached(&bar_v, j))) break;
+            if (j + 1 < steps) fetch();
+            if ((fail = !reached(&bar_p, j))) break;
+            tm_fence_after();
+            if (lane == 0) {
+#pragma unroll 1
+                for (unsigned k = 0; k < kKeys / 16; ++k) {
+                    const uint64_t v = tm_operand(vh_at + k * (D * 32), D * 16, 128);
+                    const uint32_t p = tm + S::kS + k / 2 * 32 + k % 2 * 8;
+                    tm_mma_t(tm, p, v, tm_f16(D, true), j || k);
+                    tm_mma_t(tm, p, tm_operand(vl_at + k * (D * 32), D * 16, 128), tm_f16(D, true), true);
+                    tm_mma_t(tm, p + 16, v, tm_f16(D, true), true);
+                }
+                tm_commit(&bar_o);
+            }
+            __syncwarp();
         }
-        const unsigned there = __ballot_sync(~0u, src != nullptr);
-        if (lane == 0) {
-            present = there;
-            mbar_expect_tx(&bar_raw, __popc(there) * S::kTile);
-        }
-        __syncwarp();
-        if (src)
-            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                             smem_addr(raw + lane * S::kTile)),
-                         "l"(src), "r"(S::kTile), "r"(smem_addr(&bar_raw))
-                         : "memory");
-    };
-    if (warp == 0) fetch(0);
-
+    } else {
     // Q: rows scaled to below 2^11; the upper parts to shared memory, the lower ones to tensor memory
     float row_scale;
     {
@@ -150,7 +207,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnAr
             top = fmaxf(top, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
         }
         row_top[half_][row] = top;
-        __syncthreads();
+        work_sync();
         top = fmaxf(row_top[0][row], row_top[1][row]);
         int ex = int(__float_as_uint(top) >> 23) - 127 - 10;
         ex = ex < -110 ? -110 : ex > 110 ? 110 : ex;
@@ -241,42 +298,30 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnAr
             }
         }
     };
-    auto hand_over = [&] {  // what this thread wrote, to the tensor cores
+    auto hand_over = [&](uint64_t *bar) {  // what this warp wrote, to the issuing warp and the tensor cores
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         tm_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive(bar);
     };
 
-    bool fail = !mbar_wait(&bar_raw, 0);
+    fail = !mbar_wait(&bar_raw, 0);
     if (!fail) unpack(0, false, kh, kl);
-    hand_over();
-    fail = __syncthreads_or(fail);
-    const uint32_t q_at = smem_addr(smem), kh_at = smem_addr(kh), kl_at = smem_addr(kl), vh_at = smem_addr(vh), vl_at = smem_addr(vl);
+    hand_over(&bar_k);
     float top = -INFINITY, sum = 0.0f;
     unsigned j = 0;
-    for (; j < steps && !fail; ++j) {
-        if (tid == 0) {
-            tm_fence_after();
-            constexpr uint32_t kind = tm_f16(kKeys, false);
-#pragma unroll 1
-            for (unsigned k = 0; k < D / 16; ++k) {
-                const uint64_t q = tm_operand(q_at + k * 256, 128, D * 16), kk = tm_operand(kh_at + k * 256, 128, D * 16);
-                tm_mma(tm + S::kS, q, kk, kind, k != 0);
-                tm_mma(tm + S::kS, q, tm_operand(kl_at + k * 256, 128, D * 16), kind, true);
-                tm_mma_t(tm + S::kS, tm + S::kQl + k * 8, kk, kind, true);
-            }
-            tm_commit(&bar_s);
-        }
-        if (j) fail = !mbar_wait(&bar_o, (j - 1) & 1);  // P and V are free
+    for (; j < steps; ++j) {
+        if (j && !fail) fail = !mbar_wait(&bar_o, (j - 1) & 1);  // V is free
         if (!fail) unpack(j, true, vh, vl);
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // (the raw tiles are read: the next copies may come)
-        if ((fail = __syncthreads_or(fail))) break;
-        if (warp == 0 && j + 1 < steps) fetch(j + 1);
+        hand_over(&bar_v);
 
         // scores of the row and 32 keys, in powers of two
-        fail = !mbar_wait(&bar_s, j & 1);
+        if (!fail) fail = !mbar_wait(&bar_s, j & 1);
+        if ((fail = work_sync_or(fail))) break;  // (and all keys' scales are there)
         tm_fence_after();
-        uint32_t s[32];
+        uint32_t s[32], s_low[32];
         tm_load32(tm_lane + S::kS + half_ * 32, s);
+        tm_load32(tm_lane + S::kS + kKeys + half_ * 32, s_low);
         const int key0 = int((step0 + j) * kKeys + half_ * 32);
         float mx = -INFINITY;
         const bool edge = __any_sync(~0u, key0 < low || key0 + 31 > pos);
@@ -286,7 +331,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnAr
             const float f[4] = {ks.x, ks.y, ks.z, ks.w}, g[4] = {vg.x, vg.y, vg.z, vg.w};
 #pragma unroll
             for (unsigned e = 0; e < 4; ++e) {
-                float t = fmaf(__uint_as_float(s[i + e]) * f[e], row_scale, g[e]);
+                float t = fmaf((__uint_as_float(s[i + e]) + __uint_as_float(s_low[i + e])) * f[e], row_scale, g[e]);
                 if (edge && (key0 + int(i + e) < low || key0 + int(i + e) > pos)) t = -INFINITY;
                 if (g[e] == -INFINITY) t = -INFINITY;
                 mx = fmaxf(mx, t);
@@ -294,7 +339,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnAr
             }
         }
         row_top[half_][row] = mx;
-        if ((fail = __syncthreads_or(fail))) break;
+        work_sync();
         mx = fmaxf(mx, row_top[half_ ^ 1][row]);
         if (__any_sync(~0u, mx > top)) {  // a higher maximum: 4 above the score, so that it moves seldom
             const float nt = mx > top ? mx + 4.0f : top, f = top == nt ? 1.0f : exp2_fast(top - nt);
@@ -331,34 +376,21 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnAr
                 pl[(i + e) / 2] = h2(__floats2half2_rn(w[e] - b.x, w[e + 1] - b.y));
             }
         }
-        tm_store16(tm_lane + S::kP + half_ * 16, ph);
-        tm_store16(tm_lane + S::kP + 32 + half_ * 16, pl);
+        tm_store16(tm_lane + S::kS + half_ * 32, ph);
+        tm_store16(tm_lane + S::kS + half_ * 32 + 16, pl);
         tm_wait_store();
-        hand_over();
-        __syncthreads();
-        if (tid == 0) {
-            tm_fence_after();
-            constexpr uint32_t kind = tm_f16(D, true);
-#pragma unroll 1
-            for (unsigned k = 0; k < kKeys / 16; ++k) {
-                const uint64_t v = tm_operand(vh_at + k * (D * 32), D * 16, 128);
-                tm_mma_t(tm, tm + S::kP + k * 8, v, kind, j || k);
-                tm_mma_t(tm, tm + S::kP + k * 8, tm_operand(vl_at + k * (D * 32), D * 16, 128), kind, true);
-                tm_mma_t(tm, tm + S::kP + 32 + k * 8, v, kind, true);
-            }
-            tm_commit(&bar_o);
-        }
+        hand_over(&bar_p);
         if (j + 1 < steps) {
             fail = !mbar_wait(&bar_raw, (j + 1) & 1);
             if (!fail) unpack(j + 1, false, kh, kl);
-            hand_over();
-            fail = __syncthreads_or(fail);
+            hand_over(&bar_k);
         }
     }
     if (!fail) fail = !mbar_wait(&bar_o, (steps - 1) & 1);
     tm_fence_after();
+    work_sync();  // (the last maxima are read)
     row_top[half_][row] = sum;
-    if (__syncthreads_or(fail)) {
+    if (work_sync_or(fail)) {
         // some wait ran out: say so, let what is on its way land (each wait is bounded again), and give back what is held
         if (tid == 0) {
             tell(a.status, kServeWait);
@@ -389,6 +421,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnAr
                 for (unsigned e = 0; e < 16; ++e) y[c + e] = v[e];
             }
         }
+    }
     }
     tm_fence_before();
     __syncthreads();
