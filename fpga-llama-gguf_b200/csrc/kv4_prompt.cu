@@ -43,6 +43,28 @@ __device__ __forceinline__ float exp2_fast(float x) {
 }
 __device__ __forceinline__ uint32_t h2(half2 x) { return *reinterpret_cast<uint32_t *>(&x); }
 __device__ __forceinline__ half2 as_h2(uint32_t x) { return *reinterpret_cast<half2 *>(&x); }
+// two FP32 operations in one instruction
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x;\n}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mul.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x;\n}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n fma.rn.f32x2 x, x, y, z;\n mov.b64 {%0, %1}, x;\n}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float(unsigned(127 + e) << 23); }
 
 template <int NB>
@@ -191,47 +213,65 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnAr
             __syncwarp();
         }
     } else {
-    // Q: rows scaled to below 2^11; the upper parts to shared memory, the lower ones to tensor memory
+    // Q: rows scaled to below 2^11; the upper parts to shared memory, the lower ones to tensor memory, by way of V's place.
+    // A warp takes a row at a time, its lanes four dims each.
     float row_scale;
     {
-        const float *q = a.q + (start + (real ? at_row / per : 0)) * a.q_stride + (head * per + (real ? at_row % per : 0)) * a.q_head_stride;
         const bool wide = ((reinterpret_cast<uintptr_t>(a.q) | a.q_stride * 4 | a.q_head_stride * 4) & 15) == 0;
-        auto load4 = [&](unsigned d) {
-            if (!real) return make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (wide) return *reinterpret_cast<const float4 *>(q + d);
-            return make_float4(q[d], q[d + 1], q[d + 2], q[d + 3]);
-        };
-        float top = 0.0f;
-        for (unsigned d = half_ * (D / 2); d < (half_ + 1) * (D / 2); d += 4) {
-            const float4 v = load4(d);
-            top = fmaxf(top, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+        constexpr unsigned kTurns = (D / 4 + 31) / 32, kAhead = 4;  // rows whose loads are on their way together
+        for (unsigned r0 = warp; r0 < kRows; r0 += kAhead * (kWork / 32)) {
+            float4 v[kAhead][kTurns];
+#pragma unroll
+            for (unsigned i = 0; i < kAhead; ++i) {
+                const unsigned at = row0 + r0 + i * (kWork / 32);
+                const float *q = a.q + (start + (at < all ? at / per : 0)) * a.q_stride + (head * per + (at < all ? at % per : 0)) * a.q_head_stride;
+#pragma unroll
+                for (unsigned n = 0; n < kTurns; ++n) {
+                    const unsigned d = (n * 32 + lane) * 4;
+                    v[i][n] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    if (at >= all || d >= D) continue;
+                    if (wide) v[i][n] = *reinterpret_cast<const float4 *>(q + d);
+                    else v[i][n] = make_float4(q[d], q[d + 1], q[d + 2], q[d + 3]);
+                }
+            }
+#pragma unroll
+            for (unsigned i = 0; i < kAhead; ++i) {
+                const unsigned r = r0 + i * (kWork / 32);
+                float top = 0.0f;
+#pragma unroll
+                for (unsigned n = 0; n < kTurns; ++n)
+                    top = fmaxf(top, fmaxf(fmaxf(fabsf(v[i][n].x), fabsf(v[i][n].y)), fmaxf(fabsf(v[i][n].z), fabsf(v[i][n].w))));
+                for (unsigned x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, x));
+                int ex = int(__float_as_uint(top) >> 23) - 127 - 10;
+                ex = ex < -110 ? -110 : ex > 110 ? 110 : ex;
+                const float down = pow2(-ex);
+                if (lane == 0) row_top[0][r] = a.scale * kLog2e * pow2(ex);
+#pragma unroll
+                for (unsigned n = 0; n < kTurns; ++n) {
+                    const unsigned d = (n * 32 + lane) * 4;
+                    if (d >= D) continue;
+                    const float4 y = make_float4(v[i][n].x * down, v[i][n].y * down, v[i][n].z * down, v[i][n].w * down);
+                    const half2 p = __floats2half2_rn(y.x, y.y), q = __floats2half2_rn(y.z, y.w);
+                    const float2 bp = __half22float2(p), bq = __half22float2(q);
+                    const unsigned at = r / 8 * (D * 16) + d / 8 * 128 + r % 8 * 16 + d % 8 * 2;
+                    *reinterpret_cast<uint2 *>(smem + at) = make_uint2(h2(p), h2(q));
+                    *reinterpret_cast<uint2 *>(vh + at) = make_uint2(h2(__floats2half2_rn(y.x - bp.x, y.y - bp.y)), h2(__floats2half2_rn(y.z - bq.x, y.w - bq.y)));
+                }
+            }
         }
-        row_top[half_][row] = top;
         work_sync();
-        top = fmaxf(row_top[0][row], row_top[1][row]);
-        int ex = int(__float_as_uint(top) >> 23) - 127 - 10;
-        ex = ex < -110 ? -110 : ex > 110 ? 110 : ex;
-        row_scale = a.scale * kLog2e * pow2(ex);
-        const float down = pow2(-ex);
+        row_scale = row_top[0][row];
         for (unsigned d = half_ * (D / 2); d < (half_ + 1) * (D / 2); d += 16) {
             uint32_t low_part[8];
 #pragma unroll
             for (unsigned g = 0; g < 2; ++g) {
-                uint32_t up[4];
-#pragma unroll
-                for (unsigned e = 0; e < 2; ++e) {
-                    const float4 v = load4(d + g * 8 + e * 4);
-                    const half2 x = __floats2half2_rn(v.x * down, v.y * down), z = __floats2half2_rn(v.z * down, v.w * down);
-                    const float2 bx = __half22float2(x), bz = __half22float2(z);
-                    up[2 * e] = h2(x), up[2 * e + 1] = h2(z);
-                    low_part[g * 4 + 2 * e] = h2(__floats2half2_rn(v.x * down - bx.x, v.y * down - bx.y));
-                    low_part[g * 4 + 2 * e + 1] = h2(__floats2half2_rn(v.z * down - bz.x, v.w * down - bz.y));
-                }
-                *reinterpret_cast<uint4 *>(smem + row / 8 * (D * 16) + (d / 8 + g) * 128 + row % 8 * 16) = make_uint4(up[0], up[1], up[2], up[3]);
+                const uint4 x = *reinterpret_cast<const uint4 *>(vh + row / 8 * (D * 16) + (d / 8 + g) * 128 + row % 8 * 16);
+                low_part[4 * g] = x.x, low_part[4 * g + 1] = x.y, low_part[4 * g + 2] = x.z, low_part[4 * g + 3] = x.w;
             }
             tm_store8(tm_lane + S::kQl + d / 2, low_part);
         }
         tm_wait_store();
+        work_sync();  // (V's place and row_top are read)
     }
 
     // Raw tiles to FP16 pairs of operands. A warp takes 8 keys, a lane a key and every fourth block.
@@ -325,19 +365,30 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnAr
         const int key0 = int((step0 + j) * kKeys + half_ * 32);
         float mx = -INFINITY;
         const bool edge = __any_sync(~0u, key0 < low || key0 + 31 > pos);
+        const float2 scale2 = make_float2(row_scale, row_scale);
+        float2 w[16];
 #pragma unroll
-        for (unsigned i = 0; i < 32; i += 4) {
-            const float4 ks = *reinterpret_cast<const float4 *>(k_scale + half_ * 32 + i), vg = *reinterpret_cast<const float4 *>(v_log + half_ * 32 + i);
-            const float f[4] = {ks.x, ks.y, ks.z, ks.w}, g[4] = {vg.x, vg.y, vg.z, vg.w};
+        for (unsigned i = 0; i < 16; i += 2) {
+            const float4 ks = *reinterpret_cast<const float4 *>(k_scale + half_ * 32 + 2 * i), vg = *reinterpret_cast<const float4 *>(v_log + half_ * 32 + 2 * i);
+            const float2 f[2] = {make_float2(ks.x, ks.y), make_float2(ks.z, ks.w)}, g[2] = {make_float2(vg.x, vg.y), make_float2(vg.z, vg.w)};
 #pragma unroll
-            for (unsigned e = 0; e < 4; ++e) {
-                float t = fmaf((__uint_as_float(s[i + e]) + __uint_as_float(s_low[i + e])) * f[e], row_scale, g[e]);
-                if (edge && (key0 + int(i + e) < low || key0 + int(i + e) > pos)) t = -INFINITY;
-                if (g[e] == -INFINITY) t = -INFINITY;
-                mx = fmaxf(mx, t);
-                s[i + e] = __float_as_uint(t);
+            for (unsigned e = 0; e < 2; ++e) {
+                const unsigned k = 2 * (i + e);
+                const float2 x = add2(make_float2(__uint_as_float(s[k]), __uint_as_float(s[k + 1])),
+                                      make_float2(__uint_as_float(s_low[k]), __uint_as_float(s_low[k + 1])));
+                w[i + e] = fma2(mul2(x, f[e]), scale2, g[e]);  // (a hidden key: -inf)
             }
         }
+        if (edge) {
+#pragma unroll
+            for (unsigned i = 0; i < 16; ++i) {
+                const int key = key0 + int(2 * i);
+                if (key < low || key > pos) w[i].x = -INFINITY;
+                if (key + 1 < low || key + 1 > pos) w[i].y = -INFINITY;
+            }
+        }
+#pragma unroll
+        for (unsigned i = 0; i < 16; ++i) mx = fmaxf(mx, fmaxf(w[i].x, w[i].y));
         row_top[half_][row] = mx;
         work_sync();
         mx = fmaxf(mx, row_top[half_ ^ 1][row]);
@@ -355,27 +406,24 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnAr
                 }
             }
         }
-        const float ref = top == -INFINITY ? 0.0f : top;
+        const float lift = top == -INFINITY ? 0.0f : 14.0f - top;  // weights up to 2^14
         uint32_t ph[16], pl[16];
+        float2 sum2 = make_float2(0.0f, 0.0f);
 #pragma unroll
-        for (unsigned i = 0; i < 32; i += 4) {
-            const float4 vi = *reinterpret_cast<const float4 *>(v_inv + half_ * 32 + i);
-            const float g[4] = {vi.x, vi.y, vi.z, vi.w};
-            float w[4];
+        for (unsigned i = 0; i < 16; i += 2) {
+            const float4 vi = *reinterpret_cast<const float4 *>(v_inv + half_ * 32 + 2 * i);
+            const float2 g[2] = {make_float2(vi.x, vi.y), make_float2(vi.z, vi.w)};
 #pragma unroll
-            for (unsigned e = 0; e < 4; ++e) {
-                w[e] = exp2_fast(__uint_as_float(s[i + e]) - ref);
-                sum = fmaf(w[e], g[e], sum);
-                w[e] *= 0x1p14f;
-            }
-#pragma unroll
-            for (unsigned e = 0; e < 4; e += 2) {
-                const half2 h = __floats2half2_rn(w[e], w[e + 1]);
-                const float2 b = __half22float2(h);
-                ph[(i + e) / 2] = h2(h);
-                pl[(i + e) / 2] = h2(__floats2half2_rn(w[e] - b.x, w[e + 1] - b.y));
+            for (unsigned e = 0; e < 2; ++e) {
+                const float2 x = add2(w[i + e], make_float2(lift, lift)), y = make_float2(exp2_fast(x.x), exp2_fast(x.y));
+                sum2 = fma2(y, g[e], sum2);
+                const half2 h = __floats2half2_rn(y.x, y.y);
+                const float2 b = __half22float2(h), z = add2(y, make_float2(-b.x, -b.y));
+                ph[i + e] = h2(h);
+                pl[i + e] = h2(__floats2half2_rn(z.x, z.y));
             }
         }
+        sum += sum2.x + sum2.y;
         tm_store16(tm_lane + S::kS + half_ * 32, ph);
         tm_store16(tm_lane + S::kS + half_ * 32 + 16, pl);
         tm_wait_store();
@@ -398,7 +446,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnAr
         }
     } else {
         sum = row_top[0][row] + row_top[1][row];
-        const float f = sum == 0.0f ? 0.0f : 0x1p-14f / sum;
+        const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
         // a value that is not a number makes its block's dims so, in the rows that see it
         unsigned nan_blocks = 0;
         const unsigned nb = n_bad < kBadMax ? n_bad : kBadMax;
