@@ -27,6 +27,7 @@ OP_GEMV, OP_RMSNORM, OP_ADD, OP_SILU_MUL, OP_MUL, OP_UNARY, OP_GDN, OP_CONV = 1,
 OP_STATE_LOAD, OP_ROPE, OP_TRACE = 9, 10, 11
 OP_ATTN, OP_ARGMAX, OP_GET_ROW, OP_ALLREDUCE, OP_ALLGATHER = 12, 13, 14, 15, 16  # extensions of this library
 OP_GEMV_BATCH = 17
+OP_BLOCK_MAP, OP_KV4_STORE, OP_KV4_ATTN, OP_BEAM_SELECT, OP_BEAM_REORDER, OP_KV4_REORDER = 18, 19, 20, 21, 22, 23
 BATCH_MAX = 8  # activation rows of one gemv_batch_kernel launch (more: the tensor-core GEMM)
 GEMV_SWIGLU, GEMV_CONV, GEMV_ADD = 0x100, 0x200, 0x400
 GDN_WITH_GEMV, GDN_L2_QK, GDN_GATED, GDN_GATES, GDN_WITH_OUT = 1, 2, 4, 8, 16
@@ -34,7 +35,7 @@ NORM_L2, NORM_NO_WEIGHT, NORM_DEFER = 1, 2, 4
 UNARY_SILU, UNARY_SIGMOID, UNARY_SOFTPLUS, UNARY_COPY = 1, 2, 3, 4
 SILU_MUL_SIGMOID = 1
 Q4_0, Q4_1, Q8_0, Q5_K, Q6_K = 2, 3, 8, 13, 14
-FEATURES = (0x6B51FFFF, 0x6B520001, 0x6B53007F)
+FEATURES = (0x6B51FFFF, 0x6B520001, 0x6B5300FF)
 COMM_EXPLICIT = 1
 UPLOAD_REPLICATE = 1
 UPLOAD_SRC_Q4_0X8 = 2
@@ -153,6 +154,53 @@ def gemv_batch(fmt: int, rows: int, cols: int, w_off: int, x_off: int, y_off: in
     for all rows; more rows run as the tensor-core GEMM (prefill)."""
     return cmd(OP_GEMV_BATCH, fmt | flags | ((batch - 1) << 16), rows, cols, w_off & 0xFFFFFFFF, w_off >> 32,
                x_off, y_off)
+
+
+def kv4_geometry(n_kv: int, head_dim: int, page: int) -> int:
+    """The geometry word of a 4-bit cache: n_kv | (head_dim / 32) << 8 | (page_tokens / 16) << 16."""
+    return n_kv | (head_dim // 32) << 8 | (page // 16) << 16
+
+
+def block_map_cmd(n_req: int, past: int, fresh: int, table: int, stride: int, free_pages: int, n_free: int, cursor: int,
+                  kv_len: int, q_start: int, slots: int, positions: int, n_rows: int, page: int) -> np.ndarray:
+    """BLOCK_MAP: block tables, slots, positions and row starts of a step, from the requests' lengths (uint32 in act)."""
+    return cmd_list(cmd(OP_BLOCK_MAP, n_req, past, fresh, table, stride, free_pages, n_free),
+                    cmd(cursor, kv_len, q_start, slots, positions, n_rows, page))
+
+
+def kv4_store_cmd(n: int, k: int, v: int, slots: int, geometry: int, pool: int, n_pages: int, k_stride: int = 0,
+                  v_stride: int = 0) -> np.ndarray:
+    """KV4_STORE: n rows of K and V quantized into their slots of the pool at byte `pool` of the KV buffer."""
+    return cmd_list(cmd(OP_KV4_STORE, n, k, v, slots, k_stride, v_stride, geometry), cmd(pool // 256, n_pages))
+
+
+def kv4_attn_cmd(n_head: int, q: int, y: int, table: int, stride: int, q_start: int, kv_len: int, n_req: int, n_rows: int,
+                 max_q: int, max_kv: int, scale: float, geometry: int, pool: int, n_pages: int, window: int = 0,
+                 q_stride: int = 0, q_head_stride: int = 0, y_stride: int = 0) -> np.ndarray:
+    """KV4_ATTN: causal attention of every request's new rows over its pages of the 4-bit cache."""
+    return cmd_list(cmd(OP_KV4_ATTN, n_head, q, y, table, stride, q_start, kv_len),
+                    cmd(n_req, n_rows, max_q, max_kv, fbits(scale), window, q_stride, q_head_stride),
+                    cmd(geometry, pool // 256, n_pages, y_stride))
+
+
+def beam_select_cmd(n_req: int, beams: int, vocab: int, logits: int, scores: int, n_out: int, out_scores: int,
+                    out_parent: int, out_token: int, logits_stride: int = 0) -> np.ndarray:
+    """BEAM_SELECT: the n_out best (parent beam, token) of each request."""
+    return cmd_list(cmd(OP_BEAM_SELECT, n_req, beams, vocab, logits, logits_stride, scores, n_out),
+                    cmd(out_scores, out_parent, out_token))
+
+
+def beam_reorder_cmd(n_req: int, beams: int, parent: int, src_row: int, dst_row: int, rows: int, n_layers: int = 1,
+                     layer_rows: int = 0) -> np.ndarray:
+    """BEAM_REORDER: state rows (`rows` of a beam and layer) moved to their beams' parents."""
+    return cmd_list(cmd(OP_BEAM_REORDER, n_req, beams, parent, src_row, dst_row, rows, n_layers), cmd(layer_rows))
+
+
+def kv4_reorder_cmd(n_req: int, beams: int, table: int, stride: int, kv_len: int, parent: int, geometry: int, pool: int,
+                    n_pages: int, n_layers: int = 1, layer_bytes: int = 0) -> np.ndarray:
+    """KV4_REORDER: block tables and tail pages of every layer moved to their beams' parents, in place."""
+    return cmd_list(cmd(OP_KV4_REORDER, n_req, beams, table, stride, kv_len, parent, geometry),
+                    cmd(pool // 256, n_pages, n_layers, layer_bytes // 256))
 
 
 # ---- library ---------------------------------------------------------------------------------------------------

@@ -22,6 +22,7 @@
 #include "launch.h"
 #include "layout.h"
 #include "plan.h"
+#include "serve.h"
 
 using namespace b200q;
 
@@ -76,6 +77,7 @@ constexpr size_t kSnapFloats = size_t(1) << 20;  // snapshot scratch (overlappin
 constexpr unsigned kMaxTraceEvents = 4096;
 // device words after the status words: per-KV-head chunk counters of ATTN, the ARGMAX combine slot
 constexpr unsigned kSyncAttnWord = 256, kSyncArgmaxWord = 512;
+constexpr unsigned kServeStatusWord = 2;  // of the status words: B200Q_SERVE_* bits of the commands for several sequences
 constexpr size_t kAttnPartFloats = size_t(1) << 22;  // ATTN chunk outputs (16 MiB)
 
 // B200Q_FEATURE_MASK bits that switch the executor's fusions off (include/b200q.h): the reference's feature bits
@@ -121,6 +123,10 @@ struct b200q_ctx {
     uint8_t *gemm_img = nullptr;
     size_t gemm_img_bytes = 0;
     std::vector<uint8_t *> gemm_img_old;
+    // workspace of KV4_ATTN and BEAM_SELECT commands, kept the same way (the context's lists run one after another)
+    uint8_t *serve_room = nullptr;
+    size_t serve_room_bytes = 0;
+    std::vector<uint8_t *> serve_room_old;
     int32_t *gemm_sums = nullptr;  // debug: where the next GEMM stores its first block's integer sums
     float *snap = nullptr;
     size_t snap_used = 0;
@@ -633,7 +639,146 @@ int exec_gdn(b200q_ctx *c, const Pass &p, const ImageLink &nsq_link) {
     return 0;
 }
 
+// ---- several sequences (opcodes 18 .. 23) ---------------------------------------------------------------------------
+uint32_t *words_at(b200q_ctx *c, uint32_t off) { return reinterpret_cast<uint32_t *>(c->act) + off; }
+Kv4View pool_at(b200q_ctx *c, uint32_t geo, uint32_t pool, uint32_t n_pages) {
+    Kv4View v;
+    v.base = reinterpret_cast<uint8_t *>(c->kv) + size_t(pool) * 256;
+    v.n_pages = n_pages;
+    v.n_kv = geo & 0xffu;
+    v.dim = (geo >> 8 & 0xffu) * 32u;
+    v.page = (geo >> 16) * 16u;
+    return v;
+}
+Kv4AttnArgs kv4_attn_args(b200q_ctx *c, const Pass &p) {
+    const uint32_t *w = p.cmd[0], *x = p.cmd[1], *z = p.cmd[2];
+    Kv4AttnArgs a;
+    a.c = pool_at(c, z[0], z[1], z[2]);
+    a.n_head = w[1];
+    a.q = c->act + w[2];
+    a.y = c->act + w[3];
+    a.table = words_at(c, w[4]);
+    a.stride = w[5];
+    a.q_start = words_at(c, w[6]);
+    a.kv_len = words_at(c, w[7]);
+    a.n_req = x[0];
+    a.n_rows = x[1];
+    a.max_q = x[2];
+    a.max_kv = x[3];
+    std::memcpy(&a.scale, &x[4], 4);
+    a.window = x[5];
+    a.q_head_stride = x[7] ? x[7] : a.c.dim;
+    a.q_stride = x[6] ? x[6] : a.n_head * a.q_head_stride;
+    a.y_stride = z[3] ? z[3] : size_t(a.n_head) * a.c.dim;
+    a.status = c->dstatus + kServeStatusWord;
+    a.room = c->serve_room;
+    a.pdl = c->pdl;
+    return a;
+}
+BeamSelectArgs beam_select_args(b200q_ctx *c, const Pass &p) {
+    const uint32_t *w = p.cmd[0], *x = p.cmd[1];
+    BeamSelectArgs a;
+    a.n_req = w[1];
+    a.beams = w[2];
+    a.vocab = w[3];
+    a.logits = c->act + w[4];
+    a.stride = w[5] ? w[5] : w[3];
+    a.scores = c->act + w[6];
+    a.n_out = w[7];
+    a.out = c->act + x[0];
+    a.parent = words_at(c, x[1]);
+    a.token = words_at(c, x[2]);
+    a.room = c->serve_room;
+    a.pdl = c->pdl;
+    return a;
+}
+int exec_serve(b200q_ctx *c, const Pass &p) {
+    const uint32_t *w = p.cmd[0], *x = p.cmd[1];
+    uint32_t *status = c->dstatus + kServeStatusWord;
+    int rc = flush_wait(c);
+    if (rc) return rc;
+    unsigned kernels = 1;
+    if (p.op == 18) {
+        BlockMapArgs a;
+        a.n_req = w[1];
+        a.past = words_at(c, w[2]);
+        a.fresh = words_at(c, w[3]);
+        a.table = words_at(c, w[4]);
+        a.stride = w[5];
+        a.free_pages = words_at(c, w[6]);
+        a.n_free = w[7];
+        a.cursor_in = a.cursor_out = words_at(c, x[0]);
+        a.kv_len = words_at(c, x[1]);
+        a.q_start = words_at(c, x[2]);
+        a.slots = words_at(c, x[3]);
+        a.positions = words_at(c, x[4]);
+        a.n_rows = x[5];
+        a.page = x[6];
+        a.status = status;
+        a.pdl = c->pdl;
+        kernels = block_map_launches(a);
+        CUDA_TRY(c, launch_block_map(a, c->stream));
+    } else if (p.op == 19) {
+        Kv4RowsArgs a;
+        a.c = pool_at(c, w[7], x[0], x[1]);
+        const size_t width = size_t(a.c.n_kv) * a.c.dim;
+        a.n = w[1];
+        a.k = c->act + w[2];
+        a.v = c->act + w[3];
+        a.slots = words_at(c, w[4]);
+        a.k_stride = w[5] ? w[5] : width;
+        a.v_stride = w[6] ? w[6] : width;
+        a.status = status;
+        a.pdl = c->pdl;
+        if (a.n == 0) return 0;
+        CUDA_TRY(c, launch_kv4_store(a, c->stream));
+    } else if (p.op == 20) {
+        const Kv4AttnArgs a = kv4_attn_args(c, p);
+        if (a.n_rows == 0) return 0;
+        const size_t need = kv4_attn_room(a, unsigned(c->sms));
+        if (need == 0) return set_err(c, B200Q_ERR_ARG, "KV4_ATTN: n_rows, n_req and max_kv allow for more than 2^31 tiles of work");
+        if (!a.room || c->serve_room_bytes < need) return set_err(c, B200Q_ERR_STATE, "KV4_ATTN: workspace not prepared");
+        kernels = kv4_attn_launches(a, unsigned(c->sms));
+        CUDA_TRY(c, launch_kv4_attn(a, unsigned(c->sms), c->stream));
+    } else if (p.op == 21) {
+        const BeamSelectArgs a = beam_select_args(c, p);
+        if (!a.room || c->serve_room_bytes < beam_select_room(a)) return set_err(c, B200Q_ERR_STATE, "BEAM_SELECT: workspace not prepared");
+        kernels = 2;
+        CUDA_TRY(c, launch_beam_select(a, c->stream));
+    } else if (p.op == 22) {
+        BeamReorderArgs a;
+        a.n_req = w[1];
+        a.beams = w[2];
+        a.parent = words_at(c, w[3]);
+        a.src = reinterpret_cast<const uint8_t *>(c->state) + size_t(w[4]) * 512;
+        a.dst = reinterpret_cast<uint8_t *>(c->state) + size_t(w[5]) * 512;
+        a.row_bytes = size_t(w[6]) * 512;
+        a.layers = w[7];
+        a.src_layer = a.dst_layer = x[0] ? size_t(x[0]) * 512 : size_t(a.n_req) * a.beams * a.row_bytes;
+        a.status = status;
+        a.pdl = c->pdl;
+        CUDA_TRY(c, launch_beam_reorder(a, c->stream));
+    } else {
+        Kv4ReorderArgs a;
+        a.c = pool_at(c, w[7], x[0], x[1]);
+        a.n_req = w[1];
+        a.beams = w[2];
+        a.table = words_at(c, w[3]);
+        a.stride = w[4];
+        a.kv_len = words_at(c, w[5]);
+        a.parent = words_at(c, w[6]);
+        a.layers = x[2];
+        a.layer_bytes = size_t(x[3]) * 256;
+        a.status = status;
+        a.pdl = c->pdl;
+        CUDA_TRY(c, launch_kv4_reorder(a, c->stream));
+    }
+    c->launches += kernels;
+    return 0;
+}
+
 int exec_ext(b200q_ctx *c, const Pass &p) {
+    if (p.op >= 18 && p.op <= 23) return exec_serve(c, p);
     const uint32_t *cmd = p.cmd[0];
     float *A = c->act;
     int rc = 0;
@@ -936,20 +1081,14 @@ int exec_chain(b200q_ctx *c, ChainArgs &a) {
     return 0;
 }
 
-// The image of the quantized tokens that the list's GEMV_BATCH commands of more than kBatchMax rows need, allocated
-// before the list runs or is captured (no allocation inside a capture).
-int prepare_gemm_image(b200q_ctx *c, const Plan &plan) {
-    size_t need = 0;
-    for (const Pass &p : plan.passes) {
-        if (p.op != 17 || p.kind != PassKind::Ext) continue;
-        const unsigned batch = ((p.cmd[0][1] >> 16) & 0xffffu) + 1u;
-        if (batch > kBatchMax) need = std::max(need, gemm_image_bytes(p.cmd[0][3], batch));
-    }
-    if (need <= c->gemm_img_bytes) return 0;
+// A buffer of the context that holds at least `need` bytes, allocated before a list runs or is captured (no allocation
+// inside a capture). A buffer that is replaced stays allocated until the context ends (captured graphs may still use it).
+int grow_buffer(b200q_ctx *c, uint8_t *&buf, size_t &held, std::vector<uint8_t *> &old, size_t need, const char *what) {
+    if (need <= held) return 0;
     // at least double the old size, so that a caller whose prompts grow a little at a time retires O(log) buffers;
     // exactly the need when the doubled size does not fit
     uint8_t *img = nullptr;
-    size_t bytes = std::max(need, 2 * c->gemm_img_bytes);
+    size_t bytes = std::max(need, 2 * held);
     cudaError_t e = cudaMalloc(&img, bytes);
     if (e != cudaSuccess && bytes > need) {
         cudaGetLastError();
@@ -958,12 +1097,31 @@ int prepare_gemm_image(b200q_ctx *c, const Plan &plan) {
     }
     if (e != cudaSuccess) {
         cudaGetLastError();
-        return set_err(c, B200Q_ERR_NOMEM, "GEMV_BATCH token image (%zu bytes): %s", need, cudaGetErrorString(e));
+        return set_err(c, B200Q_ERR_NOMEM, "%s (%zu bytes): %s", what, need, cudaGetErrorString(e));
     }
-    if (c->gemm_img) c->gemm_img_old.push_back(c->gemm_img);
-    c->gemm_img = img;
-    c->gemm_img_bytes = bytes;
+    if (buf) old.push_back(buf);
+    buf = img;
+    held = bytes;
     return 0;
+}
+
+// What the list's commands need besides their operands: the image of the quantized tokens of GEMV_BATCH commands of more
+// than kBatchMax rows, and the workspace of KV4_ATTN and BEAM_SELECT.
+int prepare_buffers(b200q_ctx *c, const Plan &plan) {
+    size_t image = 0, room = 0;
+    for (const Pass &p : plan.passes) {
+        if (p.kind != PassKind::Ext) continue;
+        if (p.op == 17) {
+            const unsigned batch = ((p.cmd[0][1] >> 16) & 0xffffu) + 1u;
+            if (batch > kBatchMax) image = std::max(image, gemm_image_bytes(p.cmd[0][3], batch));
+        } else if (p.op == 20) {
+            room = std::max(room, kv4_attn_room(kv4_attn_args(c, p), unsigned(c->sms)));
+        } else if (p.op == 21) {
+            room = std::max(room, beam_select_room(beam_select_args(c, p)));
+        }
+    }
+    const int rc = grow_buffer(c, c->gemm_img, c->gemm_img_bytes, c->gemm_img_old, image, "GEMV_BATCH token image");
+    return rc ? rc : grow_buffer(c, c->serve_room, c->serve_room_bytes, c->serve_room_old, room, "KV4_ATTN / BEAM_SELECT workspace");
 }
 
 // Executes the passes of a plan on the context stream (no synchronization).
@@ -1089,14 +1247,17 @@ Limits limits_of(const b200q_ctx *c) {
 
 // A pass whose bounded wait ran out sets the device error word (dstatus[1]); read and clear it after a sync.
 int check_device_status(b200q_ctx *c) {
-    unsigned st[2] = {0, 0};
+    unsigned st[3] = {0, 0, 0};
+    static_assert(kServeStatusWord == 2, "the third status word");
     CUDA_TRY(c, cudaMemcpy(st, c->dstatus, sizeof(st), cudaMemcpyDeviceToHost));
-    if (st[0] | st[1]) {
-        const unsigned zero[2] = {0, 0};
+    if (st[0] | st[1] | st[2]) {
+        const unsigned zero[3] = {0, 0, 0};
         CUDA_TRY(c, cudaMemcpy(c->dstatus, zero, sizeof(zero), cudaMemcpyHostToDevice));
+        if (st[2] & B200Q_SERVE_WAIT) return set_err(c, B200Q_ERR_TIMEOUT, "a bounded wait ran out (cache tiles)");
         if (st[1]) return set_err(c, B200Q_ERR_TIMEOUT, "a bounded wait ran out (weight tiles, or a peer GPU's rows)");
         if (st[0] & 2u) return set_err(c, B200Q_ERR_ARG, "ATTN: the position in act is outside the KV slot");
-        return set_err(c, B200Q_ERR_ARG, "GET_ROW: the row index in act is outside the matrix");
+        if (st[0]) return set_err(c, B200Q_ERR_ARG, "GET_ROW: the row index in act is outside the matrix");
+        return set_err(c, B200Q_ERR_ARG, "commands for several sequences left something out (B200Q_SERVE bits 0x%x)", st[2]);
     }
     return 0;
 }
@@ -1221,6 +1382,8 @@ void b200q_destroy(b200q_ctx *c) {
     cudaFree(c->xq);
     cudaFree(c->gemm_img);
     for (uint8_t *p : c->gemm_img_old) cudaFree(p);
+    cudaFree(c->serve_room);
+    for (uint8_t *p : c->serve_room_old) cudaFree(p);
     if (c->stream) cudaStreamDestroy(c->stream);
     delete c;
 }
@@ -1407,7 +1570,7 @@ int b200q_run_async(b200q_ctx *c, const uint32_t *cmds, unsigned n_cmds) {
     if (!cmds) return B200Q_ERR_ARG;
     const Plan plan = plan_list(cmds, n_cmds, limits_of(c));
     if (plan.status == 129) return 129;
-    if ((rc = prepare_gemm_image(c, plan))) return rc;
+    if ((rc = prepare_buffers(c, plan))) return rc;
     if ((rc = exec_plan(c, plan, n_cmds))) return rc;
     if (plan.status) c->err = plan.error;
     return plan.status;
@@ -1516,7 +1679,7 @@ int b200q_graph_create(b200q_ctx *c, const uint32_t *cmds, unsigned n_cmds, b200
         c->err = plan.error;
         return plan.status;
     }
-    if ((rc = prepare_gemm_image(c, plan))) return rc;
+    if ((rc = prepare_buffers(c, plan))) return rc;
     b200q_graph *g = new b200q_graph();
     g->ctx = c;
     CUDA_TRY(c, cudaStreamBeginCapture(c->stream, cudaStreamCaptureModeThreadLocal));
@@ -1659,7 +1822,7 @@ int b200q_debug_block_sums(b200q_ctx *c, const uint32_t cmd[8], int32_t *out) {
         CUDA_TRY(c, cudaMalloc(&d, count * 4));
         cudaMemset(d, 0, count * 4);
         c->gemm_sums = d;
-        rc = prepare_gemm_image(c, plan);
+        rc = prepare_buffers(c, plan);
         if (!rc) rc = exec_plan(c, plan, 1);
         c->gemm_sums = nullptr;
         cudaError_t e = cudaStreamSynchronize(c->stream);

@@ -304,10 +304,10 @@ template <typename T>
 cudaError_t launch_reorder(const BeamReorderArgs &a, cudaStream_t st) {
     const size_t cols = a.row_bytes / sizeof(T), want = (cols + 255) / 256;
     const dim3 grid(unsigned(want < 4096 ? want : 4096), a.n_req, a.layers);
-    if (a.beams <= 4) return launch_pdl(beam_reorder_kernel<T, 4>, grid, dim3(256), 0, st, a);
-    if (a.beams <= 8) return launch_pdl(beam_reorder_kernel<T, 8>, grid, dim3(256), 0, st, a);
-    if (a.beams <= 16) return launch_pdl(beam_reorder_kernel<T, 16>, grid, dim3(256), 0, st, a);
-    return launch_pdl(beam_reorder_kernel<T, 32>, grid, dim3(256), 0, st, a);
+    if (a.beams <= 4) return launch_pdl(a.pdl, beam_reorder_kernel<T, 4>, grid, dim3(256), 0, st, a);
+    if (a.beams <= 8) return launch_pdl(a.pdl, beam_reorder_kernel<T, 8>, grid, dim3(256), 0, st, a);
+    if (a.beams <= 16) return launch_pdl(a.pdl, beam_reorder_kernel<T, 16>, grid, dim3(256), 0, st, a);
+    return launch_pdl(a.pdl, beam_reorder_kernel<T, 32>, grid, dim3(256), 0, st, a);
 }
 
 }  // namespace
@@ -322,13 +322,13 @@ cudaError_t launch_beam_select(const BeamSelectArgs &a, cudaStream_t st) {
     auto *list = reinterpret_cast<unsigned long long *>(a.room);
     auto *stat = reinterpret_cast<float2 *>(list + size_t(rows) * chunks * a.n_out);
     const bool wide = ((reinterpret_cast<uintptr_t>(a.logits) | a.stride * 4) & 15) == 0;
-    const cudaError_t e = launch_pdl(wide ? beam_chunk_kernel<true> : beam_chunk_kernel<false>, dim3(chunks, rows), dim3(kSelThreads), 0, st, a, list, stat);
+    const cudaError_t e = launch_pdl(a.pdl, wide ? beam_chunk_kernel<true> : beam_chunk_kernel<false>, dim3(chunks, rows), dim3(kSelThreads), 0, st, a, list, stat);
     if (e != cudaSuccess) return e;
     const size_t scored = size_t(a.beams) * a.n_out * sizeof(Scored), lists = size_t(a.beams) * chunks * a.n_out * 8;
     const unsigned in_smem = lists <= kListBytes;
     const cudaError_t f = ensure_smem_attr(reinterpret_cast<const void *>(beam_merge_kernel), int(kMaxBeams * kMaxBeamOut * sizeof(Scored) + kListBytes));
     if (f != cudaSuccess) return f;
-    return launch_pdl(beam_merge_kernel, dim3(a.n_req), dim3(kMergeThreads), scored + (in_smem ? lists : 0), st, a,
+    return launch_pdl(a.pdl, beam_merge_kernel, dim3(a.n_req), dim3(kMergeThreads), scored + (in_smem ? lists : 0), st, a,
                       static_cast<const unsigned long long *>(list), static_cast<const float2 *>(stat), chunks, in_smem);
 }
 

@@ -326,12 +326,14 @@ __global__ void __launch_bounds__(128) kv4_reorder_kernel(const Kv4ReorderArgs a
 
 }  // namespace
 
+unsigned block_map_launches(const BlockMapArgs &a) { return a.n_rows <= kMapRows ? 1 : 2; }
+
 cudaError_t launch_block_map(const BlockMapArgs &a, cudaStream_t st) {
     const bool one = a.n_rows <= kMapRows;
     const unsigned most = one && a.n_rows / 4 > a.n_req ? a.n_rows / 4 : a.n_req, threads = most <= 128 ? 128 : most <= 512 ? 512 : 1024;
-    const cudaError_t e = launch_pdl(block_map_kernel, dim3(1), dim3(threads), 0, st, a, one);
+    const cudaError_t e = launch_pdl(a.pdl, block_map_kernel, dim3(1), dim3(threads), 0, st, a, one);
     if (one || e != cudaSuccess) return e;
-    return launch_pdl(map_rows_kernel, dim3((a.n_rows + 1023) / 1024), dim3(256), 0, st, a);
+    return launch_pdl(a.pdl, map_rows_kernel, dim3((a.n_rows + 1023) / 1024), dim3(256), 0, st, a);
 }
 
 // x: the values of a row; y: the rows, as many at a time as fill the GPU a few times over
@@ -343,19 +345,19 @@ static bool wide_rows(const Kv4RowsArgs &a) {
     return ((reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) | a.k_stride * 4 | a.v_stride * 4) & 15) == 0;
 }
 cudaError_t launch_kv4_store(const Kv4RowsArgs &a, cudaStream_t st) {
-    return launch_pdl(wide_rows(a) ? kv4_store_kernel<true> : kv4_store_kernel<false>, rows_grid(a), dim3(256), 0, st, a);
+    return launch_pdl(a.pdl, wide_rows(a) ? kv4_store_kernel<true> : kv4_store_kernel<false>, rows_grid(a), dim3(256), 0, st, a);
 }
 cudaError_t launch_kv4_load(const Kv4RowsArgs &a, cudaStream_t st) {
-    return launch_pdl(wide_rows(a) ? kv4_load_kernel<true> : kv4_load_kernel<false>, rows_grid(a), dim3(256), 0, st, a);
+    return launch_pdl(a.pdl, wide_rows(a) ? kv4_load_kernel<true> : kv4_load_kernel<false>, rows_grid(a), dim3(256), 0, st, a);
 }
 
 cudaError_t launch_kv4_reorder(const Kv4ReorderArgs &a, cudaStream_t st) {
     const unsigned cols = a.c.n_kv * (a.c.page / kTileTokens) * kv4_tile_bytes(a.c.dim) / 16;
     const dim3 grid((cols + 127) / 128, a.n_req, a.layers + 1);
-    if (a.beams <= 4) return launch_pdl(kv4_reorder_kernel<4>, grid, dim3(128), 0, st, a);
-    if (a.beams <= 8) return launch_pdl(kv4_reorder_kernel<8>, grid, dim3(128), 0, st, a);
-    if (a.beams <= 16) return launch_pdl(kv4_reorder_kernel<16>, grid, dim3(128), 0, st, a);
-    return launch_pdl(kv4_reorder_kernel<32>, grid, dim3(128), 0, st, a);
+    if (a.beams <= 4) return launch_pdl(a.pdl, kv4_reorder_kernel<4>, grid, dim3(128), 0, st, a);
+    if (a.beams <= 8) return launch_pdl(a.pdl, kv4_reorder_kernel<8>, grid, dim3(128), 0, st, a);
+    if (a.beams <= 16) return launch_pdl(a.pdl, kv4_reorder_kernel<16>, grid, dim3(128), 0, st, a);
+    return launch_pdl(a.pdl, kv4_reorder_kernel<32>, grid, dim3(128), 0, st, a);
 }
 
 }  // namespace b200q

@@ -22,9 +22,6 @@
 
 namespace b200q {
 
-// More requests than this, and a launch's schedule would not fit its shared memory.
-constexpr unsigned kAttnMaxReq = 4096;
-
 namespace {
 
 constexpr unsigned kWarps = 4, kThreads = kWarps * 32;
@@ -885,9 +882,9 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_merge_kernel(const Kv4AttnA
 template <int NB, int NT>
 cudaError_t launch_tiles(const Kv4AttnArgs &a, const AttnPlan &plan, unsigned grid, cudaStream_t st) {
     using S = Shape<NB, NT>;
-    const cudaError_t e = ensure_smem_attr(reinterpret_cast<const void *>(kv4_attn_kernel<NB, NT>), S::kSmem + int(kAttnMaxReq + 1) * 4);
+    const cudaError_t e = ensure_smem_attr(reinterpret_cast<const void *>(kv4_attn_kernel<NB, NT>), S::kSmem + int(kMaxAttnReq + 1) * 4);
     if (e != cudaSuccess) return e;
-    return launch_pdl(kv4_attn_kernel<NB, NT>, dim3(grid), dim3(kThreads), S::kSmem + (size_t(a.n_req) + 1) * 4, st, a, plan);
+    return launch_pdl(a.pdl, kv4_attn_kernel<NB, NT>, dim3(grid), dim3(kThreads), S::kSmem + (size_t(a.n_req) + 1) * 4, st, a, plan);
 }
 
 AttnPlan plan_of(const Kv4AttnArgs &a, unsigned sms) {
@@ -937,7 +934,7 @@ cudaError_t launch_kv4_attn(const Kv4AttnArgs &a, unsigned sms, cudaStream_t st)
     if (e != cudaSuccess) return e;
     if (p.max_ranges > 1) {  // (else nothing lies in two ranges)
         const unsigned edges = p.max_ranges - 1;
-        e = launch_pdl(kv4_attn_merge_kernel, dim3(edges < sms * 8 ? edges : sms * 8), dim3(kThreads), 0, st, a, p);
+        e = launch_pdl(a.pdl, kv4_attn_merge_kernel, dim3(edges < sms * 8 ? edges : sms * 8), dim3(kThreads), 0, st, a, p);
     }
     if (e != cudaSuccess || p.most_rows == ~0u) return e;
     return launch_kv4_prompt(a, p.most_rows + 1, st);

@@ -485,7 +485,7 @@ cudaError_t launch_prompt(const Kv4AttnArgs &a, unsigned least_rows, cudaStream_
     const cudaError_t e = ensure_smem_attr(reinterpret_cast<const void *>(kv4_prompt_kernel<NB>), S::kSmem);
     if (e != cudaSuccess) return e;
     const unsigned long long rows = (unsigned long long)(a.max_q < a.n_rows ? a.max_q : a.n_rows) * (a.n_head / a.c.n_kv);
-    return launch_pdl(kv4_prompt_kernel<NB>, dim3(a.c.n_kv * a.n_req, unsigned((rows + kRows - 1) / kRows)), dim3(kThreads), S::kSmem, st, a, least_rows);
+    return launch_pdl(a.pdl, kv4_prompt_kernel<NB>, dim3(a.c.n_kv * a.n_req, unsigned((rows + kRows - 1) / kRows)), dim3(kThreads), S::kSmem, st, a, least_rows);
 }
 
 }  // namespace

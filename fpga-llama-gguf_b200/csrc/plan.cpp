@@ -1,6 +1,7 @@
 // Command-list planner (see plan.h). Mirrors the control flow of the reference command processor
 // (fpga/src/gemvqc16.cpp:553-958) and adds range checks against the device buffers.
 #include "plan.h"
+#include "serve_limits.h"
 
 #include <cstring>
 
@@ -105,6 +106,105 @@ bool member_ranges_ok(const Ctx &c, Member &m, unsigned x_off, bool allow_missin
 
 bool ranges_meet(size_t a, size_t an, size_t b, size_t bn) { return a < b + bn && b < a + an; }
 
+// ---- the operators for several sequences (opcodes 18 .. 23; the words: include/b200q.h) -----------------------------
+unsigned serve_slots(uint32_t op) { return op == 20 ? 3u : 2u; }
+
+struct ServeSpan {
+    size_t off, n;  // act floats (uint32 words)
+    bool written;
+};
+size_t rows_span(size_t rows, size_t stride, size_t width) { return rows ? (rows - 1) * stride + width : 0; }
+
+// The act ranges of a command whose shape is valid.
+std::vector<ServeSpan> serve_spans(const uint32_t (*w)[8]) {
+    const uint32_t *a = w[0], *b = w[1], *c = w[2];
+    switch (a[0]) {
+    case 18: {
+        const size_t n = a[1];
+        return {{a[2], n, false}, {a[3], n, false}, {a[4], n * a[5], true}, {a[6], a[7], false}, {b[0], 1, true}, {b[1], n, true},
+                {b[2], n + 1, true}, {b[3], b[5], true}, {b[4], b[5], true}};
+    }
+    case 19: {
+        const size_t width = size_t(a[7] & 0xffu) * ((a[7] >> 8 & 0xffu) * 32u);
+        return {{a[2], rows_span(a[1], a[5] ? a[5] : width, width), false}, {a[3], rows_span(a[1], a[6] ? a[6] : width, width), false}, {a[4], a[1], false}};
+    }
+    case 20: {
+        const size_t dim = (c[0] >> 8 & 0xffu) * 32u, head = b[7] ? b[7] : dim, q = b[6] ? b[6] : a[1] * head, y = c[3] ? c[3] : a[1] * dim;
+        return {{a[2], rows_span(b[1], q, (a[1] - 1) * head + dim), false}, {a[3], rows_span(b[1], y, a[1] * dim), true}, {a[4], size_t(b[0]) * a[5], false},
+                {a[6], size_t(b[0]) + 1, false}, {a[7], b[0], false}};
+    }
+    case 21: {
+        const size_t rows = size_t(a[1]) * a[2], outs = size_t(a[1]) * a[7];
+        return {{a[4], rows_span(rows, a[5] ? a[5] : a[3], a[3]), false}, {a[6], rows, false}, {b[0], outs, true}, {b[1], outs, true}, {b[2], outs, true}};
+    }
+    case 22: return {{a[3], size_t(a[1]) * a[2], false}};
+    default: {
+        const size_t rows = size_t(a[1]) * a[2];
+        return {{a[3], rows * a[4], true}, {a[5], rows, false}, {a[6], rows, false}};
+    }
+    }
+}
+
+// geometry word: n_kv | (head_dim / 32) << 8 | (page_tokens / 16) << 16; the pool within the KV buffer, in 256-byte units
+bool serve_pool_ok(const Limits &lim, uint32_t geo, uint32_t pool, uint32_t n_pages, uint32_t layers, uint32_t layer_units) {
+    const unsigned n_kv = geo & 0xffu, dim = (geo >> 8 & 0xffu) * 32u, page = (geo >> 16) * 16u;
+    if (!kv4_shape_ok(n_pages, page, n_kv, dim) || layers == 0 || layers > 65534) return false;
+    const size_t layer = kv4_layer_bytes(n_pages, page, n_kv, dim), step = size_t(layer_units) * 256, at = size_t(pool) * 256;
+    if (layers > 1 && step < layer) return false;
+    const size_t all = (layers - 1) * step + layer;
+    return at <= lim.kv_bytes && all <= lim.kv_bytes - at;
+}
+
+const char *serve_check(const Ctx &C, const uint32_t (*w)[8]) {
+    const uint32_t *a = w[0], *b = w[1], *c = w[2];
+    switch (a[0]) {
+    case 18:
+        if (a[1] == 0 || a[1] > kMaxMapReq || a[5] == 0 || !page_ok(b[6]) || (unsigned long long)a[5] * b[6] >= 0xFFFFFFFFull || b[5] >= 0x80000000u || b[7])
+            return "invalid BLOCK_MAP";
+        break;
+    case 19: {
+        const size_t width = size_t(a[7] & 0xffu) * ((a[7] >> 8 & 0xffu) * 32u);
+        if (!serve_pool_ok(C.lim, a[7], b[0], b[1], 1, 0) || (a[5] && a[5] < width) || (a[6] && a[6] < width) || (b[2] | b[3] | b[4] | b[5] | b[6] | b[7]))
+            return "invalid KV4_STORE";
+        break;
+    }
+    case 20: {
+        const unsigned n_kv = c[0] & 0xffu, dim = (c[0] >> 8 & 0xffu) * 32u, page = (c[0] >> 16) * 16u;
+        const size_t head = b[7] ? b[7] : dim;
+        if (!serve_pool_ok(C.lim, c[0], c[1], c[2], 1, 0) || !attn_shape_ok(a[1], n_kv, b[0], b[1], b[2], b[3]) || a[5] == 0 ||
+            (unsigned long long)a[5] * page < b[3] || head < dim || (b[6] && b[6] < (a[1] - 1) * head + dim) || (c[3] && c[3] < size_t(a[1]) * dim) ||
+            (b[4] & 0x7f800000u) == 0x7f800000u || (c[4] | c[5] | c[6] | c[7]))
+            return "invalid KV4_ATTN";
+        break;
+    }
+    case 21:
+        if (!select_shape_ok(a[1], a[2], a[3], a[7]) || (a[5] && a[5] < a[3]) || (b[3] | b[4] | b[5] | b[6] | b[7])) return "invalid BEAM_SELECT";
+        break;
+    case 22: {
+        const size_t n = size_t(a[1]) * a[2] * a[6], step = b[0] ? b[0] : n;
+        if (a[1] == 0 || a[1] > kMaxMapReq || a[2] == 0 || a[2] > kMaxBeams || a[6] == 0 || a[7] == 0 || a[7] > 65535 || step < n ||
+            (b[1] | b[2] | b[3] | b[4] | b[5] | b[6] | b[7]))
+            return "invalid BEAM_REORDER";
+        const size_t all = (a[7] - 1) * step + n;
+        if (all > C.lim.state_rows || a[4] > C.lim.state_rows - all || a[5] > C.lim.state_rows - all || (a[4] != a[5] && ranges_meet(a[4], all, a[5], all)))
+            return "BEAM_REORDER outside the state rows, or its source and destination overlap";
+        break;
+    }
+    default:
+        if (a[1] == 0 || a[1] > kMaxMapReq || a[2] == 0 || a[2] > kMaxBeams || a[4] == 0 || !serve_pool_ok(C.lim, a[7], b[0], b[1], b[2], b[3]) ||
+            (b[4] | b[5] | b[6] | b[7]))
+            return "invalid KV4_REORDER";
+    }
+    const std::vector<ServeSpan> spans = serve_spans(w);
+    for (size_t i = 0; i < spans.size(); ++i) {
+        if (spans[i].off % 16 || !C.act(spans[i].off, spans[i].n)) return "operand outside act, or not on 16 floats";
+        for (size_t j = 0; j < spans.size(); ++j)
+            if (i != j && spans[i].written && spans[i].n && spans[j].n && ranges_meet(spans[i].off, spans[i].n, spans[j].off, spans[j].n))
+                return "an output overlaps another operand";
+    }
+    return nullptr;
+}
+
 // Act ranges a pass writes (for the deferred-norm check).
 void pass_writes(const Pass &p, std::vector<std::pair<size_t, size_t>> &w) {
     w.clear();
@@ -135,6 +235,10 @@ void pass_writes(const Pass &p, std::vector<std::pair<size_t, size_t>> &w) {
         else if (p.op == 14) w.push_back({c[6], c[2]});
         else if (p.op == 15) w.push_back({c[3], c[1]});
         else if (p.op == 16) w.push_back({c[3], size_t(c[1]) * kMaxRanks});
+        else if (p.op >= 18 && p.op <= 23) {
+            for (const ServeSpan &s : serve_spans(p.cmd))
+                if (s.written) w.push_back({s.off, s.n});
+        }
         else if (p.op == 17) w.push_back({c[7], size_t((c[1] >> 16 & 0xffffu) + 1u) * round16(c[2])});
         break;
     default: break;
@@ -587,6 +691,20 @@ Plan plan_list(const uint32_t *cmds, unsigned n_cmds, const Limits &lim) {
                 reject(c, "invalid GEMV_BATCH");
                 break;
             }
+            p.kind = PassKind::Ext;
+        } else if (op >= 18 && op <= 23) {
+            // ---- several sequences: BLOCK_MAP, KV4_STORE, KV4_ATTN, BEAM_SELECT, BEAM_REORDER, KV4_REORDER
+            const unsigned slots = serve_slots(op);
+            if (c + slots > n_cmds) {
+                reject(c, "the command's further slots are missing");
+                break;
+            }
+            for (unsigned i = 1; i < slots; ++i) std::memcpy(p.cmd[i], C.at(c + i), 32);
+            if (const char *why = serve_check(C, p.cmd)) {
+                reject(c, why);
+                break;
+            }
+            advance = slots;
             p.kind = PassKind::Ext;
         } else {
             reject(c, "unknown opcode");

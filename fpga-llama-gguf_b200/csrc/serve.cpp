@@ -195,7 +195,6 @@ Kv4View view_of(const b200q_kv4_pool *p) {
 
 size_t rows_extent(size_t rows, size_t stride, size_t width) { return rows ? ((rows - 1) * stride + width) * 4 : 0; }
 
-constexpr unsigned kMaxReq = 65535, kMaxAttnReq = 4096;
 constexpr size_t kMaxStride = size_t(1) << 32;
 
 int rows_call(const char *name, bool store, int device, const b200q_kv4_pool *pool, float *k, float *v, const uint32_t *slots, unsigned n,
@@ -275,9 +274,9 @@ B200Q_API int b200q_block_map(int device, unsigned n_req, const uint32_t *past, 
                               uint32_t *cursor_out, uint32_t *kv_len, uint32_t *q_start, uint32_t *slots, uint32_t *positions,
                               unsigned n_rows, uint32_t *status, void *stream, char *err, unsigned err_len) {
     Call c("block_map", device, stream, err, err_len);
-    c.need(n_req >= 1 && n_req <= kMaxReq, "n_req is not 1 to 65535");
+    c.need(n_req >= 1 && n_req <= kMaxMapReq, "n_req is not 1 to 65535");
     c.need(table_stride >= 1, "table_stride is 0");
-    c.need(page_tokens >= kTileTokens && page_tokens <= 4096 && page_tokens % kTileTokens == 0, "page_tokens is not a multiple of 16 up to 4096");
+    c.need(page_tokens >= kTileTokens && page_tokens <= kMaxPage && page_tokens % kTileTokens == 0, "page_tokens is not a multiple of 16 up to 4096");
     c.need((unsigned long long)table_stride * page_tokens < 0xFFFFFFFFull, "table_stride x page_tokens is over 2^32 - 2 tokens");
     c.need(n_rows < 0x80000000u, "n_rows is over 2^31 - 1");
     c.enter();
@@ -387,7 +386,7 @@ B200Q_API int b200q_kv4_attn(int device, const b200q_kv4_pool *pool, const float
 }
 
 static void check_select(Call &c, unsigned n_req, unsigned beams, unsigned vocab, unsigned n_out) {
-    c.need(n_req >= 1 && n_req <= kMaxReq / kMaxBeams, "n_req is not 1 to 2047");
+    c.need(n_req >= 1 && n_req <= kMaxSelectReq, "n_req is not 1 to 2047");
     c.need(beams >= 1 && beams <= kMaxBeams, "beams is not 1 to 32");
     c.need(vocab >= 1 && vocab <= kMaxVocab, "vocab is not 1 to 2^20");
     c.need(n_out >= 1 && n_out <= kMaxBeamOut, "n_out is not 1 to 64");
@@ -442,7 +441,7 @@ B200Q_API int b200q_beam_reorder(int device, const void *src, void *dst, const u
                                  size_t row_bytes, unsigned n_layers, size_t src_layer_bytes, size_t dst_layer_bytes, uint32_t *status,
                                  void *stream, char *err, unsigned err_len) {
     Call c("beam_reorder", device, stream, err, err_len);
-    c.need(n_req >= 1 && n_req <= kMaxReq, "n_req is not 1 to 65535");
+    c.need(n_req >= 1 && n_req <= kMaxMapReq, "n_req is not 1 to 65535");
     c.need(beams >= 1 && beams <= kMaxBeams, "beams is not 1 to 32");
     c.need(row_bytes >= 1 && row_bytes <= (size_t(1) << 40), "row_bytes is not 1 to 2^40");
     c.need(n_layers >= 1 && n_layers <= 65535, "n_layers is not 1 to 65535");
@@ -483,7 +482,7 @@ B200Q_API int b200q_kv4_reorder(int device, const b200q_kv4_pool *pool, uint32_t
     Call c("kv4_reorder", device, stream, err, err_len);
     const size_t bytes = check_pool(c, pool, true);
     c.need(table_stride >= 1, "table_stride is 0");
-    c.need(n_req >= 1 && n_req <= kMaxReq, "n_req is not 1 to 65535");
+    c.need(n_req >= 1 && n_req <= kMaxMapReq, "n_req is not 1 to 65535");
     c.need(beams >= 1 && beams <= kMaxBeams, "beams is not 1 to 32");
     c.enter();
     if (!c.ok()) return c.rc();

@@ -7,19 +7,13 @@
 #include <cstddef>
 #include <cstdint>
 
+#include "serve_limits.h"
+
 namespace b200q {
 
 // status bits (include/b200q.h, B200Q_SERVE_*)
 constexpr unsigned kServeRequest = 1, kServePage = 2, kServeSlot = 4, kServeShort = 8, kServeParent = 16, kServeWait = 32;
 constexpr unsigned kNoSlot = 0xFFFFFFFFu;  // a slot, page, parent or token that names nothing
-constexpr unsigned kTileTokens = 16;       // tokens of one cache tile
-constexpr unsigned kMaxKv4Dim = 256, kMaxBeams = 32, kMaxBeamOut = 64, kMaxVocab = 1u << 20;
-
-// A tile holds 16 tokens of one KV head: K codes, V codes (8 dim bytes each), K scales, V scales (dim bytes each).
-#if defined(__CUDACC__)
-__host__ __device__
-#endif
-inline unsigned kv4_tile_bytes(unsigned dim) { return 18 * dim; }
 
 // The cache of one layer: page p, head h, tile t at base + ((p * n_kv + h) * (page / 16) + t) * 18 dim.
 struct Kv4View {
@@ -32,6 +26,7 @@ struct BlockMapArgs {
     const uint32_t *past = nullptr, *fresh = nullptr, *free_pages = nullptr, *cursor_in = nullptr;
     uint32_t *table = nullptr, *cursor_out = nullptr, *kv_len = nullptr, *q_start = nullptr, *slots = nullptr, *positions = nullptr;
     uint32_t *status = nullptr;
+    bool pdl = true;  // programmatic dependent launch
 };
 
 struct Kv4RowsArgs {  // kv4_store (k, v read) / kv4_load (k, v written)
@@ -41,6 +36,7 @@ struct Kv4RowsArgs {  // kv4_store (k, v read) / kv4_load (k, v written)
     const uint32_t *slots = nullptr;
     unsigned n = 0;
     uint32_t *status = nullptr;
+    bool pdl = true;  // programmatic dependent launch
 };
 
 struct Kv4AttnArgs {
@@ -53,6 +49,7 @@ struct Kv4AttnArgs {
     float scale = 0.0f;
     uint8_t *room = nullptr;  // workspace of kv4_attn_room bytes
     uint32_t *status = nullptr;
+    bool pdl = true;  // programmatic dependent launch
 };
 
 struct BeamSelectArgs {
@@ -62,6 +59,7 @@ struct BeamSelectArgs {
     float *out = nullptr;
     uint32_t *parent = nullptr, *token = nullptr;
     uint8_t *room = nullptr;
+    bool pdl = true;  // programmatic dependent launch
 };
 
 struct BeamReorderArgs {
@@ -71,6 +69,7 @@ struct BeamReorderArgs {
     unsigned n_req = 0, beams = 0, layers = 0;
     size_t row_bytes = 0, src_layer = 0, dst_layer = 0;
     uint32_t *status = nullptr;
+    bool pdl = true;  // programmatic dependent launch
 };
 
 struct Kv4ReorderArgs {
@@ -80,9 +79,11 @@ struct Kv4ReorderArgs {
     uint32_t *table = nullptr;
     const uint32_t *kv_len = nullptr, *parent = nullptr;
     uint32_t *status = nullptr;
+    bool pdl = true;  // programmatic dependent launch
 };
 
 cudaError_t launch_block_map(const BlockMapArgs &a, cudaStream_t st);
+unsigned block_map_launches(const BlockMapArgs &a);
 cudaError_t launch_kv4_store(const Kv4RowsArgs &a, cudaStream_t st);
 cudaError_t launch_kv4_load(const Kv4RowsArgs &a, cudaStream_t st);
 size_t kv4_attn_room(const Kv4AttnArgs &a, unsigned sms);  // 0: more work than one launch takes
@@ -93,13 +94,13 @@ size_t beam_select_room(const BeamSelectArgs &a);
 cudaError_t launch_beam_select(const BeamSelectArgs &a, cudaStream_t st);
 cudaError_t launch_beam_reorder(const BeamReorderArgs &a, cudaStream_t st);
 cudaError_t launch_kv4_reorder(const Kv4ReorderArgs &a, cudaStream_t st);
-// kernels the launchers above start (for launch counts)
+// kernels that launch_kv4_attn starts (for launch counts; block_map_launches above likewise)
 unsigned kv4_attn_launches(const Kv4AttnArgs &a, unsigned sms);
 
 // A launch that may start while the previous kernel drains: every kernel here waits (griddepcontrol.wait) before it
 // touches global memory.
 template <typename... P, typename... A>
-inline cudaError_t launch_pdl(void (*k)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, A... args) {
+inline cudaError_t launch_pdl(bool pdl, void (*k)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, A... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = block;
@@ -109,7 +110,7 @@ inline cudaError_t launch_pdl(void (*k)(P...), dim3 grid, dim3 block, size_t sme
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = pdl ? 1 : 0;
     return cudaLaunchKernelEx(&cfg, k, args...);
 }
 

@@ -19,6 +19,7 @@ Layer i is an attention layer when i % attn_every == attn_every - 1, else a Gate
                    -> GDN step (L2 q/k, gates, gated norm * silu(z)) with ssm_out GEMV + residual ADD fused
   attention layer  RMSNORM(defer) -> {q|gate, k, v} one group -> per-head RMSNORM of q and k -> NEOX RoPE
                    -> ATTN over the F16 KV slot -> sigmoid(gate) * attention -> o GEMV + residual ADD
+                   (kv4_page: the 4-bit cache instead, a BLOCK_MAP per token and KV4_STORE, KV4_ATTN in the place of ATTN)
   both             RMSNORM(defer) -> gate + up GEMV pair with SwiGLU -> down GEMV + residual ADD
   head             RMSNORM(defer) -> Q6_K GEMV pieces (one group) -> ARGMAX
 """
@@ -29,8 +30,8 @@ from dataclasses import dataclass, replace
 import numpy as np
 
 from . import (CMD_WORDS, GDN_GATED, GDN_GATES, GDN_L2_QK, GDN_WITH_OUT, GEMV_ADD, GEMV_CONV, GEMV_SWIGLU, MAX_CMDS, NORM_DEFER,
-               Q4_0, Q6_K, UPLOAD_PASS_ROWS, UPLOAD_REPLICATE, add, allgather, allreduce, argmax, attn, cmd_list, conv, gdn,
-               gemv, get_row, gguf_row_bytes, rmsnorm, rope, silu_mul)
+               Q4_0, Q6_K, UPLOAD_PASS_ROWS, UPLOAD_REPLICATE, add, allgather, allreduce, argmax, attn, block_map_cmd, cmd_list, conv, gdn,
+               gemv, get_row, gguf_row_bytes, kv4_attn_cmd, kv4_geometry, kv4_page_bytes, kv4_store_cmd, rmsnorm, rope, silu_mul)
 from . import synth
 
 GDN_DIM = 128  # DeltaNet head size of the command ISA (state rows of 128 floats)
@@ -106,7 +107,7 @@ SHAPE_9B = Shape(hidden=4096, ffn=12288)
 class ActLayout:
     """Float offsets into act (16-float aligned): shared scratch first, then each layer's resident parameters."""
 
-    def __init__(self, s: Shape):
+    def __init__(self, s: Shape, kv4_page: int = 0):
         self.top = 0
         H, d = s.hidden, s.gdn_rows
         att, kvd = s.n_head * s.head_dim, s.n_kv_head * s.head_dim
@@ -131,6 +132,10 @@ class ActLayout:
                 p.update(conv_w=self._take(4 * 3 * d), conv_hist=self._take(3 * 3 * d), dt=self._take(s.gdn_heads),
                          a=self._take(s.gdn_heads), gdn_norm=self._take(GDN_DIM))
             self.layer.append(p)
+        if kv4_page:  # the 4-bit cache's step: one request of one new token
+            self.stride = -(-s.kv_ctx // kv4_page)
+            self.FRESH, self.TABLE, self.FREE, self.CURSOR = (self._take(n) for n in (1, self.stride, self.stride, 1))
+            self.KVLEN, self.QSTART, self.SLOT, self.PLACE = (self._take(n) for n in (1, 2, 1, 1))
         self.size = self.top
 
     def _take(self, n: int) -> int:
@@ -174,13 +179,17 @@ class HybridDecoder:
     each rank produces a partial hidden vector, rank 0 adds the residual, and one ALLREDUCE per projection sums them
     into the residual stream (two per layer). The head's logits meet in one ALLGATHER before ARGMAX."""
 
-    def __init__(self, shape: Shape = SHAPE_4B, seed: int = 4, first_token: int = 1, world: int = 1, rank: int = 0):
+    def __init__(self, shape: Shape = SHAPE_4B, seed: int = 4, first_token: int = 1, world: int = 1, rank: int = 0,
+                 kv4_page: int = 0):
+        """kv4_page: tokens of a page when the attention layers keep their K and V in the paged 4-bit cache (0: the F16
+        slots). All layers share one block table; a token's page is taken from the free pages as it is needed."""
         self.s = shape
+        self.kv4_page = kv4_page
         self.seed = seed
         self.first_token = first_token
         self.world, self.rank = world, rank
         self.ls = local_shape(shape, world)
-        self.L = ActLayout(self.ls)
+        self.L = ActLayout(self.ls, kv4_page)
         self.handles: dict = {}
 
     # ---- this rank's slices --------------------------------------------------------------------------------------
@@ -323,6 +332,11 @@ class HybridDecoder:
                 act[p["dt"]:p["dt"] + dt.size] = dt
                 act[p["a"]:p["a"] + a.size] = a
                 act[p["gdn_norm"]:p["gdn_norm"] + GDN_DIM] = r.normal(1, 0.1, GDN_DIM)
+        if self.kv4_page:  # the prompt's pages in order, the others free
+            words = act.view(np.uint32)
+            words[L.FRESH] = 1
+            words[L.TABLE:L.TABLE + L.stride] = np.arange(L.stride)
+            words[L.FREE:L.FREE + L.stride] = np.arange(L.stride) + -(-s.prefill // self.kv4_page)
         return act
 
     def initial_state(self) -> np.ndarray:
@@ -346,7 +360,20 @@ class HybridDecoder:
         if self.world > 1:
             k0 = self._kv_head0()
             kv = np.ascontiguousarray(kv[:, :, k0:k0 + self.ls.n_kv_head])
+        if self.kv4_page:
+            from .kv4 import pack_pages
+            out = np.zeros(self.kv_bytes(), np.uint8)
+            for j in range(s.n_attn):
+                at, n_pages = self.kv4_pool(j)
+                k, v = (kv[j, i, :, :s.prefill].astype(np.float32).transpose(1, 0, 2) for i in (0, 1))
+                pages = pack_pages(k, v, self.kv4_page, n_pages).reshape(-1)
+                out[at:at + pages.size] = pages
+            return out
         return kv.view(np.uint16).reshape(-1)
+
+    def kv_bytes(self) -> int:
+        """Bytes of the KV buffer: the layers' F16 slots, or their 4-bit pools."""
+        return self.kv4_pool(self.s.n_attn)[0] if self.kv4_page else self.s.n_attn * self.ls.kv_slot_bytes
 
     def record(self, pos: int) -> np.ndarray:
         """Host record of the token at position pos: the position (uint32 bits) and the NEOX RoPE cos/sin row
@@ -405,9 +432,23 @@ class HybridDecoder:
             rmsnorm(hd, L.K, p["k_norm"], L.KN, s.eps, rows=ls.n_kv_head),
             rope(s.rope_dims, L.QN, L.CS, L.QR, hd, ls.n_head),
             rope(s.rope_dims, L.KN, L.CS, L.KR, hd, ls.n_kv_head),
-            attn(ls.n_head, ls.n_kv_head, hd, L.QR, L.KR, L.V, L.YA, L.POS, slot),
+            *self._attend(slot),
             silu_mul(att, L.QG + hd, L.YA, L.YG, sigmoid=True, row=hd, stride=2 * hd),
         ] + self._project_out(Q4_0, att, h[f"{i}.wo"], L.YG) + self._ffn(i)
+
+    def kv4_pool(self, slot: int):
+        """(byte of the KV buffer, pages) of an attention layer's 4-bit pool."""
+        layer = self.L.stride * kv4_page_bytes(self.kv4_page, self.ls.n_kv_head, self.s.head_dim)
+        return slot * (-(-layer // 256) * 256), self.L.stride
+
+    def _attend(self, slot: int):
+        s, ls, L = self.s, self.ls, self.L
+        nh, nkv, hd = ls.n_head, ls.n_kv_head, s.head_dim
+        if not self.kv4_page:
+            return [attn(nh, nkv, hd, L.QR, L.KR, L.V, L.YA, L.POS, slot)]
+        geo, (pool, n_pages) = kv4_geometry(nkv, hd, self.kv4_page), self.kv4_pool(slot)
+        return [kv4_store_cmd(1, L.KR, L.V, L.SLOT, geo, pool, n_pages),
+                kv4_attn_cmd(nh, L.QR, L.YA, L.TABLE, L.stride, L.QSTART, L.KVLEN, 1, 1, 1, s.kv_ctx, hd ** -0.5, geo, pool, n_pages)]
 
     def _ffn(self, i: int):
         s, ls, L, h = self.s, self.ls, self.L, self.handles
@@ -435,6 +476,9 @@ class HybridDecoder:
         """The token's command blocks: the embedding row, one per layer, the head."""
         s, L = self.s, self.L
         blocks = [[get_row(Q4_0, s.hidden, self.handles["tok_embd"], L.TOK, L.X)]]
+        if self.kv4_page:  # the position is the tokens held so far
+            blocks[0].append(block_map_cmd(1, L.POS, L.FRESH, L.TABLE, L.stride, L.FREE, L.stride, L.CURSOR, L.KVLEN, L.QSTART, L.SLOT, L.PLACE, 1,
+                                           self.kv4_page))
         j = slot = 0
         for i in range(s.n_layers):
             if s.is_attn(i):
@@ -482,6 +526,8 @@ class HybridDecoder:
         ALLREDUCE after each projection back to the hidden size and ALLGATHER of the logits. Returns (graph, names):
         names maps "rec", "tok", "logits", "onorm" and (layer, parameter) to the node ids of the INPUT / PARAM
         tensors."""
+        if self.kv4_page:
+            raise ValueError("the op graph has no node for the 4-bit cache: use token_lists")
         from .graph import Graph
         from . import UNARY_SIGMOID, UNARY_SILU, UNARY_SOFTPLUS
         s, ls, h = self.s, self.ls, self.handles
@@ -581,7 +627,7 @@ class HybridDecoder:
             fl_rank = (fl & 0xFF) | UPLOAD_PASS_ROWS((fl >> 8) * (r1 - r0) // rows)  # the hint as the upload scales it
             wb += (weight_device_bytes(r1 - r0, cols, fmt, fl_rank) + 255) // 256 * 256
         return dict(weight_bytes=wb + (64 << 20), act_floats=self.L.size, state_rows=s.n_gdn * ls.gdn_rows,
-                    kv_bytes=s.n_attn * ls.kv_slot_bytes, kv_ctx=s.kv_ctx)
+                    kv_bytes=self.kv_bytes(), kv_ctx=s.kv_ctx)
 
     def load(self, ctx, keep: dict | None = None) -> None:
         """Uploads the weights and writes act, the DeltaNet states and the KV cache."""

@@ -92,6 +92,29 @@ extern "C" {
  * A GEMV_BATCH does not consume a deferred RMSNORM: it reads x as act holds it. The batch path of the reference's
  * roadmap (docs/ROADMAP.md:80-96, P2), and the prompt's matrix products. */
 #define B200Q_OP_GEMV_BATCH 17u
+/* Several sequences (see "several sequences" below for what they compute): commands of two slots (KV4_ATTN: three), whose
+ * counts, lengths, tables, slots, parents and tokens are uint32 words in act. Offsets are multiples of 16; the operands of a
+ * command that it writes lie apart from its others; strides of 0 mean packed rows; unused words are 0. G is the cache's
+ * geometry, n_kv_head | (head_dim / 32) << 8 | (page_tokens / 16) << 16, and pool its place in the KV buffer, in units of
+ * 256 bytes. What the device finds outside its bounds is left out and makes b200q_run / b200q_synchronize return
+ * B200Q_ERR_ARG with the B200Q_SERVE_* bits in b200q_last_error.
+ *   BLOCK_MAP    [18, n_req, past, fresh, table, table_stride, free_pages, n_free]
+ *                [cursor (read and advanced), kv_len, q_start, slots, positions, n_rows, page_tokens, 0]
+ *   KV4_STORE    [19, n, k, v, slots, k_stride, v_stride, G] [pool, n_pages, 0 ...]
+ *   KV4_ATTN     [20, n_head, q, y, table, table_stride, q_start, kv_len]
+ *                [n_req, n_rows, max_q, max_kv, scale (FP32 bits), window, q_stride, q_head_stride]
+ *                [G, pool, n_pages, y_stride, 0 ...]
+ *   BEAM_SELECT  [21, n_req, beams, vocab, logits, logits_stride, scores, n_out] [out_scores, out_parent, out_token, 0 ...]
+ *   BEAM_REORDER [22, n_req, beams, parent, src_row, dst_row, rows, n_layers] [layer_rows, 0 ...]: state rows; a beam holds
+ *                `rows` rows of each layer, layers lie layer_rows apart (0: packed); src_row = dst_row, or apart
+ *   KV4_REORDER  [23, n_req, beams, table, table_stride, kv_len, parent, G] [pool, n_pages, n_layers, layer (256-byte
+ *                units), 0 ...] */
+#define B200Q_OP_BLOCK_MAP 18u
+#define B200Q_OP_KV4_STORE 19u
+#define B200Q_OP_KV4_ATTN 20u
+#define B200Q_OP_BEAM_SELECT 21u
+#define B200Q_OP_BEAM_REORDER 22u
+#define B200Q_OP_KV4_REORDER 23u
 
 #define B200Q_GEMV_SWIGLU 0x100u
 #define B200Q_GEMV_CONV 0x200u
@@ -126,10 +149,11 @@ extern "C" {
  * reference's marker and bit meanings, all bits set (Q5_K, Q6_K, Q4_1, every fusion, ROPE, TRACE). act[2] holds
  * this library's own word: marker 0x6B53 in the high half, bit 0 ATTN, bit 1 ARGMAX, bit 2 GET_ROW, bit 3
  * row-sharded multi-GPU lists, bit 4 ALLREDUCE / ALLGATHER, bit 5 GEMV_BATCH, bit 6 GEMV_BATCH of more than 8
- * rows (the 16-bit batch field; the tensor-core prefill GEMM). */
+ * rows (the 16-bit batch field; the tensor-core prefill GEMM), bit 7 the commands for several sequences (opcodes 18
+ * to 23). */
 #define B200Q_FEATURES 0x6B51FFFFu
 #define B200Q_FEATURES2 0x6B520001u
-#define B200Q_FEATURES3 0x6B53007Fu
+#define B200Q_FEATURES3 0x6B5300FFu
 
 /* ---- status codes ------------------------------------------------------------------------------------------ */
 #define B200Q_OK 0
