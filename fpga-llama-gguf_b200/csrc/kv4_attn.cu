@@ -25,15 +25,13 @@ namespace b200q {
 namespace {
 
 constexpr unsigned kWarps = 4, kThreads = kWarps * 32;
-#ifndef UC
-#define UC 24
-#endif
-constexpr unsigned kUnitCost = UC;        // what a unit costs besides its tiles (its queries, its joined output), in tiles
 constexpr unsigned kMaxRange = 1024;     // a warp adds at most 256 tiles into its accumulators before they are joined in FP32
-#ifndef PW
-#define PW 6144
-#endif
-constexpr unsigned kPromptRows = 64, kPromptWork = PW;
+// What a unit costs besides its tiles, in tiles: its queries' way into matrix operands, the joining of its warps' outputs,
+// the start of its copies. 64 requests of 5 to 8192 keys, three rows of 32 heads of 128 each: 87 us with 9, 74 with 12, 70
+// with 16, 74 with 24 (short requests pile up on a CTA with less, its long ones wait with more).
+constexpr unsigned kUnitCost = 16;
+// Requests with this many rows (token, head of a KV head's group) are the prompt kernel's when a call has work for it.
+constexpr unsigned kPromptRows = 64, kPromptWork = 6144;
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ void tell(uint32_t *status, unsigned bit) {
@@ -49,7 +47,7 @@ struct AttnPlan {
 };
 
 // ---- the schedule ---------------------------------------------------------------------------------------------------
-// A unit is a group of up to 4 or 8 query rows of one KV head; its work is the tiles of keys that they see. All units' tiles
+// A unit is a group of up to 4, 8, 12 or 16 query rows of one KV head; its work is the tiles of keys that they see. All units' tiles
 // lie in one line, a unit's kUnitCost and its tiles behind the unit before it, and the line is cut into ranges of equal
 // length, one a CTA (several, when a range would pass kMaxRange): every CTA has the same to do whatever the requests'
 // lengths, and at most two of a range's pieces are parts of a unit: one that an earlier range began (its
@@ -197,8 +195,10 @@ __device__ __forceinline__ half2 as_h2(uint32_t x) { return *reinterpret_cast<ha
 // K: left as they are they read c 2^-24 (16 c 2^-24), and the 8 that a code stands above its value comes off in the sum.
 __device__ __forceinline__ uint32_t low_raw(uint32_t x) { return x & 0x000f000fu; }
 __device__ __forceinline__ uint32_t high_raw(uint32_t x) { return x & 0x00f000f0u; }
+
 // V (whose sums run over many tokens, where that 8 would swamp them): put into the mantissa of 1024 they read 1024 + c
-// (1024 + 16 c); less 1032 (1152) that is c - 8 (16 (c - 8)), exactly.
+// (1024 + 16 c); less 1032 (1152) that is c - 8 (16 (c - 8)), exactly. (A product of its own that takes the 8 off, with raw
+// codes beside it, measured the same with one set of rows and more with several.)
 __device__ __forceinline__ uint32_t low_codes(uint32_t x) {
     uint32_t y;
     asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;" : "=r"(y) : "r"(x));
@@ -265,20 +265,23 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {  // an 8 x 8 matrix
     return y;
 }
 
+// CTAs on an SM, by the accumulators a thread holds (8 for each of `blocks` = NB NT) and the registers they leave: 128, 168 or
+// 255 a thread. One query token of four heads on 131,000 keys, us a call with 2 / 3 / 4 CTAs: heads of 64 31.8 / 25.9 /
+// 24.9, of 128 35.9 / 32.3 / 33.4, of 256 47.7 / 48.9 / -.
+constexpr unsigned ctas_of(unsigned blocks) { return blocks <= 2 ? 4 : blocks <= 4 ? 3 : 2; }
+// Sets of four rows that a unit may have, as far as their accumulators fit the registers. Twelve rows of heads of 128 in one
+// unit took 1430 cycles a tile, in two (of eight and four rows) 2200.
+constexpr unsigned most_sets(unsigned nb) { return nb <= 4 ? 4 : 16 / nb; }
+
 // NB: 32-dim blocks of a head; NT: sets of four query rows.
 template <int NB, int NT>
 struct Shape {
     static constexpr int kTile = NB * 576;                       // bytes of a tile
-    #ifndef TS
-#define TS 3
-#define TQ 4
-#define TC 3
-#endif
-    static constexpr int kSlots = NB <= 2 ? 8 : NB <= 4 ? TS * 2 : TS;  // tiles a warp has on their way
+    static constexpr int kSlots = NB <= 2 ? 8 : NB <= 4 ? 6 : 3;  // tiles a warp has on their way: all CTAs' rings fill shared memory
     static constexpr int kRows = NT * 4;
-    static constexpr int kCtas = NB * NT <= 8 ? TC : 2;           // on an SM, by the accumulators' registers (8 NB NT a thread)
-    static constexpr bool kQInRegs = NB * NT <= TQ;
-    static constexpr int kQBytes = kQInRegs ? 0 : NT * NB * 2 * 32 * 8;
+    static constexpr int kCtas = ctas_of(NB * NT);           // on an SM, by the accumulators' registers (8 NB NT a thread)
+    static constexpr bool kQInRegs = NB * NT <= 8;                // 4 registers a block and set; with more they stay in shared memory
+    static constexpr int kQBytes = NT * NB * 2 * 32 * 8;
     static constexpr int kOutBytes = kWarps * kRows * NB * 32 * 4;  // the warps' results
     static constexpr int kRing = kWarps * kSlots * kTile;
     static constexpr int kSmem = kQBytes + kOutBytes + kRing;
@@ -297,6 +300,7 @@ __global__ void __launch_bounds__(kThreads, Shape<NB, NT>::kCtas) kv4_attn_kerne
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint64_t bars[kWarps][S::kSlots];
     __shared__ float m_of[kWarps][S::kRows], l_of[kWarps][S::kRows];
+    __shared__ float start_of[S::kRows][NB], scale_of[S::kRows];
     auto *before = reinterpret_cast<unsigned *>(smem + S::kSmem);
     const unsigned tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const unsigned per = a.n_head / a.c.n_kv, tiles_per_page = a.c.page / kTileTokens;
@@ -377,9 +381,9 @@ __global__ void __launch_bounds__(kThreads, Shape<NB, NT>::kCtas) kv4_attn_kerne
 
     // A warp's tiles: the k-th lies where lane k % 32 keeps.
     Piece pc;
-    unsigned done = 0;     // tiles this warp has taken from its ring before this piece (slot and phase go by it)
-    unsigned ahead = 0;    // of the piece's tiles, fetched
-    unsigned present = 0;  // bit s: slot s holds a tile
+    unsigned slot = 0, phase = 0;  // of the warp's next tile
+    unsigned ahead = 0;            // of the piece's tiles, fetched
+    unsigned present = 0;          // bit s: slot s holds a tile
     const uint8_t *where = nullptr;
     bool late = false;
     auto look_up = [&](unsigned k) {
@@ -390,9 +394,8 @@ __global__ void __launch_bounds__(kThreads, Shape<NB, NT>::kCtas) kv4_attn_kerne
             else tell(a.status, kServePage);
         }
     };
-    auto fetch = [&](unsigned k) {
+    auto fetch = [&](unsigned k, unsigned slot) {
         const uint8_t *src = reinterpret_cast<const uint8_t *>(__shfl_sync(~0u, (unsigned long long)where, k % 32));
-        const unsigned slot = (done + k) % S::kSlots;
         if (lane == 0) {
             if (src) {
                 mbar_expect_tx(&bars[warp][slot], S::kTile);
@@ -408,22 +411,88 @@ __global__ void __launch_bounds__(kThreads, Shape<NB, NT>::kCtas) kv4_attn_kerne
     };
     auto begin_piece = [&] {
         look_up(lane);
-        for (ahead = 0; ahead < unsigned(S::kSlots) && ahead < pc.mine; ++ahead) fetch(ahead);
+        unsigned s = slot;
+        for (ahead = 0; ahead < unsigned(S::kSlots) && ahead < pc.mine; ++ahead) {
+            fetch(ahead, s);
+            s = s + 1 == unsigned(S::kSlots) ? 0 : s + 1;
+        }
+    };
+    // waits (each bounded) for n tiles on their way, from the next one on
+    auto land = [&](unsigned n) {
+        for (unsigned i = 0, s = slot, p = phase; i < n; ++i) {
+            mbar_wait(&bars[warp][s], p);
+            if (++s == unsigned(S::kSlots)) s = 0, p ^= 1;
+        }
+    };
+
+    // A warp takes the rows warp, warp + 4, ...; lane: four dims (of 128), then the four 128 behind them.
+    constexpr int kQuads = (NB * 8 + 31) / 32;
+    float4 x[NT][kQuads];
+    const bool wide = ((reinterpret_cast<uintptr_t>(a.q) | a.q_stride * 4 | a.q_head_stride * 4) & 15) == 0;
+    auto load_q = [&] {
+#pragma unroll
+        for (int m = 0; m < NT; ++m) {
+            const unsigned at = pc.row0 + m * 4 + warp, row = at < pc.all ? at : pc.row0;
+            const float *src = a.q + (pc.start + row / per) * a.q_stride + (pc.head * per + row % per) * a.q_head_stride + lane * 4;
+#pragma unroll
+            for (int i = 0; i < kQuads; ++i) {
+                x[m][i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (lane + 32 * i >= NB * 8) break;
+                const float *at_i = src + i * 128;
+                if (wide) x[m][i] = *reinterpret_cast<const float4 *>(at_i);
+                else x[m][i] = make_float4(at_i[0], at_i[1], at_i[2], at_i[3]);
+            }
+        }
     };
 
     bool more = next_piece(pc);
-    if (more) begin_piece();
+    if (more) {
+        load_q();
+        begin_piece();
+    }
     while (more) {
         // The queries as B operands, in the order in which a block's words hold the dims: column g is the upper (g even) or
-        // lower part of row g / 2.
+        // lower part of row g / 2. With them -8 sum q over each block, for the 8 that K's codes stand too high.
+        const unsigned all = pc.all, row0 = pc.row0, mine = pc.mine;
+        const int base = pc.base;
+#pragma unroll
+        for (int m = 0; m < NT; ++m) {
+            float big = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kQuads; ++i) big = fmaxf(big, fmaxf(fmaxf(fabsf(x[m][i].x), fabsf(x[m][i].y)), fmaxf(fabsf(x[m][i].z), fabsf(x[m][i].w))));
+            big = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(big)));
+            int ex = int(__float_as_uint(big) >> 23) - 127 - 10;  // x / 2^ex is below 2^11
+            ex = ex < -110 ? -110 : ex > 100 ? 100 : ex;
+            const float down = __uint_as_float(unsigned(127 - ex) << 23);
+            if (lane == 0) scale_of[m * 4 + warp] = a.scale * kLog2e * __uint_as_float(unsigned(127 + 24 + ex) << 23);  // (K's codes come times 2^-24)
+#pragma unroll
+            for (int i = 0; i < kQuads; ++i) {
+                const unsigned quad = lane + 32 * i, set = quad / 4;
+                const bool high = set & 1;  // the high nibbles' codes come times 16
+                const float f = high ? down * 0.0625f : down;
+                uint32_t h0, l0, h1, l1;
+                split2(x[m][i].x * f, x[m][i].z * f, h0, l0);
+                split2(x[m][i].y * f, x[m][i].w * f, h1, l1);
+                const float2 s0 = __half22float2(as_h2(h0)), s1 = __half22float2(as_h2(l0)), s2 = __half22float2(as_h2(h1)),
+                             s3 = __half22float2(as_h2(l1));
+                float sum_q = (high ? 16.0f : 1.0f) * (((s0.x + s0.y) + (s2.x + s2.y)) + ((s1.x + s1.y) + (s3.x + s3.y)) * (1.0f / 2048));
+                sum_q += __shfl_xor_sync(~0u, sum_q, 1);
+                sum_q += __shfl_xor_sync(~0u, sum_q, 2);
+                sum_q += __shfl_xor_sync(~0u, sum_q, 4);
+                if (quad < NB * 8) {
+                    uint8_t *to = smem + ((m * NB * 2 + set) * 32 + warp * 8 + quad % 4) * 8;
+                    *reinterpret_cast<uint2 *>(to) = make_uint2(h0, h1);
+                    *reinterpret_cast<uint2 *>(to + 32) = make_uint2(l0, l1);
+                    if (quad % 8 == 0) start_of[m * 4 + warp][quad / 8] = -0x1p-21f * sum_q;
+                }
+            }
+        }
+        __syncthreads();
         uint32_t qb[S::kQInRegs ? NT : 1][S::kQInRegs ? NB * 2 : 1][2];
-        float start[NT][NB];    // -8 sum q over a block, of row t
-        float scale[NT];        // of row t
+        float start[NT][NB];    // of row t
+        float scale[NT];
         int pos[NT], low[NT];   // the keys row t sees: [low, pos]
         int wpos[NT], wlow[NT]; // and row g / 2
-        const unsigned all = pc.all, row0 = pc.row0, head = pc.head, mine = pc.mine;
-        const int base = pc.base;
-        const bool wide = ((reinterpret_cast<uintptr_t>(a.q) | a.q_stride * 4 | a.q_head_stride * 4) & 15) == 0;
         auto sees = [&](unsigned row, int &lo, int &hi) {
             const int p = base + int(row / per);
             hi = row < all ? p : -1;
@@ -433,52 +502,17 @@ __global__ void __launch_bounds__(kThreads, Shape<NB, NT>::kCtas) kv4_attn_kerne
         for (int m = 0; m < NT; ++m) {
             sees(row0 + m * 4 + t, low[m], pos[m]);
             sees(row0 + m * 4 + g / 2, wlow[m], wpos[m]);
-            const unsigned row = row0 + m * 4 + g / 2 < all ? row0 + m * 4 + g / 2 : row0;
-            const float *src = a.q + (pc.start + row / per) * a.q_stride + (head * per + row % per) * a.q_head_stride + t * 4;
-            float x[NB * 2][4], top = 0.0f;
+            scale[m] = scale_of[m * 4 + t];
 #pragma unroll
-            for (int i = 0; i < NB * 2; ++i) {
-                if (wide) {
-                    const float4 v = *reinterpret_cast<const float4 *>(src + i * 16);
-                    x[i][0] = v.x, x[i][1] = v.y, x[i][2] = v.z, x[i][3] = v.w;
-                } else {
-                    for (int e = 0; e < 4; ++e) x[i][e] = src[i * 16 + e];
+            for (int b = 0; b < NB; ++b) start[m][b] = start_of[m * 4 + t][b];
+            if constexpr (S::kQInRegs) {
+#pragma unroll
+                for (int i = 0; i < NB * 2; ++i) {
+                    const uint2 v = *reinterpret_cast<const uint2 *>(smem + ((m * NB * 2 + i) * 32 + lane) * 8);
+                    qb[m][i][0] = v.x, qb[m][i][1] = v.y;
                 }
-            }
-#pragma unroll
-            for (int i = 0; i < NB * 2; ++i)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(x[i][e]));
-            top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-            int ex = int(__float_as_uint(top) >> 23) - 127 - 10;  // x / 2^ex is below 2^11
-            ex = ex < -110 ? -110 : ex > 100 ? 100 : ex;
-            const float down = __uint_as_float(unsigned(127 - ex) << 23);
-            scale[m] = a.scale * kLog2e * __uint_as_float(unsigned(127 + 24 + ex) << 23);  // (K's codes come times 2^-24)
-            scale[m] = __shfl_sync(~0u, scale[m], t * 8);
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                float sum_q = 0.0f;
-#pragma unroll
-                for (int i = 2 * b; i < 2 * b + 2; ++i) {
-                    const float f = i & 1 ? down * 0.0625f : down;  // the high nibbles' codes come times 16
-                    uint32_t h0, l0, h1, l1;
-                    split2(x[i][0] * f, x[i][2] * f, h0, l0);
-                    split2(x[i][1] * f, x[i][3] * f, h1, l1);
-                    const float2 s0 = __half22float2(as_h2(h0)), s1 = __half22float2(as_h2(l0)), s2 = __half22float2(as_h2(h1)),
-                                 s3 = __half22float2(as_h2(l1));
-                    sum_q += (i & 1 ? 16.0f : 1.0f) * (((s0.x + s0.y) + (s2.x + s2.y)) + ((s1.x + s1.y) + (s3.x + s3.y)) * (1.0f / 2048));
-                    const uint2 mine_q = make_uint2(g & 1 ? l0 : h0, g & 1 ? l1 : h1);
-                    if constexpr (S::kQInRegs) qb[m][i][0] = mine_q.x, qb[m][i][1] = mine_q.y;
-                    else if (warp == 0) *reinterpret_cast<uint2 *>(smem + ((m * NB * 2 + i) * 32 + lane) * 8) = mine_q;
-                }
-                sum_q += __shfl_xor_sync(~0u, sum_q, 1);
-                sum_q = -0x1p-21f * (sum_q + __shfl_xor_sync(~0u, sum_q, 2));
-                start[m][b] = __shfl_sync(~0u, sum_q, t * 8);
             }
         }
-
-        if constexpr (!S::kQInRegs) __syncthreads();
 
         float o[NT][NB * 2][4], top[NT], sum[NT], limit = 0.0f, lift = 1.0f, lift_d = 1.0f;
 #pragma unroll
@@ -691,52 +725,32 @@ __global__ void __launch_bounds__(kThreads, Shape<NB, NT>::kCtas) kv4_attn_kerne
             }
         };
 
-        // Tile k's values are taken beside tile k + 1's scores: two chains that do not wait for one another.
         float s[NT][2];
-        auto arrived = [&](unsigned k) {
-            const unsigned slot = (done + k) % S::kSlots, phase = (done + k) / S::kSlots & 1;
-            if (!__any_sync(~0u, !mbar_wait(&bars[warp][slot], phase))) return true;
-            // A copy did not arrive. Let those on their way land (each wait is bounded again); the CTA stops below.
-            for (unsigned i = k; i < ahead; ++i) mbar_wait(&bars[warp][(done + i) % S::kSlots], (done + i) / S::kSlots & 1);
-            late = true;
-            return false;
-        };
-        auto key_of = [&](unsigned k) { return int((pc.tile0 + k * kWarps) * kTileTokens); };
-        auto tile_of = [&](unsigned k) { return ring + (done + k) % S::kSlots * S::kTile; };
-        auto is_there = [&](unsigned k) { return present >> (done + k) % S::kSlots & 1; };
-        if (mine && arrived(0) && is_there(0)) {
-            score(tile_of(0), s);
-            weigh(key_of(0), s);
-        }
-        for (unsigned k = 0; k < mine && !late; ++k) {
-            const bool next = k + 1 < mine && arrived(k + 1) && is_there(k + 1);
-            if (late) break;
-            if (is_there(k)) {
-                if (next) {
-                    float ns[NT][2];
-                    score(tile_of(k + 1), ns);
-                    value(tile_of(k), key_of(k), s);
-                    weigh(key_of(k + 1), ns);
-#pragma unroll
-                    for (int m = 0; m < NT; ++m) s[m][0] = ns[m][0], s[m][1] = ns[m][1];
-                } else {
-                    value(tile_of(k), key_of(k), s);
-                }
-            } else if (next) {
-                score(tile_of(k + 1), s);
-                weigh(key_of(k + 1), s);
+        int key0 = int(pc.tile0 * kTileTokens);
+        for (unsigned k = 0; k < mine; ++k) {
+            if (__any_sync(~0u, !mbar_wait(&bars[warp][slot], phase))) {
+                land(ahead - k);  // a copy did not arrive: those on their way land, and the CTA stops below
+                late = true;
+                break;
+            }
+            const uint8_t *tile = ring + slot * S::kTile;
+            if (present >> slot & 1) {
+                score(tile, s);
+                weigh(key0, s);
+                value(tile, key0, s);
             }
             __syncwarp();
-            if (ahead < mine) {  // tile k's slot is free again
+            if (ahead < mine) {  // the tile's slot is free again, for the one kSlots behind it
                 if (ahead % 32 == 0) look_up(ahead + lane);
-                fetch(ahead);
+                fetch(ahead, slot);
                 ++ahead;
             }
+            if (++slot == unsigned(S::kSlots)) slot = 0, phase ^= 1;
+            key0 += int(kWarps * kTileTokens);
         }
         const Piece was = pc;
-        done += mine;
-        ahead = 0;
         if (!late) {
+            ahead = 0;
             more = next_piece(pc);
             if (more) begin_piece();  // the next piece's tiles come while this one's results are joined
         }
@@ -759,10 +773,11 @@ __global__ void __launch_bounds__(kThreads, Shape<NB, NT>::kCtas) kv4_attn_kerne
         }
         if (__syncthreads_or(late)) {
             // some copy did not arrive: let the others land (each wait is bounded again), and stop
-            for (unsigned i = 0; i < ahead; ++i) mbar_wait(&bars[warp][(done + i) % S::kSlots], (done + i) / S::kSlots & 1);
+            if (!late) land(ahead);
             if (tid == 0) tell(a.status, kServeWait);
             return;
         }
+        if (more) load_q();
         for (unsigned i = tid; i < S::kRows * D / 4; i += kThreads) {
             const unsigned row = i / (D / 4), dim = i % (D / 4) * 4, at = was.row0 + row;
             if (at >= was.all) break;
@@ -887,13 +902,30 @@ cudaError_t launch_tiles(const Kv4AttnArgs &a, const AttnPlan &plan, unsigned gr
     return launch_pdl(a.pdl, kv4_attn_kernel<NB, NT>, dim3(grid), dim3(kThreads), S::kSmem + (size_t(a.n_req) + 1) * 4, st, a, plan);
 }
 
+template <int NB>
+cudaError_t launch_sets(const Kv4AttnArgs &a, const AttnPlan &plan, cudaStream_t st) {
+    switch (plan.rows / 4) {
+        case 1: return launch_tiles<NB, 1>(a, plan, plan.grid, st);
+        case 2: return launch_tiles<NB, 2>(a, plan, plan.grid, st);
+        case 3:
+            if constexpr (most_sets(NB) >= 3) return launch_tiles<NB, 3>(a, plan, plan.grid, st);
+            break;
+        case 4:
+            if constexpr (most_sets(NB) >= 4) return launch_tiles<NB, 4>(a, plan, plan.grid, st);
+            break;
+    }
+    return cudaErrorInvalidValue;
+}
+
 AttnPlan plan_of(const Kv4AttnArgs &a, unsigned sms) {
     AttnPlan p;
     const unsigned per = a.n_head / a.c.n_kv;
-    const unsigned sets = (unsigned long long)a.max_q * per > 4 ? 2 : 1;
+    const unsigned nb = a.c.dim / 32, most = most_sets(nb) * 4;
+    const unsigned long long rows_of = (unsigned long long)a.max_q * per, groups_of = (rows_of + most - 1) / most;
+    const unsigned sets = unsigned((rows_of + groups_of * 4 - 1) / (groups_of * 4));
     p.rows = 4 * sets;
     if ((unsigned long long)a.max_q * per >= kPromptRows && (unsigned long long)a.n_rows * a.n_head >= kPromptWork) p.most_rows = kPromptRows - 1;
-    p.grid = sms * (a.c.dim / 32 * sets <= 8 ? TC : 2);  // as many as run at once
+    p.grid = sms * ctas_of(nb * sets);  // as many as run at once
     // the most units there can be, and the line's length
     const unsigned long long q = a.max_q < a.n_rows ? a.max_q : a.n_rows, rows = (unsigned long long)a.n_rows * per;
     unsigned long long groups = rows / p.rows + (a.n_req < a.n_rows ? a.n_req : a.n_rows);
@@ -921,16 +953,17 @@ unsigned kv4_attn_launches(const Kv4AttnArgs &a, unsigned sms) {
 
 cudaError_t launch_kv4_attn(const Kv4AttnArgs &a, unsigned sms, cudaStream_t st) {
     const AttnPlan p = plan_of(a, sms);
-    const unsigned nb = a.c.dim / 32;
     cudaError_t e = cudaErrorInvalidValue;
-#define B200Q_TILES(NB)                                                       \
-    case NB:                                                                 \
-        e = p.rows == 4 ? launch_tiles<NB, 1>(a, p, p.grid, st) : launch_tiles<NB, 2>(a, p, p.grid, st); \
-        break;
-    switch (nb) {
-        B200Q_TILES(1) B200Q_TILES(2) B200Q_TILES(3) B200Q_TILES(4) B200Q_TILES(5) B200Q_TILES(6) B200Q_TILES(7) B200Q_TILES(8)
+    switch (a.c.dim / 32) {
+        case 1: e = launch_sets<1>(a, p, st); break;
+        case 2: e = launch_sets<2>(a, p, st); break;
+        case 3: e = launch_sets<3>(a, p, st); break;
+        case 4: e = launch_sets<4>(a, p, st); break;
+        case 5: e = launch_sets<5>(a, p, st); break;
+        case 6: e = launch_sets<6>(a, p, st); break;
+        case 7: e = launch_sets<7>(a, p, st); break;
+        case 8: e = launch_sets<8>(a, p, st); break;
     }
-#undef B200Q_TILES
     if (e != cudaSuccess) return e;
     if (p.max_ranges > 1) {  // (else nothing lies in two ranges)
         const unsigned edges = p.max_ranges - 1;
