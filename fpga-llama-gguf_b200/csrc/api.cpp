@@ -744,7 +744,7 @@ int exec_serve(b200q_ctx *c, const Pass &p) {
         const BeamSelectArgs a = beam_select_args(c, p);
         if (!a.room || c->serve_room_bytes < beam_select_room(a)) return set_err(c, B200Q_ERR_STATE, "BEAM_SELECT: workspace not prepared");
         kernels = 2;
-        CUDA_TRY(c, launch_beam_select(a, c->stream));
+        CUDA_TRY(c, launch_beam_select(a, unsigned(c->sms), c->stream));
     } else if (p.op == 22) {
         BeamReorderArgs a;
         a.n_req = w[1];

@@ -55,120 +55,172 @@ __device__ __forceinline__ unsigned reached_by(unsigned mine, unsigned n, unsign
     return __reduce_max_sync(~0u, low);
 }
 
-// Of 8192 logits of one row: the maximum m, sum e^(x - m), and the n_out best in order. The logits are read once, by
-// asynchronous copies into shared memory (a thread's own: no registers held and no barrier, so that five CTAs an SM
-// keep loads on their way while others compute): the threads' own best give a bound that n_out reach, and the few
-// candidates at or above it are ranked by counting. Should ties put more than kFound there, the best are taken out one
-// by one.
-constexpr unsigned kFound = 512;
+// A segment of a row: some chunks of 8192 logits after one another. Of them the maximum m, sum e^(x - m), and the n_out best in
+// order. The logits are read once, by asynchronous copies into shared memory (a thread's own, so no barrier; the next
+// chunk's are on their way while one is looked through). A thread keeps a maximum and a sum of its own. In the first chunk
+// the threads' own best give a bound that n_out of them reach; what is above it in the segment's chunks, some dozens each, is
+// collected and ranked by counting at the end. Should more come together, the n_out best so far are taken out first and the
+// worst of them is the bound from then on; should ties put more there than can be held, they are taken out one by one.
+// 16 requests of 8 beams over 151,936 logits, 16 each: 26 us, and 8 for the lists' merge behind it (the bytes alone: 12). A
+// chunk takes a CTA 1.9 us (0.6 to issue the next one's copies, 0.2 maxima, 0.5 exponentials, 0.4 candidates and the barrier),
+// at which three CTAs an SM ask for all of the memory's rate; the first one (2.5 with its bound) and the end (1.5) do not. With
+// a list a chunk instead, each ranked by itself and five CTAs an SM, the whole call took 40 us (36 now), with chunks of
+// 4096 57.
+constexpr unsigned kFound = 512, kSelCtas = 3;  // CTAs on an SM, by shared memory
+static_assert(kSelPer == 32 && kFound / 2 > kMaxBeamOut);
 template <bool kWide>  // rows on 16 bytes
-__global__ void __launch_bounds__(kSelThreads, 5) beam_chunk_kernel(const BeamSelectArgs a, unsigned long long *list, float2 *stat) {
-    __shared__ __align__(16) float values[kSelChunk];
-    __shared__ unsigned long long found[kFound], kept[kMaxBeamOut], best_of[kSelThreads / 32];
+__global__ void __launch_bounds__(kSelThreads, kSelCtas)
+    beam_chunk_kernel(const BeamSelectArgs a, unsigned long long *list, float2 *stat, unsigned chunks) {
+    extern __shared__ __align__(16) float rooms[];  // two chunks, or the segment's only one
+    __shared__ __align__(16) unsigned long long found[kFound];
+    __shared__ unsigned long long kept[kMaxBeamOut], best_of[kSelThreads / 32];
     __shared__ unsigned sorted[kSelThreads / 32][32];
-    __shared__ unsigned n_found;
-    __shared__ float red[kSelThreads / 32];
+    __shared__ unsigned more_found[3];
+    __shared__ float2 sums[kSelThreads / 32];
     pdl_wait();
     pdl_launch_dependents();
-    const unsigned tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, chunk = blockIdx.x, row = blockIdx.y, first = chunk * kSelChunk;
+    const unsigned tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row = blockIdx.y, n_out = a.n_out;
+    const unsigned c0 = unsigned((unsigned long long)chunks * blockIdx.x / gridDim.x), c1 = unsigned((unsigned long long)chunks * (blockIdx.x + 1) / gridDim.x);
     const float *x = a.logits + row * a.stride;
+    auto place = [&](unsigned i) { return (i / 4 * kSelThreads + tid) * 4 + i % 4; };  // of the thread's value i in a chunk
+    auto fetch = [&](unsigned chunk, float *values) {
+        const unsigned first = chunk * kSelChunk;
 #pragma unroll
-    for (unsigned i = 0; i < kSelPer; i += 4) {  // four values of this thread
-        float *to = values + (i / 4 * kSelThreads + tid) * 4;
-        const unsigned at = first + (i / 4 * kSelThreads + tid) * 4;
-        if (kWide && at + 4 <= a.vocab) {
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(to)), "l"(x + at) : "memory");
-        } else {
-            for (unsigned e = 0; e < 4; ++e) {
-                if (at + e < a.vocab) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_addr(to + e)), "l"(x + at + e) : "memory");
-                else to[e] = -INFINITY;
-            }
-        }
-    }
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    auto token = [&](unsigned i) { return first + (i / 4 * kSelThreads + tid) * 4 + i % 4; };
-    auto four = [&](unsigned i) { return *reinterpret_cast<const float4 *>(values + (i / 4 * kSelThreads + tid) * 4); };
-    float m = -INFINITY;  // (fmaxf passes a NaN over)
-#pragma unroll
-    for (unsigned i = 0; i < kSelPer; i += 4) {
-        const float4 y = four(i);
-        m = fmaxf(fmaxf(m, y.x), fmaxf(fmaxf(y.y, y.z), y.w));
-    }
-    if (tid == 0) n_found = 0;
-    float top = m;
-    for (unsigned o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-    if (lane == 0) red[warp] = top;
-    const unsigned limit = reached_by<kSelThreads / 32>(order_of(m), a.n_out, sorted);  // (with a barrier)
-    const float floor = limit ? __uint_as_float(limit & 0x80000000u ? limit & 0x7FFFFFFFu : ~limit) : -3.402823466e38f;
-    if (m >= floor) {
         for (unsigned i = 0; i < kSelPer; i += 4) {
-            const float4 y = four(i);
-            if (!(fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w)) >= floor)) continue;
-            for (unsigned e = 0; e < 4; ++e) {
-                const float v = e == 0 ? y.x : e == 1 ? y.y : e == 2 ? y.z : y.w;
-                if (!(v >= floor)) continue;
-                const unsigned at = atomicAdd(&n_found, 1u);
-                if (at < kFound) found[at] = cand(v, token(i + e));
+            float *to = values + place(i);
+            const unsigned at = first + place(i);
+            if (kWide && at + 4 <= a.vocab) {
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(to)), "l"(x + at) : "memory");
+            } else {
+                for (unsigned e = 0; e < 4; ++e) {
+                    if (at + e < a.vocab) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_addr(to + e)), "l"(x + at + e) : "memory");
+                    else to[e] = -INFINITY;
+                }
             }
         }
-    }
-    top = red[0];
-#pragma unroll
-    for (unsigned w = 1; w < kSelThreads / 32; ++w) top = fmaxf(top, red[w]);
-    // e^(x - m) as a power of two (a chunk without a finite logit adds nothing)
-    const float shift = top == -INFINITY ? 0.0f : top;
-    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    auto power = [&](float v) {  // (a NaN counts as -inf)
-        float e;
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"((fmaxf(v, -INFINITY) - shift) * 1.4426950408889634f));
-        return e;
+        asm volatile("cp.async.commit_group;" ::: "memory");
     };
-#pragma unroll
-    for (unsigned i = 0; i < kSelPer; i += 4) {
-        const float4 y = four(i);
-        s[0] += power(y.x), s[1] += power(y.y), s[2] += power(y.z), s[3] += power(y.w);
-    }
-    float sum = (s[0] + s[1]) + (s[2] + s[3]);
-    for (unsigned o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-    __syncthreads();  // found is whole, red is read
-    if (lane == 0) red[warp] = sum;
-    const unsigned n = n_found;
-    if (n <= kFound) {
+    fetch(c0, rooms);
+    if (tid < 3) more_found[tid] = 0;
+    __syncthreads();
+    float m = -INFINITY, sum = 0.0f;  // of the thread's values so far
+    float floor = -INFINITY;          // candidates are above it
+    unsigned have = 0;                // of them
+    // The best n_out of n candidates (kept, or written out), and 0 where there are fewer.
+    auto rank = [&](unsigned n, unsigned long long *to) {
+        if (n % 2 && tid == 0) found[n] = 0;  // (n < kFound)
+        __syncthreads();
         for (unsigned i = tid; i < n; i += kSelThreads) {
             const unsigned long long c = found[i];
             unsigned r = 0;
-            for (unsigned j = 0; j < n; ++j) r += found[j] > c;
-            if (r < a.n_out) kept[r] = c;
-        }
-        for (unsigned i = n + tid; i < a.n_out; i += kSelThreads) kept[i] = 0;
-    } else {
-        unsigned long long last = ~0ull;
-        for (unsigned r = 0; r < a.n_out; ++r) {
-            unsigned long long best = 0;
-            for (unsigned i = 0; i < kSelPer; ++i) {
-                const unsigned long long c = cand(values[(i / 4 * kSelThreads + tid) * 4 + i % 4], token(i));
-                if (c < last && c > best) best = c;
+#pragma unroll 8
+            for (unsigned j = 0; j < n; j += 2) {
+                const ulonglong2 y = *reinterpret_cast<const ulonglong2 *>(found + j);
+                r += (y.x > c) + (y.y > c);
             }
-            for (unsigned o = 16; o; o >>= 1) {
-                const unsigned long long y = __shfl_xor_sync(~0u, best, o);
-                best = y > best ? y : best;
-            }
-            __syncthreads();
-            if (lane == 0) best_of[warp] = best;
-            __syncthreads();
-            for (unsigned w = 0; w < kSelThreads / 32; ++w) best = best_of[w] > best ? best_of[w] : best;
-            last = best;
-            if (tid == 0) kept[r] = best;
+            if (r < n_out) to[r] = c;
         }
+        for (unsigned i = n + tid; i < n_out; i += kSelThreads) to[i] = 0;
+    };
+    for (unsigned c = c0; c < c1; ++c) {
+        const unsigned turn = c - c0, first = c * kSelChunk;
+        const float *values = rooms + turn % 2 * kSelChunk;
+        if (c + 1 < c1) {
+            fetch(c + 1, rooms + (turn + 1) % 2 * kSelChunk);
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+        } else {
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+        }
+        auto four = [&](unsigned i) { return *reinterpret_cast<const float4 *>(values + place(i)); };
+        float top = -INFINITY;  // (fmaxf passes a NaN over)
+#pragma unroll
+        for (unsigned i = 0; i < kSelPer; i += 4) {
+            const float4 y = four(i);
+            top = fmaxf(fmaxf(top, y.x), fmaxf(fmaxf(y.y, y.z), y.w));
+        }
+        if (floor == -INFINITY) {
+            const unsigned limit = reached_by<kSelThreads / 32>(order_of(top), n_out, sorted);
+            // the number below it (none lies between +0 and the largest negative one: -0 counts as +0)
+            if (limit > order_of(-3.402823466e38f)) floor = cand_logit((unsigned long long)(limit - (limit == 0x80000000u ? 2 : 1)) << 32);
+        }
+        // e^(x - m) as a power of two (values that are all -inf or NaN add nothing)
+        const float was = m;
+        m = fmaxf(m, top);
+        const float shift = m == -INFINITY ? 0.0f : m;
+        auto power = [&](float v) {  // (a NaN counts as -inf)
+            float e;
+            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"((fmaxf(v, -INFINITY) - shift) * 1.4426950408889634f));
+            return e;
+        };
+        if (was != m) sum *= power(was);
+        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        unsigned hits = 0;  // of the thread's values, those above the bound
+#pragma unroll
+        for (unsigned i = 0; i < kSelPer; i += 4) {
+            const float4 y = four(i);
+            s[0] += power(y.x), s[1] += power(y.y), s[2] += power(y.z), s[3] += power(y.w);
+            hits |= (y.x > floor ? 1u << i : 0u) | (y.y > floor ? 2u << i : 0u) | (y.z > floor ? 4u << i : 0u) | (y.w > floor ? 8u << i : 0u);
+        }
+        sum += (s[0] + s[1]) + (s[2] + s[3]);
+        if (hits) {
+            unsigned at = have + atomicAdd(&more_found[turn % 3], unsigned(__popc(hits)));
+            for (; hits; hits &= hits - 1, ++at) {
+                const unsigned i = place(__ffs(hits) - 1);
+                if (at < kFound) found[at] = cand(values[i], first + i);
+            }
+        }
+        if (tid == 0) more_found[(turn + 1) % 3] = 0;  // (last looked at two chunks ago)
+        __syncthreads();
+        const unsigned held = have;
+        have += more_found[turn % 3];
+        if (have < kFound / 2) continue;
+        if (have < kFound) {
+            rank(have, kept);
+        } else {
+            unsigned long long last = ~0ull;
+            for (unsigned r = 0; r < n_out; ++r) {
+                unsigned long long best = 0;
+                for (unsigned i = tid; i < held; i += kSelThreads)
+                    if (found[i] < last && found[i] > best) best = found[i];
+                for (unsigned i = 0; i < kSelPer; ++i) {
+                    const unsigned long long y = cand(values[place(i)], first + place(i));
+                    if (y < last && y > best) best = y;
+                }
+                for (unsigned o = 16; o; o >>= 1) {
+                    const unsigned long long y = __shfl_xor_sync(~0u, best, o);
+                    best = y > best ? y : best;
+                }
+                __syncthreads();
+                if (lane == 0) best_of[warp] = best;
+                __syncthreads();
+                for (unsigned w = 0; w < kSelThreads / 32; ++w) best = best_of[w] > best ? best_of[w] : best;
+                last = best;
+                if (tid == 0) kept[r] = best;
+            }
+        }
+        __syncthreads();
+        if (tid < n_out) found[tid] = kept[tid];
+        floor = cand_logit(kept[n_out - 1]);  // (a later token loses a tie)
+        have = n_out;
+        __syncthreads();
     }
+    const size_t at = size_t(row) * gridDim.x + blockIdx.x;
+    rank(have, list + at * n_out);
+    // the threads' maxima and sums
+    float all = m;
+    for (unsigned o = 16; o; o >>= 1) all = fmaxf(all, __shfl_xor_sync(~0u, all, o));
+    if (m != all) sum *= exp2f((m - all) * 1.4426950408889634f);
+    for (unsigned o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+    if (lane == 0) sums[warp] = make_float2(all, sum);
     __syncthreads();
-    const size_t at = size_t(row) * gridDim.x + chunk;
-    if (tid == 0) {
-        sum = red[0];
-        for (unsigned w = 1; w < kSelThreads / 32; ++w) sum += red[w];
-        stat[at] = make_float2(top, sum);
+    if (warp == 0) {
+        const float2 part = lane < kSelThreads / 32 ? sums[lane] : make_float2(-INFINITY, 0.0f);
+        m = part.x;
+        for (unsigned o = 4; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+        sum = part.x == m ? part.y : part.y * exp2f((part.x - m) * 1.4426950408889634f);
+        for (unsigned o = 4; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+        if (lane == 0) stat[at] = make_float2(m, sum);
     }
-    for (unsigned i = tid; i < a.n_out; i += kSelThreads) list[at * a.n_out + i] = kept[i];
 }
 
 // One CTA a request. A warp a beam: log sum e^x from the chunks' statistics (in 64 bits), and the n_out best of the
@@ -192,26 +244,29 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamSel
     const unsigned req = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = a.n_out;
     const size_t per_beam = size_t(chunks) * n;
     const unsigned long long *lists = list + size_t(req) * a.beams * per_beam;
-    auto *held = reinterpret_cast<unsigned long long *>(best + size_t(a.beams) * n);
+    auto *rank = reinterpret_cast<unsigned *>(best + size_t(a.beams) * n);
+    auto *held = reinterpret_cast<unsigned long long *>(rank + (size_t(a.beams) * n + 1) / 2 * 2);
+    for (unsigned i = threadIdx.x; i < a.beams * n; i += kMergeThreads) rank[i] = 0;
     for (unsigned b = warp; b < a.beams; b += kMergeThreads / 32) {
         const unsigned row = req * a.beams + b;
         const float score = a.scores[row];
         const float2 *st = stat + size_t(row) * chunks;
+        const float2 st0 = lane < chunks ? st[lane] : make_float2(-INFINITY, 0.0f);
         const unsigned long long *mine = lists + b * per_beam;
         if (in_smem) {
             for (unsigned i = lane; i < per_beam; i += 32) held[b * per_beam + i] = mine[i];
             mine = held + b * per_beam;
         }
-        float m = -INFINITY;
-        for (unsigned c = lane; c < chunks; c += 32) m = fmaxf(m, st[c].x);
+        float m = st0.x;
+        for (unsigned c = lane + 32; c < chunks; c += 32) m = fmaxf(m, st[c].x);
         for (unsigned o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-        double s = 0.0;
-        for (unsigned c = lane; c < chunks; c += 32)
+        double s = st0.x > -INFINITY ? double(st0.y) * exp2((double(st0.x) - double(m)) * 1.4426950408889634074) : 0.0;
+        for (unsigned c = lane + 32; c < chunks; c += 32)
             if (st[c].x > -INFINITY) s += double(st[c].y) * exp2((double(st[c].x) - double(m)) * 1.4426950408889634074);
         for (unsigned o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
         unsigned got = 0;
         if (fabsf(m) < INFINITY && fabsf(score) < INFINITY) {
-            const double offset = double(score) - (double(m) + log(s));
+            const double log_s = log(s);
             __syncwarp();
             unsigned long long head[kHeads];
             unsigned at[kHeads];
@@ -230,7 +285,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamSel
                 if (key == 0) break;
                 const unsigned low = __reduce_max_sync(~0u, unsigned(top >> 32) == key ? unsigned(top) : 0u);
                 if (unsigned(top >> 32) == key && unsigned(top) == low) {
-                    best[b * n + got] = Scored{offset + double(cand_logit(top)), cand_token(top)};
+                    best[b * n + got] = Scored{double(score) + ((double(cand_logit(top)) - double(m)) - log_s), cand_token(top)};
 #pragma unroll
                     for (unsigned i = 0; i < kHeads; ++i)
                         if (i == which) head[i] = ++at[i] < n ? mine[(i * 32 + lane) * n + at[i]] : 0;
@@ -242,27 +297,32 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamSel
     __syncthreads();
     unsigned total = 0;
     for (unsigned b = 0; b < a.beams; ++b) total += count[b];
-    for (unsigned i = threadIdx.x; i < a.beams * n; i += kMergeThreads) {
-        const unsigned b = i / n, k = i % n;
+    // A candidate's rank: its place in its own beam's list, and the places before it in every other one's, a thread a list.
+    for (unsigned p = threadIdx.x; p < a.beams * n * a.beams; p += kMergeThreads) {
+        const unsigned i = p / a.beams, x = p % a.beams, b = i / n, k = i % n;
         if (k >= count[b]) continue;
-        const Scored c = best[i];
-        unsigned rank = k;
-        for (unsigned x = 0; x < a.beams && rank < n; ++x) {
-            if (x == b) continue;
-            unsigned lo = 0, hi = count[x];  // candidates of beam x that come before c
+        unsigned before = k;
+        if (x != b) {
+            const double score = best[i].score;
+            unsigned lo = 0, hi = count[x];
             while (lo < hi) {
                 const unsigned mid = (lo + hi) / 2;
                 const double o = best[x * n + mid].score;
-                if (o > c.score || (o == c.score && x < b)) lo = mid + 1;
+                if (o > score || (o == score && x < b)) lo = mid + 1;
                 else hi = mid;
             }
-            rank += lo;
+            before = lo;
         }
-        if (rank < n) {
-            a.out[req * n + rank] = float(c.score);
-            a.parent[req * n + rank] = b;
-            a.token[req * n + rank] = c.token;
-        }
+        if (before) atomicAdd(&rank[i], before);
+    }
+    __syncthreads();
+    for (unsigned i = threadIdx.x; i < a.beams * n; i += kMergeThreads) {
+        const unsigned b = i / n;
+        if (i % n >= count[b] || rank[i] >= n) continue;
+        const Scored c = best[i];
+        a.out[req * n + rank[i]] = float(c.score);
+        a.parent[req * n + rank[i]] = b;
+        a.token[req * n + rank[i]] = c.token;
     }
     for (unsigned i = total + threadIdx.x; i < n; i += kMergeThreads) {
         a.out[req * n + i] = -INFINITY;
@@ -317,19 +377,25 @@ size_t beam_select_room(const BeamSelectArgs &a) {
     return lists * (a.n_out * sizeof(unsigned long long) + sizeof(float2));
 }
 
-cudaError_t launch_beam_select(const BeamSelectArgs &a, cudaStream_t st) {
+cudaError_t launch_beam_select(const BeamSelectArgs &a, unsigned sms, cudaStream_t st) {
     const unsigned chunks = chunks_of(a.vocab), rows = a.n_req * a.beams;
     auto *list = reinterpret_cast<unsigned long long *>(a.room);
     auto *stat = reinterpret_cast<float2 *>(list + size_t(rows) * chunks * a.n_out);
     const bool wide = ((reinterpret_cast<uintptr_t>(a.logits) | a.stride * 4) & 15) == 0;
-    const cudaError_t e = launch_pdl(a.pdl, wide ? beam_chunk_kernel<true> : beam_chunk_kernel<false>, dim3(chunks, rows), dim3(kSelThreads), 0, st, a, list, stat);
+    const auto kernel = wide ? beam_chunk_kernel<true> : beam_chunk_kernel<false>;
+    constexpr int kRooms = 2 * kSelChunk * sizeof(float);
+    cudaError_t e = ensure_smem_attr(reinterpret_cast<const void *>(kernel), kRooms);
     if (e != cudaSuccess) return e;
-    const size_t scored = size_t(a.beams) * a.n_out * sizeof(Scored), lists = size_t(a.beams) * chunks * a.n_out * 8;
+    // Segments: as many as run at once, as far as rows and chunks go round.
+    const unsigned fit = sms * kSelCtas / rows, segments = fit < 1 ? 1 : fit < chunks ? fit : chunks;
+    e = launch_pdl(a.pdl, kernel, dim3(segments, rows), dim3(kSelThreads), segments == chunks ? kRooms / 2 : kRooms, st, a, list, stat, chunks);
+    if (e != cudaSuccess) return e;
+    const size_t scored = size_t(a.beams) * a.n_out * sizeof(Scored) + (size_t(a.beams) * a.n_out + 1) / 2 * 8, lists = size_t(a.beams) * segments * a.n_out * 8;
     const unsigned in_smem = lists <= kListBytes;
-    const cudaError_t f = ensure_smem_attr(reinterpret_cast<const void *>(beam_merge_kernel), int(kMaxBeams * kMaxBeamOut * sizeof(Scored) + kListBytes));
-    if (f != cudaSuccess) return f;
+    e = ensure_smem_attr(reinterpret_cast<const void *>(beam_merge_kernel), int(kMaxBeams * kMaxBeamOut * (sizeof(Scored) + 4) + kListBytes));
+    if (e != cudaSuccess) return e;
     return launch_pdl(a.pdl, beam_merge_kernel, dim3(a.n_req), dim3(kMergeThreads), scored + (in_smem ? lists : 0), st, a,
-                      static_cast<const unsigned long long *>(list), static_cast<const float2 *>(stat), chunks, in_smem);
+                      static_cast<const unsigned long long *>(list), static_cast<const float2 *>(stat), segments, in_smem);
 }
 
 cudaError_t launch_beam_reorder(const BeamReorderArgs &a, cudaStream_t st) {

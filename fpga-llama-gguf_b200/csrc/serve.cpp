@@ -433,7 +433,7 @@ B200Q_API int b200q_beam_select(int device, const float *logits, unsigned vocab,
     c.memory("out_token", out_token, outs * 4, 4, true);
     c.memory("workspace", workspace, room, 16, true);
     c.check_memory();
-    if (c.ok()) c.cuda(launch_beam_select(a, c.stream()), "launch");
+    if (c.ok()) c.cuda(launch_beam_select(a, c.sms(), c.stream()), "launch");
     return c.rc();
 }
 

@@ -91,7 +91,7 @@ cudaError_t launch_kv4_attn(const Kv4AttnArgs &a, unsigned sms, cudaStream_t st)
 // requests of least_rows (token, head of the group) rows or more, on tcgen05; the others are left out
 cudaError_t launch_kv4_prompt(const Kv4AttnArgs &a, unsigned least_rows, cudaStream_t st);
 size_t beam_select_room(const BeamSelectArgs &a);
-cudaError_t launch_beam_select(const BeamSelectArgs &a, cudaStream_t st);
+cudaError_t launch_beam_select(const BeamSelectArgs &a, unsigned sms, cudaStream_t st);
 cudaError_t launch_beam_reorder(const BeamReorderArgs &a, cudaStream_t st);
 cudaError_t launch_kv4_reorder(const Kv4ReorderArgs &a, cudaStream_t st);
 // kernels that launch_kv4_attn starts (for launch counts; block_map_launches above likewise)
