@@ -190,27 +190,22 @@ __global__ void __launch_bounds__(256) kv4_store_kernel(const Kv4RowsArgs a) {
         }
 #pragma unroll
         for (unsigned i = 0; i < kRowsTurn; ++i) {
-            float best = 0.0f, amax = 0.0f;
-            bool bad = false;
+            float amax = fmaxf(fmaxf(fabsf(x[i][0]), fabsf(x[i][1])), fmaxf(fabsf(x[i][2]), fabsf(x[i][3])));
 #pragma unroll
-            for (unsigned e = 0; e < 4; ++e) {
-                bad = bad || !(fabsf(x[i][e]) <= 3.402823466e38f);
-                if (fabsf(x[i][e]) > amax) amax = fabsf(x[i][e]), best = x[i][e];
-            }
+            for (unsigned o = 1; o < 8; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, o));
+            // The sign of the first value that is as large, and whether one is none (fmaxf passes a NaN over)
+            float mine = x[i][3];
 #pragma unroll
-            for (unsigned o = 1; o < 8; o <<= 1) {
-                const float v = __shfl_xor_sync(~0u, best, o);
-                if (fabsf(v) > amax || (fabsf(v) == amax && (p.l & o))) best = v;  // the lower lanes' value on ties
-                amax = fabsf(best);
-            }
-            bad = __ballot_sync(~0u, bad) >> (threadIdx.x & 24) & 0xff;
-            const float d = best * -0.125f, inv = d != 0.0f ? fdiv(1.0f, d) : 0.0f;
-            uint32_t half = 0;
+            for (int e = 2; e >= 0; --e) mine = fabsf(x[i][e]) == amax ? x[i][e] : mine;
+            const unsigned has = __ballot_sync(~0u, fabsf(mine) == amax) >> (threadIdx.x & 24) & 0xff, minus = __ballot_sync(~0u, mine < 0.0f) >> (threadIdx.x & 24);
+            const float zero = fmaf(x[i][0], 0.0f, fmaf(x[i][1], 0.0f, fmaf(x[i][2], 0.0f, x[i][3] * 0.0f)));
+            const bool bad = __ballot_sync(~0u, zero != 0.0f) >> (threadIdx.x & 24) & 0xff;
+            const float d = amax * (minus & has & (0u - has) ? 0.125f : -0.125f), inv = d != 0.0f ? fdiv(1.0f, d) : 0.0f;
+            uint32_t code[4];
 #pragma unroll
-            for (unsigned e = 0; e < 4; ++e) {
-                const int q = bad ? 8 : int(fadd(fmul(x[i][e], inv), 8.5f));
-                half |= uint32_t(q < 15 ? (q < 0 ? 0 : q) : 15) << (8 * e);
-            }
+            for (unsigned e = 0; e < 4; ++e)  // (to an integer by an addition that drops what is behind the point; a NaN: 0)
+                code[e] = __float_as_uint(__fadd_rz(fminf(fmaxf(fadd(fmul(x[i][e], inv), 8.5f), 0.0f), 15.0f), 0x1p23f));
+            const uint32_t half = __byte_perm(__byte_perm(code[0], code[1], 0x0040), __byte_perm(code[2], code[3], 0x0040), 0x5410);
             const uint32_t high = __shfl_down_sync(~0u, half, 4);
             const unsigned slot = slots[i];
             if (slot == kNoSlot) continue;
