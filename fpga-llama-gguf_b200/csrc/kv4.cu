@@ -138,11 +138,11 @@ __global__ void __launch_bounds__(256) map_rows_kernel(const BlockMapArgs a) {
 // Eight lanes take a 32-dim block (four values each); lane l < 4 writes word l, whose high nibbles lane l + 4 holds.
 // The quantizer is Q4_0's: d = x[argmax |x|] / -8 (the first on ties), code = min(15, trunc(x (1 / d) + 8.5)), every step
 // rounded to FP32 by itself; a block that holds a NaN or an infinity gets a NaN scale, so that it reads back as NaN.
-__device__ __forceinline__ uint8_t *tile_of(const Kv4View &c, unsigned slot, unsigned head) {
-    const unsigned page = slot / c.page, t = slot % c.page / kTileTokens;
-    return c.base + ((size_t(page) * c.n_kv + head) * (c.page / kTileTokens) + t) * kv4_tile_bytes(c.dim);
-}
-
+// Both are bound by memory once there are rows enough: 8192 tokens of 8 heads of 128 stored and read back (145 MB) take 39 us,
+// 22 at the measured copy rate. What kept them from it was arithmetic (50 us): each thread's own divisions of the slot by the
+// page, the search for the largest value's sign, conversions at a quarter of the rate of additions. Two or eight rows a
+// turn took 43 and 45 us, a quarter of the CTAs 48.
+//
 // A thread stays with its values of its block and goes down the rows, kRowsTurn at a time, so that what places them in a
 // row is worked out once and several rows' loads are on their way together.
 constexpr unsigned kRowsTurn = 4;
@@ -151,6 +151,8 @@ struct RowPlace {
     unsigned head, b, l;  // KV head, block of the head, lane of the block
     bool is_v, real;
     size_t in_row;        // of the thread's values, in floats
+    uint8_t *head0;       // its KV head's first tile of page 0
+    unsigned word, scale; // of token 0 in a tile: byte offsets of word l % 4 and of the scale
 };
 __device__ __forceinline__ RowPlace row_place(const Kv4RowsArgs &a) {
     const unsigned nb = a.c.dim / 32, half = a.c.n_kv * nb, i = blockIdx.x * 256 + threadIdx.x, blk = i / 8;
@@ -162,7 +164,34 @@ __device__ __forceinline__ RowPlace row_place(const Kv4RowsArgs &a) {
     p.head = hb / nb;
     p.b = hb % nb;
     p.in_row = size_t(hb) * 32 + p.l * 4;
+    p.head0 = a.c.base + size_t(p.head) * (a.c.page / kTileTokens) * kv4_tile_bytes(a.c.dim);
+    p.word = p.is_v ? kv4_v_word(nb, 0, p.b, p.l % 4) : kv4_k_word(nb, 0, p.b, p.l % 4);
+    p.scale = p.is_v ? kv4_v_scale(nb, 0, p.b) : kv4_k_scale(nb, 0, p.b);
     return p;
+}
+
+// Where the turn's rows lie: lane i works it out for row i, with the divisions, and the warp asks it.
+struct Spots {
+    unsigned long long tile;  // of KV head 0, bytes from the pool's start
+    unsigned t;               // its token there; kTileTokens: no slot
+    __device__ __forceinline__ Spots(const Kv4RowsArgs &a, unsigned row0) : tile(0), t(kTileTokens) {
+        const unsigned i = threadIdx.x & 31, slot = i < kRowsTurn && row0 + i < a.n ? a.slots[row0 + i] : kNoSlot;
+        if (slot == kNoSlot) return;
+        const unsigned page = slot / a.c.page, at = slot - page * a.c.page, tiles = a.c.page / kTileTokens;
+        if (page >= a.c.n_pages) {
+            tell(a.status, kServeSlot);
+            return;
+        }
+        tile = ((unsigned long long)page * a.c.n_kv * tiles + at / kTileTokens) * kv4_tile_bytes(a.c.dim);
+        t = at % kTileTokens;
+    }
+    __device__ __forceinline__ unsigned token(unsigned i) const { return __shfl_sync(~0u, t, i); }
+    __device__ __forceinline__ unsigned long long at(unsigned i) const { return __shfl_sync(~0u, tile, i); }
+};
+// token t's word and scale behind token 0's
+__device__ __forceinline__ unsigned word_of(const RowPlace &p, unsigned nb, unsigned t) {
+    const unsigned row = kv4_plane_blocks(nb, p.b / 4) * 4;
+    return p.word + row * (p.is_v ? (t / 8 * 2 + t % 2) * 16 + t / 2 % 4 : t * 4);
 }
 
 template <bool kWide>  // rows on 16 bytes
@@ -175,11 +204,9 @@ __global__ void __launch_bounds__(256) kv4_store_kernel(const Kv4RowsArgs a) {
     const size_t stride = p.is_v ? a.v_stride : a.k_stride;
     for (unsigned row0 = blockIdx.y * kRowsTurn; row0 < a.n; row0 += gridDim.y * kRowsTurn) {
         float x[kRowsTurn][4];
-        unsigned slots[kRowsTurn];
 #pragma unroll
         for (unsigned i = 0; i < kRowsTurn; ++i) {
             const bool in = p.real && row0 + i < a.n;
-            slots[i] = in ? a.slots[row0 + i] : kNoSlot;
             const float *src = from + (row0 + i) * stride;
             if (kWide && in) {
                 const float4 v = __ldcs(reinterpret_cast<const float4 *>(src));
@@ -188,6 +215,7 @@ __global__ void __launch_bounds__(256) kv4_store_kernel(const Kv4RowsArgs a) {
                 for (unsigned e = 0; e < 4; ++e) x[i][e] = in ? src[e] : 0.0f;
             }
         }
+        const Spots spots(a, row0);  // while the values come
 #pragma unroll
         for (unsigned i = 0; i < kRowsTurn; ++i) {
             float amax = fmaxf(fmaxf(fabsf(x[i][0]), fabsf(x[i][1])), fmaxf(fabsf(x[i][2]), fabsf(x[i][3])));
@@ -207,18 +235,13 @@ __global__ void __launch_bounds__(256) kv4_store_kernel(const Kv4RowsArgs a) {
                 code[e] = __float_as_uint(__fadd_rz(fminf(fmaxf(fadd(fmul(x[i][e], inv), 8.5f), 0.0f), 15.0f), 0x1p23f));
             const uint32_t half = __byte_perm(__byte_perm(code[0], code[1], 0x0040), __byte_perm(code[2], code[3], 0x0040), 0x5410);
             const uint32_t high = __shfl_down_sync(~0u, half, 4);
-            const unsigned slot = slots[i];
-            if (slot == kNoSlot) continue;
-            if (slot / a.c.page >= a.c.n_pages) {
-                tell(a.status, kServeSlot);
-                continue;
-            }
-            uint8_t *tile = tile_of(a.c, slot, p.head);
-            const unsigned t = slot % a.c.page % kTileTokens;
+            const unsigned tok = spots.token(i);
+            uint8_t *tile = p.head0 + spots.at(i);
+            if (tok == kTileTokens || !p.real) continue;
             if (p.l < 4)
-                *reinterpret_cast<uint32_t *>(tile + (p.is_v ? kv4_v_word(nb, t, p.b, p.l) : kv4_k_word(nb, t, p.b, p.l))) = half | high << 4;
+                *reinterpret_cast<uint32_t *>(tile + word_of(p, nb, tok)) = half | high << 4;
             else if (p.l == 4)
-                *reinterpret_cast<uint16_t *>(tile + (p.is_v ? kv4_v_scale(nb, t, p.b) : kv4_k_scale(nb, t, p.b))) =
+                *reinterpret_cast<uint16_t *>(tile + p.scale + tok * nb * 2) =
                     bad ? uint16_t(0x7e00) : float_to_half_bits(d);
         }
     }
@@ -229,35 +252,31 @@ __global__ void __launch_bounds__(256) kv4_load_kernel(const Kv4RowsArgs a) {
     pdl_wait();
     pdl_launch_dependents();
     const RowPlace p = row_place(a);
-    if (!p.real) return;
-    const unsigned nb = a.c.dim / 32, w = p.l & 3;
+    const unsigned nb = a.c.dim / 32;
     float *to = (p.is_v ? a.v : a.k) + p.in_row;
     const size_t stride = p.is_v ? a.v_stride : a.k_stride;
     for (unsigned row0 = blockIdx.y * kRowsTurn; row0 < a.n; row0 += gridDim.y * kRowsTurn) {
-        unsigned slots[kRowsTurn];
         uint32_t word[kRowsTurn];
         uint16_t scale[kRowsTurn];
-#pragma unroll
-        for (unsigned i = 0; i < kRowsTurn; ++i) slots[i] = row0 + i < a.n ? a.slots[row0 + i] : kNoSlot;
+        bool some[kRowsTurn];
+        const Spots spots(a, row0);
 #pragma unroll
         for (unsigned i = 0; i < kRowsTurn; ++i) {
-            if (slots[i] != kNoSlot && slots[i] / a.c.page >= a.c.n_pages) {
-                tell(a.status, kServeSlot);
-                slots[i] = kNoSlot;
-            }
-            if (slots[i] == kNoSlot) continue;
-            const uint8_t *tile = tile_of(a.c, slots[i], p.head);
-            const unsigned t = slots[i] % a.c.page % kTileTokens;
-            word[i] = *reinterpret_cast<const uint32_t *>(tile + (p.is_v ? kv4_v_word(nb, t, p.b, w) : kv4_k_word(nb, t, p.b, w)));
-            scale[i] = *reinterpret_cast<const uint16_t *>(tile + (p.is_v ? kv4_v_scale(nb, t, p.b) : kv4_k_scale(nb, t, p.b)));
+            const unsigned tok = spots.token(i);
+            const uint8_t *tile = p.head0 + spots.at(i);
+            some[i] = tok != kTileTokens && p.real;
+            if (!some[i]) continue;
+            word[i] = *reinterpret_cast<const uint32_t *>(tile + word_of(p, nb, tok));
+            scale[i] = *reinterpret_cast<const uint16_t *>(tile + p.scale + tok * nb * 2);
         }
 #pragma unroll
         for (unsigned i = 0; i < kRowsTurn; ++i) {
-            if (slots[i] == kNoSlot) continue;
+            if (!some[i]) continue;
             const float d = half_bits_to_float(scale[i]);
             float x[4];
 #pragma unroll
-            for (unsigned e = 0; e < 4; ++e) x[e] = fmul(float(int(word[i] >> (8 * e + (p.l & 4)) & 15) - 8), d);
+            for (unsigned e = 0; e < 4; ++e)   // 2^23 + code, less 2^23 + 8
+                x[e] = fmul(__uint_as_float((word[i] >> (8 * e + (p.l & 4)) & 15) | 0x4b000000u) - 8388616.0f, d);
             float *dst = to + (row0 + i) * stride;
             if (kWide) __stcs(reinterpret_cast<float4 *>(dst), make_float4(x[0], x[1], x[2], x[3]));
             else
