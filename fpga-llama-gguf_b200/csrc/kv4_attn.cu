@@ -191,14 +191,11 @@ __device__ __forceinline__ float exp2_fast(float x) {
 __device__ __forceinline__ uint32_t h2(half2 x) { return *reinterpret_cast<uint32_t *>(&x); }
 __device__ __forceinline__ half2 as_h2(uint32_t x) { return *reinterpret_cast<half2 *>(&x); }
 
-// Two nibbles of a word, bits 0..3 and 16..19 (low) or 4..7 and 20..23 (high), as FP16.
-// K: left as they are they read c 2^-24 (16 c 2^-24), and the 8 that a code stands above its value comes off in the sum.
-__device__ __forceinline__ uint32_t low_raw(uint32_t x) { return x & 0x000f000fu; }
-__device__ __forceinline__ uint32_t high_raw(uint32_t x) { return x & 0x00f000f0u; }
-
-// V (whose sums run over many tokens, where that 8 would swamp them): put into the mantissa of 1024 they read 1024 + c
-// (1024 + 16 c); less 1032 (1152) that is c - 8 (16 (c - 8)), exactly. (A product of its own that takes the 8 off, with raw
-// codes beside it, measured the same with one set of rows and more with several.)
+// Two nibbles of a word, bits 0..3 and 16..19 (low) or 4..7 and 20..23 (high), as FP16: put into the mantissa of 1024 they
+// read 1024 + c (1024 + 16 c); less 1032 (1152) that is c - 8 (16 (c - 8)), exactly. The subtractions run at half the
+// issue rate, 16 a block of a tile. Raw codes (c 2^-24, as they are) with the 8 taken off a block's sum of K, or by a
+// product of its own for V, saved 3% at one set of rows and nothing at several, but the sums they swamp cost accuracy: 513
+// keys of heads of 256 came out off by 1.3 10^-6 and not 4 10^-7, as FP32 arithmetic is.
 __device__ __forceinline__ uint32_t low_codes(uint32_t x) {
     uint32_t y;
     asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;" : "=r"(y) : "r"(x));
@@ -300,7 +297,7 @@ __global__ void __launch_bounds__(kThreads, Shape<NB, NT>::kCtas) kv4_attn_kerne
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint64_t bars[kWarps][S::kSlots];
     __shared__ float m_of[kWarps][S::kRows], l_of[kWarps][S::kRows];
-    __shared__ float start_of[S::kRows][NB], scale_of[S::kRows];
+    __shared__ float scale_of[S::kRows];
     auto *before = reinterpret_cast<unsigned *>(smem + S::kSmem);
     const unsigned tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const unsigned per = a.n_head / a.c.n_kv, tiles_per_page = a.c.page / kTileTokens;
@@ -452,7 +449,7 @@ __global__ void __launch_bounds__(kThreads, Shape<NB, NT>::kCtas) kv4_attn_kerne
     }
     while (more) {
         // The queries as B operands, in the order in which a block's words hold the dims: column g is the upper (g even) or
-        // lower part of row g / 2. With them -8 sum q over each block, for the 8 that K's codes stand too high.
+        // lower part of row g / 2.
         const unsigned all = pc.all, row0 = pc.row0, mine = pc.mine;
         const int base = pc.base;
 #pragma unroll
@@ -464,7 +461,7 @@ __global__ void __launch_bounds__(kThreads, Shape<NB, NT>::kCtas) kv4_attn_kerne
             int ex = int(__float_as_uint(big) >> 23) - 127 - 10;  // x / 2^ex is below 2^11
             ex = ex < -110 ? -110 : ex > 100 ? 100 : ex;
             const float down = __uint_as_float(unsigned(127 - ex) << 23);
-            if (lane == 0) scale_of[m * 4 + warp] = a.scale * kLog2e * __uint_as_float(unsigned(127 + 24 + ex) << 23);  // (K's codes come times 2^-24)
+            if (lane == 0) scale_of[m * 4 + warp] = a.scale * kLog2e * __uint_as_float(unsigned(127 + ex) << 23);
 #pragma unroll
             for (int i = 0; i < kQuads; ++i) {
                 const unsigned quad = lane + 32 * i, set = quad / 4;
@@ -473,24 +470,16 @@ __global__ void __launch_bounds__(kThreads, Shape<NB, NT>::kCtas) kv4_attn_kerne
                 uint32_t h0, l0, h1, l1;
                 split2(x[m][i].x * f, x[m][i].z * f, h0, l0);
                 split2(x[m][i].y * f, x[m][i].w * f, h1, l1);
-                const float2 s0 = __half22float2(as_h2(h0)), s1 = __half22float2(as_h2(l0)), s2 = __half22float2(as_h2(h1)),
-                             s3 = __half22float2(as_h2(l1));
-                float sum_q = (high ? 16.0f : 1.0f) * (((s0.x + s0.y) + (s2.x + s2.y)) + ((s1.x + s1.y) + (s3.x + s3.y)) * (1.0f / 2048));
-                sum_q += __shfl_xor_sync(~0u, sum_q, 1);
-                sum_q += __shfl_xor_sync(~0u, sum_q, 2);
-                sum_q += __shfl_xor_sync(~0u, sum_q, 4);
                 if (quad < NB * 8) {
                     uint8_t *to = smem + ((m * NB * 2 + set) * 32 + warp * 8 + quad % 4) * 8;
                     *reinterpret_cast<uint2 *>(to) = make_uint2(h0, h1);
                     *reinterpret_cast<uint2 *>(to + 32) = make_uint2(l0, l1);
-                    if (quad % 8 == 0) start_of[m * 4 + warp][quad / 8] = -0x1p-21f * sum_q;
                 }
             }
         }
         __syncthreads();
         uint32_t qb[S::kQInRegs ? NT : 1][S::kQInRegs ? NB * 2 : 1][2];
-        float start[NT][NB];    // of row t
-        float scale[NT];
+        float scale[NT];        // of row t
         int pos[NT], low[NT];   // the keys row t sees: [low, pos]
         int wpos[NT], wlow[NT]; // and row g / 2
         auto sees = [&](unsigned row, int &lo, int &hi) {
@@ -503,8 +492,6 @@ __global__ void __launch_bounds__(kThreads, Shape<NB, NT>::kCtas) kv4_attn_kerne
             sees(row0 + m * 4 + t, low[m], pos[m]);
             sees(row0 + m * 4 + g / 2, wlow[m], wpos[m]);
             scale[m] = scale_of[m * 4 + t];
-#pragma unroll
-            for (int b = 0; b < NB; ++b) start[m][b] = start_of[m * 4 + t][b];
             if constexpr (S::kQInRegs) {
 #pragma unroll
                 for (int i = 0; i < NB * 2; ++i) {
@@ -557,8 +544,8 @@ __global__ void __launch_bounds__(kThreads, Shape<NB, NT>::kCtas) kv4_attn_kerne
                         if (b >= nbp) break;
                         const int bb = 4 * p + b;
                         const uint32_t w8[2] = {w[0][b] >> 8, w[1][b] >> 8};
-                        const uint32_t lo[4] = {low_raw(w[0][b]), low_raw(w[1][b]), low_raw(w8[0]), low_raw(w8[1])};
-                        const uint32_t hi[4] = {high_raw(w[0][b]), high_raw(w[1][b]), high_raw(w8[0]), high_raw(w8[1])};
+                        const uint32_t lo[4] = {low_codes(w[0][b]), low_codes(w[1][b]), low_codes(w8[0]), low_codes(w8[1])};
+                        const uint32_t hi[4] = {high_codes(w[0][b]), high_codes(w[1][b]), high_codes(w8[0]), high_codes(w8[1])};
                         const float d0 = half_at(ds[0], bb), d1 = half_at(ds[1], bb);
 #pragma unroll
                         for (int m = 0; m < NT; ++m) {
@@ -573,8 +560,8 @@ __global__ void __launch_bounds__(kThreads, Shape<NB, NT>::kCtas) kv4_attn_kerne
                             }
                             mma16816(e, lo, q0.x, q0.y, kZero);
                             mma16816(c, hi, q1.x, q1.y, e);
-                            s[m][0] += d0 * ((c[0] + start[m][bb]) + c[1] * (1.0f / 2048));
-                            s[m][1] += d1 * ((c[2] + start[m][bb]) + c[3] * (1.0f / 2048));
+                            s[m][0] += d0 * (c[0] + c[1] * (1.0f / 2048));
+                            s[m][1] += d1 * (c[2] + c[3] * (1.0f / 2048));
                         }
                     }
                 }
