@@ -30,6 +30,10 @@ namespace b200q {
 namespace {
 
 constexpr unsigned kRows = 128, kKeys = 64, kWork = 256, kThreads = kWork + 32;  // 8 warps, and one that issues products and copies
+// Steps whose products tensor memory adds up before O goes over to y in FP32. Its sums drop what is below their last bit, a
+// part in 10^8 on average and 12 times a step: with 32 steps O comes out 2 parts in 10^6 too small at most, and the way to
+// y (16,000 cycles of 6500 a step) takes less than a tenth of the time.
+constexpr unsigned kFold = 32;
 constexpr unsigned kBadMax = 96;  // values that are not numbers, remembered by (key, block)
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -72,8 +76,9 @@ struct Prompt {
     static constexpr int D = NB * 32, kTile = NB * 576;
     static constexpr int kQ = kRows * D * 2, kPart = kKeys * D * 2;
     static constexpr int kRaw = kQ + 4 * kPart, kSmem = kRaw + 4 * kTile;
-    // columns of tensor memory: O, S (qh kh + ql kh, then qh kl; P takes the place of the former, 32 keys' upper and lower
-    // parts by 16 columns), ql
+    // columns of tensor memory: O, S (qh kh, then qh kl + ql kh: the sums in tensor memory drop what is below their last bit, so
+    // that the small products go to a sum of their own; P takes the place of the former, 32 keys' upper and lower parts by
+    // 16 columns), ql
     static constexpr unsigned kS = D, kQl = D + 128, kNeed = D + 128 + D / 2;
     static constexpr unsigned kCols = kNeed <= 256 ? 256 : 512;
     static_assert(kNeed <= 512 && kSmem <= 216 * 1024);
@@ -190,7 +195,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnAr
                 for (unsigned k = 0; k < D / 16; ++k) {
                     const uint64_t kk = tm_operand(kh_at + k * 256, 128, D * 16);
                     tm_mma(tm + S::kS, tm_operand(q_at + k * 256, 128, D * 16), kk, tm_f16(2 * kKeys, false), k != 0);
-                    tm_mma_t(tm + S::kS, tm + S::kQl + k * 8, kk, tm_f16(kKeys, false), true);
+                    tm_mma_t(tm + S::kS + kKeys, tm + S::kQl + k * 8, kk, tm_f16(kKeys, false), true);
                 }
                 tm_commit(&bar_s);
             }
@@ -204,7 +209,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnAr
                 for (unsigned k = 0; k < kKeys / 16; ++k) {
                     const uint64_t v = tm_operand(vh_at + k * (D * 32), D * 16, 128);
                     const uint32_t p = tm + S::kS + k / 2 * 32 + k % 2 * 8;
-                    tm_mma_t(tm, p, v, tm_f16(D, true), j || k);
+                    tm_mma_t(tm, p, v, tm_f16(D, true), j % kFold || k);
                     tm_mma_t(tm, p, tm_operand(vl_at + k * (D * 32), D * 16, 128), tm_f16(D, true), true);
                     tm_mma_t(tm, p + 16, v, tm_f16(D, true), true);
                 }
@@ -349,6 +354,33 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnAr
     if (!fail) unpack(0, false, kh, kl);
     hand_over(&bar_k);
     float top = -INFINITY, sum = 0.0f;
+    float y_factor = 0.0f;  // of what lies in y (0: nothing yet)
+    const bool wide_y = ((reinterpret_cast<uintptr_t>(a.y) | a.y_stride * 4) & 15) == 0;
+    // O and what lies in y, times f: of this thread's row, its half of the dims, 16 at a time
+    auto fold = [&](float f, unsigned nan_blocks, bool none) {
+        for (unsigned c = half_ * (D / 2); c < (half_ + 1) * (D / 2); c += 16) {
+            uint32_t o[16];
+            tm_load16(tm_lane + c, o);
+            if (!real) continue;
+            const bool bad_block = nan_blocks >> c / 32 & 1;
+#pragma unroll
+            for (unsigned e = 0; e < 16; e += 4) {
+                float4 v = make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]), __uint_as_float(o[e + 2]), __uint_as_float(o[e + 3]));
+                float *to = y + c + e;
+                if (y_factor != 0.0f) {
+                    float4 was;
+                    if (wide_y) was = *reinterpret_cast<const float4 *>(to);
+                    else was = make_float4(to[0], to[1], to[2], to[3]);
+                    v.x += was.x * y_factor, v.y += was.y * y_factor, v.z += was.z * y_factor, v.w += was.w * y_factor;
+                }
+                v.x *= f, v.y *= f, v.z *= f, v.w *= f;
+                if (none) v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (bad_block) v.x = v.y = v.z = v.w = __uint_as_float(0x7fc00000u);
+                if (wide_y) *reinterpret_cast<float4 *>(to) = v;
+                else to[0] = v.x, to[1] = v.y, to[2] = v.z, to[3] = v.w;
+            }
+        }
+    };
     unsigned j = 0;
     for (; j < steps; ++j) {
         if (j && !fail) fail = !mbar_wait(&bar_o, (j - 1) & 1);  // V is free
@@ -392,11 +424,17 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnAr
         row_top[half_][row] = mx;
         work_sync();
         mx = fmaxf(mx, row_top[half_ ^ 1][row]);
+        const bool fresh = j % kFold == 0;  // O begins again with this step
+        if (fresh && j) {
+            fold(1.0f, 0, false);
+            y_factor = 1.0f;
+        }
         if (__any_sync(~0u, mx > top)) {  // a higher maximum: 4 above the score, so that it moves seldom
             const float nt = mx > top ? mx + 4.0f : top, f = top == nt ? 1.0f : exp2_fast(top - nt);
             sum *= f;
+            y_factor *= f;
             top = nt;
-            if (j) {
+            if (!fresh) {
                 for (unsigned c = half_ * (D / 2); c < (half_ + 1) * (D / 2); c += 16) {
                     uint32_t o[16];
                     tm_load16(tm_lane + c, o);
@@ -452,23 +490,18 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnAr
         const unsigned nb = n_bad < kBadMax ? n_bad : kBadMax;
         for (unsigned i = 0; i < nb; ++i)
             if (int(bad[i] / 8) >= low && int(bad[i] / 8) <= pos) nan_blocks |= 1u << bad[i] % 8;
-        if (n_bad > kBadMax && pos >= 0) nan_blocks = ~0u;  // more than are remembered
-        const bool wide = ((reinterpret_cast<uintptr_t>(a.y) | a.y_stride * 4) & 15) == 0;
-        for (unsigned c = half_ * (D / 2); c < (half_ + 1) * (D / 2); c += 16) {
-            uint32_t o[16];
-            tm_load16(tm_lane + c, o);
-            if (!real) continue;
-            float v[16];
-#pragma unroll
-            for (unsigned e = 0; e < 16; ++e) v[e] = nan_blocks >> c / 32 & 1 ? __uint_as_float(0x7fc00000u) : sum == 0.0f ? 0.0f : __uint_as_float(o[e]) * f;
-            if (wide) {
-#pragma unroll
-                for (unsigned e = 0; e < 16; e += 4) *reinterpret_cast<float4 *>(y + c + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-            } else {
-#pragma unroll
-                for (unsigned e = 0; e < 16; ++e) y[c + e] = v[e];
+        if (n_bad > kBadMax) {  // more than are remembered: the scales again, those of the keys this row sees
+            const unsigned tiles_per_page = a.c.page / kTileTokens;
+            for (int k = low; k <= pos; ++k) {
+                const unsigned tile = unsigned(k) / kTileTokens, page = a.table[size_t(req) * a.stride + tile / tiles_per_page];
+                if (page >= a.c.n_pages) continue;
+                const auto *d = reinterpret_cast<const half *>(a.c.base + ((size_t(page) * a.c.n_kv + head) * tiles_per_page + tile % tiles_per_page) * S::kTile +
+                                                               NB * 544 + unsigned(k) % kTileTokens * NB * 2);
+                for (unsigned b = 0; b < NB; ++b)
+                    if (!(fabsf(__half2float(d[b])) <= 65504.0f)) nan_blocks |= 1u << b;
             }
         }
+        fold(f, nan_blocks, sum == 0.0f);
     }
     }
     tm_fence_before();

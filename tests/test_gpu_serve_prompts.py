@@ -165,3 +165,26 @@ def test_units_of_nine_to_sixteen_rows(b2, dim, group, new):
     b = Batch(b2, rng(309, dim, group), [(new, 130), (1, 1), (new, new), (1, 65), (new, 1), (0, 5), (new, 333)], 2, group, dim, 32)
     b.check(b.run(pad=1))
     b.check(b.run(window=50), 50)
+
+
+@pytest.mark.parametrize("dim,y_pad,window", [(32, 0, 0), (64, 1, 0), (32, 0, 2500)])
+def test_prompts_on_long_caches(b2, dim, y_pad, window):
+    # Sums in tensor memory drop what is below their last bit: over 9000 keys without a break (12 products of 16 keys each a
+    # step of 64, half of 2^-23 lost each time) O would come out 2^-24 * 12 * 141 / 2 > 2^-15 too small, four times the bound
+    b = Batch(b2, rng(310, dim), [(60, 9000), (30, 4097), (1, 9100), (20, 2048), (18, 2049)], 1, 64, dim, 64)
+    b.check(b.run(window, y_pad=y_pad), window)
+
+
+@pytest.mark.parametrize("dim", [64, 256])
+def test_prompts_before_many_values_that_are_no_numbers(b2, dim):
+    n, at = 400, 150  # V of every token from `at` on is infinite in block 1 of KV head 0: the rows before it do not see it
+    b = Batch(b2, rng(311, dim), [(n, n), (1, 90)], 2, 8, dim, 16)
+    tok = np.arange(at, n)
+    v = np.ones((len(tok), 2 * dim), np.float32)
+    v[:, 40] = np.inf
+    b.p.fill(b.table[0][tok // 16] * 16 + tok % 16, np.zeros((len(tok), 2 * dim), np.float32), v)
+    got = b.run()
+    assert np.isnan(got[at:n, :8, 32:64]).all()
+    rest = got.copy()
+    rest[at:n, :8, 32:64] = 0
+    assert np.isfinite(rest).all()
