@@ -448,8 +448,9 @@ B200Q_API int b200q_kv4_load(int device, const b200q_kv4_pool *pool, const uint3
  *   y = softmax(scale q K^T) V, with FP32 inputs, sums and outputs.
  * q: rows q_stride and heads q_head_stride floats apart; y: rows y_stride apart, heads packed (0: packed). max_q and
  * max_kv bound the requests' new tokens and kv_len, and shape the launch; a request beyond them is left out and
- * reported, and so is every request from the first on whose row starts run backwards. n_req <= 4096. workspace: b200q_kv4_attn_workspace bytes for the same shape, 16-byte aligned; nothing in it has to be kept or cleared
- * between calls. */
+ * reported, and so is every request from the first on whose row starts run backwards. n_req <= 4096. workspace:
+ * b200q_kv4_attn_workspace bytes for the same shape, 16-byte aligned; nothing in it has to be kept or cleared between
+ * calls. y is written in parts, and read again, while a call runs. */
 B200Q_API size_t b200q_kv4_attn_workspace(int device, const b200q_kv4_pool *pool, unsigned n_rows, unsigned n_head,
                                           unsigned n_req, unsigned max_q, unsigned max_kv);
 B200Q_API int b200q_kv4_attn(int device, const b200q_kv4_pool *pool, const float *q, float *y, unsigned n_rows,
