@@ -916,13 +916,14 @@ AttnPlan plan_of(const Kv4AttnArgs &a, unsigned sms) {
     // the most units there can be, and the line's length
     const unsigned long long q = a.max_q < a.n_rows ? a.max_q : a.n_rows, rows = (unsigned long long)a.n_rows * per;
     unsigned long long groups = rows / p.rows + (a.n_req < a.n_rows ? a.n_req : a.n_rows);
-    const unsigned long long each = (q * per + p.rows - 1) / p.rows * a.n_req;
+    const unsigned long long most_of = q * per < p.most_rows ? q * per : p.most_rows;  // of a request's rows
+    const unsigned long long each = (most_of + p.rows - 1) / p.rows * a.n_req;
     if (each < groups) groups = each;
     const unsigned long long units = groups * a.c.n_kv, line = units * ((a.max_kv + kTileTokens - 1) / kTileTokens + kUnitCost);
     if ((line + kWarps - 1) / kWarps < p.grid) p.grid = unsigned((line + kWarps - 1) / kWarps);
     const unsigned long long turns = (line + (unsigned long long)p.grid * kMaxRange - 1) / ((unsigned long long)p.grid * kMaxRange);
     p.max_ranges = unsigned(turns * p.grid);
-    p.fits = line < 0x80000000ull;
+    p.fits = line < 0x80000000ull && rows < 0x80000000ull && (rows / 128 + a.n_req + 1) * a.c.n_kv < 0x80000000ull;
     return p;
 }
 

@@ -108,17 +108,52 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnAr
     __shared__ __align__(16) float k_scale[kKeys], v_log[kKeys], v_inv[kKeys];  // read four at a time
     __shared__ float row_top[2][kRows];
     __shared__ unsigned present, n_bad, bad[kBadMax];
+    __shared__ unsigned whole_of[kThreads / 32], count_of[kThreads / 32], found_req, found_tile;
     const unsigned tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const unsigned per = a.n_head / a.c.n_kv, head = blockIdx.x % a.c.n_kv, req = blockIdx.x / a.c.n_kv, row0 = (gridDim.y - 1 - blockIdx.y) * kRows;
+    const unsigned per = a.n_head / a.c.n_kv, head = blockIdx.x % a.c.n_kv;
     pdl_wait();
     pdl_launch_dependents();
 
-    // the request (left out, as kv4_attn.cu says, when its rows or lengths lie outside the bounds)
-    bool broken = false;
-    for (unsigned i = tid; i <= req; i += kThreads) broken = broken || a.q_start[i] > a.q_start[i + 1];
-    if (__syncthreads_or(broken)) return;
+    // The CTA's tile: those of all requests with enough rows lie in one line, the last (which see the most keys) come first. A
+    // thread counts some requests; one is left out as kv4_attn.cu says, when its rows or lengths lie outside the bounds.
+    const unsigned each = (a.n_req + kThreads - 1) / kThreads, r0 = tid * each < a.n_req ? tid * each : a.n_req, r1 = r0 + each < a.n_req ? r0 + each : a.n_req;
+    unsigned whole = a.n_req;  // the requests before the first whose rows run backwards
+    for (unsigned r = r1; r > r0; --r)
+        if (a.q_start[r - 1] > a.q_start[r]) whole = r - 1;
+    whole = __reduce_min_sync(~0u, whole);
+    if (lane == 0) whole_of[warp] = whole;
+    __syncthreads();
+    for (unsigned w = 0; w < kThreads / 32; ++w) whole = min(whole, whole_of[w]);
+    auto tiles_of = [&](unsigned r) {
+        const unsigned s = a.q_start[r], e = a.q_start[r + 1];
+        if (r >= whole || e > a.n_rows || e - s > a.max_q || a.kv_len[r] > a.max_kv || (e - s) * per < least_rows) return 0u;
+        return ((e - s) * per + kRows - 1) / kRows;
+    };
+    unsigned count = 0;
+    for (unsigned r = r0; r < r1; ++r) count += tiles_of(r);
+    unsigned upto = count;
+    for (unsigned o = 1; o < 32; o <<= 1) {
+        const unsigned x = __shfl_up_sync(~0u, upto, o);
+        if (lane >= o) upto += x;
+    }
+    if (lane == 31) count_of[warp] = upto;
+    __syncthreads();
+    unsigned total = 0;
+    for (unsigned w = 0; w < kThreads / 32; ++w) {
+        if (w < warp) upto += count_of[w];
+        total += count_of[w];
+    }
+    const unsigned turn = blockIdx.x / a.c.n_kv, mine = total - 1 - turn;
+    if (turn >= total) return;
+    if (mine < upto && mine >= upto - count) {
+        unsigned at = upto - count, r = r0;
+        while (at + tiles_of(r) <= mine) at += tiles_of(r++);
+        found_req = r;
+        found_tile = mine - at;
+    }
+    __syncthreads();
+    const unsigned req = found_req, row0 = found_tile * kRows;
     const unsigned start = a.q_start[req], end = a.q_start[req + 1], len = a.kv_len[req], all = (end - start) * per;
-    if (end > a.n_rows || end - start > a.max_q || len > a.max_kv || all < least_rows || row0 >= all) return;
     const int base = int(len) - int(end - start);
     const unsigned last = row0 + kRows < all ? row0 + kRows - 1 : all - 1;
     const int hi = base + int(last / per), first_pos = base + int(row0 / per);
@@ -512,13 +547,18 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnAr
     }
 }
 
+// the most tiles that n_rows rows of requests of least_rows and more can make
+unsigned long long prompt_tiles(const Kv4AttnArgs &a, unsigned least_rows) {
+    const unsigned long long rows = (unsigned long long)a.n_rows * (a.n_head / a.c.n_kv), requests = rows / least_rows;
+    return rows / kRows + (requests < a.n_req ? requests : a.n_req) + 1;
+}
+
 template <int NB>
 cudaError_t launch_prompt(const Kv4AttnArgs &a, unsigned least_rows, cudaStream_t st) {
     using S = Prompt<NB>;
     const cudaError_t e = ensure_smem_attr(reinterpret_cast<const void *>(kv4_prompt_kernel<NB>), S::kSmem);
     if (e != cudaSuccess) return e;
-    const unsigned long long rows = (unsigned long long)(a.max_q < a.n_rows ? a.max_q : a.n_rows) * (a.n_head / a.c.n_kv);
-    return launch_pdl(a.pdl, kv4_prompt_kernel<NB>, dim3(a.c.n_kv * a.n_req, unsigned((rows + kRows - 1) / kRows)), dim3(kThreads), S::kSmem, st, a, least_rows);
+    return launch_pdl(a.pdl, kv4_prompt_kernel<NB>, dim3(unsigned(prompt_tiles(a, least_rows)) * a.c.n_kv), dim3(kThreads), S::kSmem, st, a, least_rows);
 }
 
 }  // namespace

@@ -188,3 +188,21 @@ def test_prompts_before_many_values_that_are_no_numbers(b2, dim):
     rest = got.copy()
     rest[at:n, :8, 32:64] = 0
     assert np.isfinite(rest).all()
+
+
+@pytest.mark.parametrize("n_req", [300, 600])
+def test_prompts_among_hundreds_of_single_tokens(b2, n_req):
+    # more requests than threads count one by one; the bound on new tokens far above what any request has
+    lengths = [(1, 1 + i % 70) for i in range(n_req)]
+    lengths[7], lengths[n_req // 2], lengths[-1] = (200, 260), (90, 90), (150, 151)
+    b = Batch(b2, rng(312, n_req), lengths, 2, 8, 32, 16)
+    b.check(b.run(pad=5, max_q=1 << 20))
+    assert u32(b.status)[0] == 0
+    got = b.run(q_start=np.concatenate([b.q_start[:n_req // 2 + 1], [0], b.q_start[n_req // 2 + 2:]]))  # the rows of one run backwards
+    assert u32(b.status)[0] & b2.SERVE_REQUEST
+    # those before it are served (where the line of tiles is cut has moved with its length, and the roundings with it)
+    k = n_req // 2
+    rows = int(b.q_start[k])
+    assert (got[rows:] == 7).all()
+    b.q_start, b.kv, b.q = b.q_start[:k + 1], b.kv[:k], b.q[:rows]
+    b.check(got[:rows])
