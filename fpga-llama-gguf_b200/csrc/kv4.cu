@@ -21,7 +21,7 @@ constexpr unsigned kMapRows = 4096;
 
 // rows j0 .. j0 + 3: each one's request is found once, by bisection, and then followed
 __device__ __forceinline__ void map_rows(const BlockMapArgs &a, unsigned j0) {
-    const unsigned rows = a.q_start[a.n_req];
+    const unsigned rows = a.q_start[a.n_req], most = 0xFFFFFFFFu / a.page;  // pages whose slots 32 bits count
     unsigned slot[4], pos[4];
     unsigned r = 0;
     if (j0 < rows) {
@@ -52,7 +52,8 @@ __device__ __forceinline__ void map_rows(const BlockMapArgs &a, unsigned j0) {
         pos[i] = unsigned(p);
         const unsigned b = pos[i] / a.page;
         if (b != block) page = a.table[size_t(r) * a.stride + b], block = b;
-        if (page != kNoSlot) slot[i] = page * a.page + (pos[i] - b * a.page);
+        if (page < most) slot[i] = page * a.page + (pos[i] - b * a.page);
+        else if (page != kNoSlot) tell(a.status, kServePage);
     }
     if (j0 + 4 <= a.n_rows && ((reinterpret_cast<uintptr_t>(a.slots) | reinterpret_cast<uintptr_t>(a.positions)) & 15) == 0) {
         *reinterpret_cast<uint4 *>(a.slots + j0) = make_uint4(slot[0], slot[1], slot[2], slot[3]);
@@ -103,11 +104,20 @@ __global__ void __launch_bounds__(1024) block_map_kernel(const BlockMapArgs a, b
         }
         if (r < a.n_req) {
             a.q_start[r] = unsigned(row0);
-            for (unsigned b = first; b < last; ++b) {
-                const unsigned long long f = cursor + need0 + (b - first);
-                a.table[size_t(r) * a.stride + b] = f < a.n_free ? a.free_pages[f] : kNoSlot;
-            }
             if (last > first && cursor + need0 + (last - first) > a.n_free) tell(a.status, kServeShort);
+        }
+        // a request's pages: a few by its thread, more by its warp
+        auto take = [&](unsigned req, unsigned b, unsigned from, unsigned long long at) {
+            const unsigned long long f = cursor + at + (b - from);
+            a.table[size_t(req) * a.stride + b] = f < a.n_free ? a.free_pages[f] : kNoSlot;
+        };
+        const bool few = last - first <= 8;
+        if (few)
+            for (unsigned b = first; b < last; ++b) take(r, b, first, need0);
+        for (unsigned many = __ballot_sync(~0u, !few); many; many &= many - 1) {
+            const unsigned of = __ffs(many) - 1, from = __shfl_sync(~0u, first, of), to = __shfl_sync(~0u, last, of);
+            const unsigned long long at = __shfl_sync(~0u, need0, of);
+            for (unsigned b = from + lane; b < to; b += 32) take(r - lane + of, b, from, at);
         }
         __syncthreads();
         if (tid == blockDim.x - 1) {

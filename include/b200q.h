@@ -422,7 +422,8 @@ B200Q_API size_t b200q_kv4_page_bytes(unsigned page_tokens, unsigned n_kv_head, 
  *   *cursor_in itself);
  *   row j of the step (j < n_rows, rows in request order): positions[j] and slots[j]; rows behind the last token get
  *   B200Q_NO_SLOT and position 0, so that a step padded to a fixed n_rows stores nothing for them.
- * Without a free page or a table entry left, a token's slot is B200Q_NO_SLOT (and kv_len stops at the table's end). */
+ * Without a free page or a table entry left, a token's slot is B200Q_NO_SLOT (and kv_len stops at the table's end); so it
+ * is where the page's slots would pass 32 bits, which is reported as B200Q_SERVE_PAGE. */
 B200Q_API int b200q_block_map(int device, unsigned n_req, const uint32_t *past, const uint32_t *fresh, uint32_t *table,
                               unsigned table_stride, unsigned page_tokens, const uint32_t *free_pages, unsigned n_free,
                               const uint32_t *cursor_in, uint32_t *cursor_out, uint32_t *kv_len, uint32_t *q_start,
