@@ -333,7 +333,8 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamSel
 
 // ---- beam_reorder ---------------------------------------------------------------------------------------------------
 // A thread owns one column (16, 4 or 1 bytes, by the rows' alignment) of a request's beams in one layer and reads every
-// beam's parent before it writes any, so that src and dst may be the same.
+// beam's parent before it writes any, so that src and dst may be the same. Bound by memory: 277 MB in 44.4 us, 6.2 TB/s, 95%
+// of the measured copy rate.
 template <typename T, int W>
 __global__ void __launch_bounds__(256) beam_reorder_kernel(const BeamReorderArgs a) {
     pdl_wait();

@@ -30,7 +30,10 @@ constexpr unsigned kMaxRange = 1024;     // a warp adds at most 256 tiles into i
 // the start of its copies. 64 requests of 5 to 8192 keys, three rows of 32 heads of 128 each: 87 us with 9, 74 with 12, 70
 // with 16, 74 with 24 (short requests pile up on a CTA with less, its long ones wait with more).
 constexpr unsigned kUnitCost = 16;
-// Requests with this many rows (token, head of a KV head's group) are the prompt kernel's when a call has work for it.
+// Requests with this many rows (token, head of a KV head's group) are the prompt kernel's when a call's rows and heads make
+// work enough for it. New tokens on 512 keys before them, 16 heads of 128 (of 256), us here / there: 128 tokens 32 / 46 (40 / 64),
+// 256 45 / 52 (68 / 71), 384 64 / 57 (101 / 79), 1024 204 / 87 (371 / 118); 32 requests of 16 tokens on 1000 keys, 32 heads
+// 104 / 100 (161 / 133), of 8 tokens (32 rows a request) 70 / 122 (98 / 164).
 constexpr unsigned kPromptRows = 64, kPromptWork = 6144;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -290,6 +293,12 @@ struct Shape {
 //
 // A warp takes every fourth tile of its CTA's chunk, with a running maximum, sum and output of its own; it fetches its
 // tiles itself (one bulk copy each), so that nothing in the loop waits for another warp.
+//
+// Instructions and their latencies bound it: the registers leave two to four warps a quarter SM. A tile of 16 keys takes a
+// quarter 300 cycles at 4 rows of heads of 32, 680 at 128, 1190 at 256 (4.6 KB: 820 at the copy rate), 1380 at 12 rows of 128.
+// One row of 16 heads of 256 on 131,000 keys: 47.8 us, 3.2 TB/s; 12 us of it lie before and behind the loop (the wait for
+// the kernel before, 2 us of schedule, 2 until the first tile is there, 5 for the merge). Tried without gain: two tiles'
+// products at a time, one tile's values beside the next one's scores, the next piece looked up before this one's tiles.
 template <int NB, int NT>
 __global__ void __launch_bounds__(kThreads, Shape<NB, NT>::kCtas) kv4_attn_kernel(const Kv4AttnArgs a, const AttnPlan plan) {
     using S = Shape<NB, NT>;
