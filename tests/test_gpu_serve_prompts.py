@@ -206,3 +206,13 @@ def test_prompts_among_hundreds_of_single_tokens(b2, n_req):
     assert (got[rows:] == 7).all()
     b.q_start, b.kv, b.q = b.q_start[:k + 1], b.kv[:k], b.q[:rows]
     b.check(got[:rows])
+
+
+@pytest.mark.parametrize("dim,group,prompt", [(32, 2, False), (256, 1, False), (64, 4, True)])
+def test_as_many_requests_as_a_call_takes(b2, dim, group, prompt):
+    lengths = [(1, 1 + i % 23) if i % 5 else (0, i % 30) for i in range(4096)]
+    if prompt:
+        lengths[2000], lengths[4095] = (70, 90), (33, 33)
+    b = Batch(b2, rng(313, dim), lengths, 1, group, dim, 16)
+    b.check(b.run(pad=1))
+    assert u32(b.status)[0] == 0
