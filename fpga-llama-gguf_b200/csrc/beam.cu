@@ -61,10 +61,10 @@ __device__ __forceinline__ unsigned reached_by(unsigned mine, unsigned n, unsign
 // the threads' own best give a bound that n_out of them reach; what is above it in the segment's chunks, some dozens each, is
 // collected and ranked by counting at the end. Should more come together, the n_out best so far are taken out first and the
 // worst of them is the bound from then on; should ties put more there than can be held, they are taken out one by one.
-// 16 requests of 8 beams over 151,936 logits, 16 each: 26 us, and 8 for the lists' merge behind it (the bytes alone: 12). A
+// 16 requests of 8 beams over 151,936 logits, 16 each: 26 us, and 7 for the lists' merge behind it (the bytes alone: 12). A
 // chunk takes a CTA 1.9 us (0.6 to issue the next one's copies, 0.2 maxima, 0.5 exponentials, 0.4 candidates and the barrier),
 // at which three CTAs an SM ask for all of the memory's rate; the first one (2.5 with its bound) and the end (1.5) do not. With
-// a list a chunk instead, each ranked by itself and five CTAs an SM, the whole call took 40 us (36 now), with chunks of
+// a list a chunk instead, each ranked by itself and five CTAs an SM, the whole call took 40 us (35 now), with chunks of
 // 4096 57.
 constexpr unsigned kFound = 512, kSelCtas = 3;  // CTAs on an SM, by shared memory
 static_assert(kSelPer == 32 && kFound / 2 > kMaxBeamOut);
@@ -233,6 +233,7 @@ struct Scored {
 };
 constexpr unsigned kHeads = kMaxVocab / kSelChunk / 32;  // lists a lane holds
 constexpr unsigned kListBytes = 64 * 1024;               // of lists in shared memory, at most
+constexpr unsigned kCounted = 128;                       // a beam's candidates that are ranked by counting
 
 __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamSelectArgs a, const unsigned long long *list, const float2 *stat,
                                                                    unsigned chunks, unsigned in_smem) {
@@ -268,27 +269,49 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamSel
         if (fabsf(m) < INFINITY && fabsf(score) < INFINITY) {
             const double log_s = log(s);
             __syncwarp();
-            unsigned long long head[kHeads];
-            unsigned at[kHeads];
+            auto put = [&](unsigned place, unsigned long long c) {
+                best[b * n + place] = Scored{double(score) + ((double(cand_logit(c)) - double(m)) - log_s), cand_token(c)};
+            };
+            if (in_smem && per_beam <= kCounted) {  // few: each one's place is the number of larger ones
+                unsigned long long c[kCounted / 32];
+                unsigned place[kCounted / 32];
 #pragma unroll
-            for (unsigned i = 0; i < kHeads; ++i) {
-                at[i] = 0;
-                head[i] = i * 32 + lane < chunks ? mine[(i * 32 + lane) * n] : 0;
-            }
-            for (; got < n; ++got) {
-                unsigned long long top = head[0];
-                unsigned which = 0;
+                for (unsigned i = 0; i < kCounted / 32; ++i) c[i] = i * 32 + lane < per_beam ? mine[i * 32 + lane] : 0, place[i] = 0;
+#pragma unroll 4
+                for (unsigned j = 0; j < per_beam; ++j) {
+                    const unsigned long long y = mine[j];
 #pragma unroll
-                for (unsigned i = 1; i < kHeads; ++i)
-                    if (head[i] > top) top = head[i], which = i;
-                const unsigned key = __reduce_max_sync(~0u, unsigned(top >> 32));
-                if (key == 0) break;
-                const unsigned low = __reduce_max_sync(~0u, unsigned(top >> 32) == key ? unsigned(top) : 0u);
-                if (unsigned(top >> 32) == key && unsigned(top) == low) {
-                    best[b * n + got] = Scored{double(score) + ((double(cand_logit(top)) - double(m)) - log_s), cand_token(top)};
+                    for (unsigned i = 0; i < kCounted / 32; ++i) place[i] += y > c[i];
+                }
 #pragma unroll
-                    for (unsigned i = 0; i < kHeads; ++i)
-                        if (i == which) head[i] = ++at[i] < n ? mine[(i * 32 + lane) * n + at[i]] : 0;
+                for (unsigned i = 0; i < kCounted / 32; ++i) {
+                    got += __popc(__ballot_sync(~0u, c[i] != 0));
+                    if (c[i] && place[i] < n) put(place[i], c[i]);
+                }
+                got = got < n ? got : n;
+            } else {
+                unsigned long long head[kHeads];
+                unsigned at[kHeads];
+#pragma unroll
+                for (unsigned i = 0; i < kHeads; ++i) {
+                    at[i] = 0;
+                    head[i] = i * 32 + lane < chunks ? mine[(i * 32 + lane) * n] : 0;
+                }
+                for (; got < n; ++got) {
+                    unsigned long long top = head[0];
+                    unsigned which = 0;
+#pragma unroll
+                    for (unsigned i = 1; i < kHeads; ++i)
+                        if (head[i] > top) top = head[i], which = i;
+                    const unsigned key = __reduce_max_sync(~0u, unsigned(top >> 32));
+                    if (key == 0) break;
+                    const unsigned low = __reduce_max_sync(~0u, unsigned(top >> 32) == key ? unsigned(top) : 0u);
+                    if (unsigned(top >> 32) == key && unsigned(top) == low) {
+                        put(got, top);
+#pragma unroll
+                        for (unsigned i = 0; i < kHeads; ++i)
+                            if (i == which) head[i] = ++at[i] < n ? mine[(i * 32 + lane) * n + at[i]] : 0;
+                    }
                 }
             }
         }
@@ -387,7 +410,8 @@ cudaError_t launch_beam_select(const BeamSelectArgs &a, unsigned sms, cudaStream
     constexpr int kRooms = 2 * kSelChunk * sizeof(float);
     cudaError_t e = ensure_smem_attr(reinterpret_cast<const void *>(kernel), kRooms);
     if (e != cudaSuccess) return e;
-    // Segments: as many as run at once, as far as rows and chunks go round.
+    // Segments: as many as run at once, as far as rows and chunks go round. (For two / three / four CTAs an SM 128 rows of 151,936
+    // took 35.9 / 35.7 / 37.1 us, 192 rows 50.6 / 44.3 / 48.3, 256 rows 51.3 / 51.3 / 60.9.)
     const unsigned fit = sms * kSelCtas / rows, segments = fit < 1 ? 1 : fit < chunks ? fit : chunks;
     e = launch_pdl(a.pdl, kernel, dim3(segments, rows), dim3(kSelThreads), segments == chunks ? kRooms / 2 : kRooms, st, a, list, stat, chunks);
     if (e != cudaSuccess) return e;

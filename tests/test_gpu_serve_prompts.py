@@ -210,7 +210,8 @@ def test_prompts_among_hundreds_of_single_tokens(b2, n_req):
 
 @pytest.mark.parametrize("dim,group,prompt", [(32, 2, False), (256, 1, False), (64, 4, True)])
 def test_as_many_requests_as_a_call_takes(b2, dim, group, prompt):
-    lengths = [(1, 1 + i % 23) if i % 5 else (0, i % 30) for i in range(4096)]
+    most = 5 if dim == 256 else 23  # keys (quantizing them on the host takes the time here)
+    lengths = [(1, 1 + i % most) if i % 5 else (0, i % most) for i in range(4096)]
     if prompt:
         lengths[2000], lengths[4095] = (70, 90), (33, 33)
     b = Batch(b2, rng(313, dim), lengths, 1, group, dim, 16)
