@@ -928,7 +928,9 @@ AttnPlan plan_of(const Kv4AttnArgs &a, unsigned sms) {
     const unsigned long long most_of = q * per < p.most_rows ? q * per : p.most_rows;  // of a request's rows
     const unsigned long long each = (most_of + p.rows - 1) / p.rows * a.n_req;
     if (each < groups) groups = each;
-    const unsigned long long units = groups * a.c.n_kv, line = units * ((a.max_kv + kTileTokens - 1) / kTileTokens + kUnitCost);
+    const unsigned long long units = groups * a.c.n_kv;
+    unsigned long long line = units * ((a.max_kv + kTileTokens - 1) / kTileTokens + kUnitCost);
+    if (line == 0) line = 1;  // (no rows: a workspace all the same, so that a room of 0 means a shape that is refused)
     if ((line + kWarps - 1) / kWarps < p.grid) p.grid = unsigned((line + kWarps - 1) / kWarps);
     const unsigned long long turns = (line + (unsigned long long)p.grid * kMaxRange - 1) / ((unsigned long long)p.grid * kMaxRange);
     p.max_ranges = unsigned(turns * p.grid);

@@ -1,0 +1,62 @@
+"""Sizes at the ends of what the calls and commands for several sequences take: steps without rows. No GPU needed, but for the
+tests marked so."""
+import subprocess
+import sys
+
+import pytest
+
+from conftest import ROOT, load_package
+
+b2 = load_package()
+
+
+def pool(dim=64, n_kv=2, page=16, n_pages=8):
+    return b2.Kv4Pool(4096, n_pages, page, n_kv, dim, 1, 0)
+
+
+ROOM_OF_NO_ROWS = """
+import sys
+sys.path.insert(0, "tests")
+from conftest import load_package
+b2 = load_package()
+for dim in range(32, 257, 32):
+    for n_head in (2, 4, 64):
+        for n_req, max_q, max_kv in ((1, 1, 512), (4096, 1, 1), (7, 1 << 24, 1 << 28), (1, 16, 300)):
+            h = b2.Kv4Pool(4096, 8, 16, 2, dim, 1, 0)
+            none, one = (b2.kv4_attn_workspace(0, h, rows, n_head, n_req, max_q, max_kv) for rows in (0, 1))
+            assert 0 < none <= one, (dim, n_head, n_req, none, one)
+"""
+
+
+def test_the_workspace_of_no_rows():
+    """In a process of its own: an integer division by zero would end this one."""
+    got = subprocess.run([sys.executable, "-c", ROOM_OF_NO_ROWS], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert got.returncode == 0, (got.returncode, got.stderr)
+
+
+def empty_attention(n_req=2):
+    return b2.kv4_attn_cmd(4, 1024, 4096, 0, 4, 64, 128, n_req, 0, 2, 64, 0.125, b2.kv4_geometry(2, 64, 16), 256, 8)
+
+
+def test_an_attention_of_no_rows_plans():
+    assert b2.plan(empty_attention())[0] == 0
+
+
+@pytest.mark.gpu
+def test_an_attention_of_no_rows_runs_in_lists_and_graphs():
+    import numpy as np
+    cl = b2.cmd_list(b2.add(16, 0, 16, 32), empty_attention(), b2.add(16, 0, 16, 48))
+    layer = b2.kv4_page_bytes(16, 2, 64) * 8
+    with b2.Context(device=0, weight_bytes=1 << 20, act_floats=8192, state_rows=8, kv_bytes=256 + layer) as ctx:
+        act = np.arange(8192, dtype=np.float32)
+        ctx.write(0, act)
+        want = act.copy()
+        want[32:48] = want[48:64] = act[:16] + act[16:32]
+        assert ctx.run(cl) == 0
+        assert np.array_equal(ctx.read(0, 8192), want)
+        ctx.write(0, act)
+        g = ctx.graph(cl)
+        g.launch()
+        ctx.synchronize()
+        assert np.array_equal(ctx.read(0, 8192), want)
+        g.close()
