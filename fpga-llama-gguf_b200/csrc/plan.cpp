@@ -181,13 +181,16 @@ const char *serve_check(const Ctx &C, const uint32_t (*w)[8]) {
         if (!select_shape_ok(a[1], a[2], a[3], a[7]) || (a[5] && a[5] < a[3]) || (b[3] | b[4] | b[5] | b[6] | b[7])) return "invalid BEAM_SELECT";
         break;
     case 22: {
-        const size_t n = size_t(a[1]) * a[2] * a[6], step = b[0] ? b[0] : n;
-        if (a[1] == 0 || a[1] > kMaxMapReq || a[2] == 0 || a[2] > kMaxBeams || a[6] == 0 || a[7] == 0 || a[7] > 65535 || step < n ||
+        if (a[1] == 0 || a[1] > kMaxMapReq || a[2] == 0 || a[2] > kMaxBeams || a[6] == 0 || a[7] == 0 || a[7] > 65535 ||
             (b[1] | b[2] | b[3] | b[4] | b[5] | b[6] | b[7]))
             return "invalid BEAM_REORDER";
+        // (n is below 2^53; the layers' product with it may pass 64 bits, so that they are divided out)
+        const size_t n = size_t(a[1]) * a[2] * a[6], step = b[0] ? b[0] : n, held = C.lim.state_rows;
+        if (step < n) return "invalid BEAM_REORDER";
+        const char *outside = "BEAM_REORDER outside the state rows, or its source and destination overlap";
+        if (n > held || a[7] - 1 > (held - n) / step) return outside;
         const size_t all = (a[7] - 1) * step + n;
-        if (all > C.lim.state_rows || a[4] > C.lim.state_rows - all || a[5] > C.lim.state_rows - all || (a[4] != a[5] && ranges_meet(a[4], all, a[5], all)))
-            return "BEAM_REORDER outside the state rows, or its source and destination overlap";
+        if (a[4] > held - all || a[5] > held - all || (a[4] != a[5] && ranges_meet(a[4], all, a[5], all))) return outside;
         break;
     }
     default:

@@ -1,10 +1,11 @@
-"""Sizes at the ends of what the calls and commands for several sequences take: steps without rows. No GPU needed, but for the
-tests marked so."""
+"""Sizes at the ends of what the calls and commands for several sequences take: steps without rows, and products of sizes
+that pass 64 bits. No GPU needed, but for the tests marked so."""
 import subprocess
 import sys
 
 import pytest
 
+import plan_limits
 from conftest import ROOT, load_package
 
 b2 = load_package()
@@ -60,3 +61,30 @@ def test_an_attention_of_no_rows_runs_in_lists_and_graphs():
         ctx.synchronize()
         assert np.array_equal(ctx.read(0, 8192), want)
         g.close()
+
+
+@pytest.fixture(scope="module")
+def plan(tmp_path_factory):
+    return plan_limits.build(str(tmp_path_factory.mktemp("plan")))
+
+
+def raw(*slots):
+    return b2.cmd_list(*(b2.cmd(*s) for s in slots))
+
+
+@pytest.mark.parametrize("n_req,beams,rows,layers,step", [
+    (32768, 32, 1 << 29, 32768, 0),               # layers x a layer's rows: 2^64
+    (8192, 32, 1 << 31, 32768, 0),
+    (32768, 32, 1 << 29, 32769, 0),               # 2^64 and a layer more
+    (65535, 32, (1 << 32) - 1, 65535, 0),
+    (1, 2, 256, 3, 1 << 9), (1, 2, 256, 3, 512), (1, 2, 513, 1, 0), (1, 1, 1, 2, 1024)])
+def test_state_rows_behind_the_buffer_are_refused_whatever_their_product(plan, n_req, beams, rows, layers, step):
+    assert n_req * beams * rows + (layers - 1) * (step or n_req * beams * rows) > 1024
+    for dst in (0, 512):
+        assert plan(raw((b2.OP_BEAM_REORDER, n_req, beams, 0, 0, dst, rows, layers), (step,))) == 1
+
+
+@pytest.mark.parametrize("n_req,beams,rows,layers,step,src,dst", [
+    (1, 2, 256, 2, 0, 0, 0), (1, 2, 256, 1, 0, 0, 512), (1, 1, 1, 2, 1023, 0, 0), (4, 4, 8, 8, 128, 0, 0), (1, 1, 1024, 1, 0, 0, 0), (1, 2, 4, 3, 50, 916, 800)])
+def test_state_rows_up_to_the_buffers_end_are_taken(plan, n_req, beams, rows, layers, step, src, dst):
+    assert plan(raw((b2.OP_BEAM_REORDER, n_req, beams, 0, src, dst, rows, layers), (step,))) == 0
