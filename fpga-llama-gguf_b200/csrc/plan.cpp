@@ -113,7 +113,11 @@ struct ServeSpan {
     size_t off, n;  // act floats (uint32 words)
     bool written;
 };
-size_t rows_span(size_t rows, size_t stride, size_t width) { return rows ? (rows - 1) * stride + width : 0; }
+// (SIZE_MAX, which no buffer holds, where the product passes 64 bits)
+size_t rows_span(size_t rows, size_t stride, size_t width) {
+    if (rows == 0) return 0;
+    return stride && rows - 1 > (SIZE_MAX - width) / stride ? SIZE_MAX : (rows - 1) * stride + width;
+}
 
 // The act ranges of a command whose shape is valid.
 std::vector<ServeSpan> serve_spans(const uint32_t (*w)[8]) {

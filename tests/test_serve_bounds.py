@@ -88,3 +88,27 @@ def test_state_rows_behind_the_buffer_are_refused_whatever_their_product(plan, n
     (1, 2, 256, 2, 0, 0, 0), (1, 2, 256, 1, 0, 0, 512), (1, 1, 1, 2, 1023, 0, 0), (4, 4, 8, 8, 128, 0, 0), (1, 1, 1024, 1, 0, 0, 0), (1, 2, 4, 3, 50, 916, 800)])
 def test_state_rows_up_to_the_buffers_end_are_taken(plan, n_req, beams, rows, layers, step, src, dst):
     assert plan(raw((b2.OP_BEAM_REORDER, n_req, beams, 0, src, dst, rows, layers), (step,))) == 0
+
+
+def attention(n_head, n_rows, q_stride, q_head_stride, y=1 << 25):
+    # one KV head of 32; q before y
+    geo = b2.kv4_geometry(1, 32, 16)
+    return raw((b2.OP_KV4_ATTN, n_head, 1 << 20, y, 0, 4, 64, 128), (1, n_rows, 1, 64, 0x3F800000, 0, q_stride, q_head_stride), (geo, 0, 8, 0))
+
+
+@pytest.mark.parametrize("n_head,n_rows,q_head_stride", [
+    (510, 16777124, 2155916975),                   # the last row's place is 2^64 and some 7 million
+    (1024, (1 << 24) - 1, (1 << 32) - 1), (1024, 1 << 24, 1 << 30), (512, (1 << 23) + 1, 1 << 31), (1, 2, (1 << 32) - 1)])
+def test_queries_behind_the_buffer_are_refused_whatever_their_product(plan, n_head, n_rows, q_head_stride):
+    # an act buffer that y fits, and q does not (the planner's arithmetic alone: no GPU holds y where the product wraps)
+    act = (1 << 25) + n_rows * n_head * 32
+    assert (1 << 20) + ((n_rows - 1) * n_head + n_head - 1) * q_head_stride + 32 > act
+    assert plan(attention(n_head, n_rows, 0, q_head_stride), act_floats=act) == 1
+
+
+def test_queries_up_to_the_buffers_end_are_taken(plan):
+    # 3 rows of 4 heads 100 floats apart, the rows 500: the last float of q is the buffer's
+    for stride, head, n in ((500, 100, 2 * 500 + 3 * 100 + 32), (0, 100, 2 * 400 + 3 * 100 + 32), (0, 0, 3 * 128)):
+        cl = attention(4, 3, stride, head, y=4096)
+        assert plan(cl, act_floats=(1 << 20) + n) == 0
+        assert plan(cl, act_floats=(1 << 20) + n - 1) == 1
