@@ -345,11 +345,13 @@ B200Q_API int b200q_kv4_attn(int device, const b200q_kv4_pool *pool, const float
     if (!c.ok()) return c.rc();
     const size_t dim = pool->head_dim, width = n_head * dim;
     if (q_head_stride == 0) q_head_stride = dim;
+    c.need(q_head_stride <= kMaxStride, "a stride of q or y is over 2^32 floats");  // (before it is multiplied)
+    if (!c.ok()) return c.rc();
     const size_t q_width = (n_head - 1) * q_head_stride + dim;
     if (q_stride == 0) q_stride = n_head * q_head_stride;
     if (y_stride == 0) y_stride = width;
-    c.need(q_head_stride >= dim && q_stride >= q_width && y_stride >= width && q_stride <= kMaxStride && y_stride <= kMaxStride,
-           "a stride of q or y is smaller than what it steps over");
+    c.need(q_stride <= kMaxStride && y_stride <= kMaxStride, "a stride of q or y is over 2^32 floats");
+    c.need(q_head_stride >= dim && q_stride >= q_width && y_stride >= width, "a stride of q or y is smaller than what it steps over");
     c.need(table_stride >= 1 && (unsigned long long)table_stride * pool->page_tokens >= max_kv, "max_kv does not fit table_stride pages");
     c.need(std::isfinite(scale), "scale is not finite");
     c.enter();

@@ -112,3 +112,12 @@ def test_queries_up_to_the_buffers_end_are_taken(plan):
         cl = attention(4, 3, stride, head, y=4096)
         assert plan(cl, act_floats=(1 << 20) + n) == 0
         assert plan(cl, act_floats=(1 << 20) + n - 1) == 1
+
+
+@pytest.mark.parametrize("n_head,q_stride,q_head_stride", [
+    (17, 0, 1 << 60),           # 16 x 2^60 floats: a row's width wraps to one head's
+    (17, 64, 1 << 60), (16, 0, 1 << 60), (2, 0, (1 << 64) - 64), (2, 0, (1 << 32) + 1), (5, 1 << 33, 1 << 33), (3, (1 << 32) + 1, 64)])
+def test_query_strides_beyond_all_memory_are_refused_before_the_device(n_head, q_stride, q_head_stride):
+    h = pool(n_kv=1)
+    with pytest.raises(b2.B200QError, match="stride"):
+        b2.kv4_attn(0, h, 4096, 4096, 2, n_head, 4096, 4, 4096, 4096, 1, 1, 64, 1.0, 4096, 1 << 30, q_stride, q_head_stride)
