@@ -195,7 +195,7 @@ Kv4View view_of(const b200q_kv4_pool *p) {
 
 size_t rows_extent(size_t rows, size_t stride, size_t width) { return rows ? ((rows - 1) * stride + width) * 4 : 0; }
 
-constexpr size_t kMaxStride = size_t(1) << 32;
+constexpr size_t kMaxStride = size_t(1) << 32, kMaxSpan = size_t(1) << 60;  // floats
 
 int rows_call(const char *name, bool store, int device, const b200q_kv4_pool *pool, float *k, float *v, const uint32_t *slots, unsigned n,
               size_t k_stride, size_t v_stride, uint32_t *status, void *stream, char *err, unsigned err_len) {
@@ -206,6 +206,8 @@ int rows_call(const char *name, bool store, int device, const b200q_kv4_pool *po
     if (k_stride == 0) k_stride = width;
     if (v_stride == 0) v_stride = width;
     c.need(k_stride >= width && v_stride >= width && k_stride <= kMaxStride && v_stride <= kMaxStride, "a row stride is smaller than n_kv_head x head_dim");
+    // (n and the strides are below 2^32 and 2^32 + 1: their products fit 64 bits, and so do the rows' bytes)
+    c.need(!c.ok() || (n * k_stride <= kMaxSpan && n * v_stride <= kMaxSpan), "rows and their stride pass 2^60 floats");
     c.enter();
     if (!c.ok() || n == 0) return c.rc();
     c.memory("pool", pool->base, bytes, 16, store);

@@ -121,3 +121,12 @@ def test_query_strides_beyond_all_memory_are_refused_before_the_device(n_head, q
     h = pool(n_kv=1)
     with pytest.raises(b2.B200QError, match="stride"):
         b2.kv4_attn(0, h, 4096, 4096, 2, n_head, 4096, 4, 4096, 4096, 1, 1, 64, 1.0, 4096, 1 << 30, q_stride, q_head_stride)
+
+
+@pytest.mark.parametrize("k_stride,v_stride", [(1 << 32, 128), (128, 1 << 32), (1 << 32, 0)])
+def test_rows_whose_bytes_pass_64_bits_are_refused_before_the_device(k_stride, v_stride):
+    n = (1 << 30) + 1  # rows 2^34 bytes apart: the last one lies 2^64 bytes behind the first
+    for call in (lambda: b2.kv4_store(0, pool(), 4096, 4096, 4096, n, k_stride, v_stride),
+                 lambda: b2.kv4_load(0, pool(), 4096, n, 4096, 4096, k_stride, v_stride)):
+        with pytest.raises(b2.B200QError, match="rows and their stride"):
+            call()
