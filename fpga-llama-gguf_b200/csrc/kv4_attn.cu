@@ -307,6 +307,9 @@ __global__ void __launch_bounds__(kThreads, Shape<NB, NT>::kCtas) kv4_attn_kerne
     __shared__ uint64_t bars[kWarps][S::kSlots];
     __shared__ float m_of[kWarps][S::kRows], l_of[kWarps][S::kRows];
     __shared__ float scale_of[S::kRows];
+    // of a warp's piece, by block: the scales seen are below 2^top_of, and are lifted by 4^lift_of
+    constexpr int kNoScale = -128;
+    __shared__ int8_t top_of[kWarps][NB], lift_of[kWarps][NB];
     auto *before = reinterpret_cast<unsigned *>(smem + S::kSmem);
     const unsigned tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const unsigned per = a.n_head / a.c.n_kv, tiles_per_page = a.c.page / kTileTokens;
@@ -486,6 +489,7 @@ __global__ void __launch_bounds__(kThreads, Shape<NB, NT>::kCtas) kv4_attn_kerne
                 }
             }
         }
+        if (lane < NB) top_of[warp][lane] = int8_t(kNoScale), lift_of[warp][lane] = 0;
         __syncthreads();
         uint32_t qb[S::kQInRegs ? NT : 1][S::kQInRegs ? NB * 2 : 1][2];
         float scale[NT];        // of row t
@@ -510,7 +514,8 @@ __global__ void __launch_bounds__(kThreads, Shape<NB, NT>::kCtas) kv4_attn_kerne
             }
         }
 
-        float o[NT][NB * 2][4], top[NT], sum[NT], limit = 0.0f, lift = 1.0f, lift_d = 1.0f;
+        float o[NT][NB * 2][4], top[NT], sum[NT], limit = 0.0f, lift = 1.0f;
+        bool mixed = false;  // a block has a lift of its own
 #pragma unroll
         for (int m = 0; m < NT; ++m) {
             top[m] = -INFINITY;
@@ -525,6 +530,8 @@ __global__ void __launch_bounds__(kThreads, Shape<NB, NT>::kCtas) kv4_attn_kerne
         const int last_row = base + int((row0 + plan.rows < all ? row0 + plan.rows - 1 : all - 1) / per);
         const int all_low = a.window && last_row >= 0 && unsigned(last_row) + 1 > a.window ? last_row + 1 - int(a.window) : 0;
         const int all_high = base + int(row0 / per);
+        // and keys that some row sees lie in [any_low, last_row]
+        const int any_low = a.window && all_high >= 0 && unsigned(all_high) + 1 > a.window ? all_high + 1 - int(a.window) : 0;
         auto edge = [&](int key0) { return key0 < all_low || key0 + int(kTileTokens) - 1 > all_high; };
 
         // the scores of row t and the tile's keys g, g + 8
@@ -610,64 +617,109 @@ __global__ void __launch_bounds__(kThreads, Shape<NB, NT>::kCtas) kv4_attn_kerne
                 sum[m] += s[m][0] + s[m][1];
             }
         };
+        // A tile holds scales that pass what they are lifted for: every block's largest so far (four lanes a block), and from these
+        // the common lift of the weights and each block's own, 4^lift_of: none where its largest scale is within 2^4 of `limit`, so
+        // that most caches need none. What the outputs hold already follows. (With one lift for all blocks, values 2^20 below
+        // another block's were off by 3 10^-5, and lost from 2^30 on. The lifts of their own cost 0.7% on average, 3% at most, over 30
+        // shapes of one request and of 64 whose scales are alike: the first tile of a piece raises, and a second one where the largest
+        // scale passes a power of two. With 1/2 as the least limit in the place of 1, where more pieces raise twice, 1.7%.)
+        auto raise = [&](const uint8_t *tile, int key0) {
+            const unsigned b = lane % 8;
+            unsigned big = 0;  // the largest number among the block's scales that some row sees, in a half's bits
+            if (b < NB) {
+#pragma unroll
+                for (unsigned i = 0; i < 4; ++i) {
+                    const unsigned tok = lane / 8 * 4 + i, d = *reinterpret_cast<const uint16_t *>(tile + NB * 544 + (tok * NB + b) * 2) & 0x7fffu;
+                    const int key = key0 + int(tok);
+                    if (key >= any_low && key <= last_row && d <= 0x7bffu) big = max(big, d);
+                }
+            }
+            big = max(big, __shfl_xor_sync(~0u, big, 8));
+            big = max(big, __shfl_xor_sync(~0u, big, 16));
+            const int exponent = int(__float_as_uint(__half2float(__ushort_as_half(uint16_t(big)))) >> 23) - 126;
+            const int own = b < NB ? max(int(top_of[warp][b]), big ? exponent : kNoScale) : kNoScale;  // below 2^own so far
+            const int most = __reduce_max_sync(~0u, own), at = most < 0 ? 0 : most > 8 ? 8 : most;
+            // limit = 2^at: at 2^8 p's lower part loses as much as a scale that is lowered does
+            const int r = at - own, own_lift = r >= 30 ? 15 : r >= 4 ? r / 2 : r >= 0 ? 0 : (r - 1) / 2;
+            const float now = __uint_as_float(unsigned(127 + 14 - at) << 23);
+            if (limit != 0.0f) {  // (else the outputs hold nothing yet)
+                const float follow = now / lift * __uint_as_float(unsigned(127 + 2 * (b < NB ? own_lift - lift_of[warp][b] : 0)) << 23);
+#pragma unroll
+                for (int i = 0; i < NB; ++i) {
+                    const float f = __shfl_sync(~0u, follow, i);
+#pragma unroll
+                    for (int m = 0; m < NT; ++m)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[m][2 * i][e] *= f, o[m][2 * i + 1][e] *= f;
+                }
+            }
+            mixed = __any_sync(~0u, b < NB && own_lift != 0);
+            if (lane < NB) top_of[warp][lane] = int8_t(own), lift_of[warp][lane] = int8_t(own_lift);
+            __syncwarp();
+            lift = now;
+            limit = __uint_as_float(unsigned(127 + at) << 23);
+        };
         auto value = [&](const uint8_t *tile, int key0, const float (&s)[NT][2]) {
             // The weighted sum of the values: dims by keys, keys by rows.
             // A weight p d is a product of FP16 pairs: with p = ph + pl, wh = fp16(ph d) and wl = fp16(pl d + (ph d - wh)),
-            // where ph d - wh is exact in one FP16 multiply-add. p is lifted by a power of two that keeps the largest weight
-            // below 2^14 (`limit`: a power of two that no scale seen so far passes), so that small values keep 22 bits too; scales
-            // below 1/16 are lifted as well.
+            // where ph d - wh is exact in one FP16 multiply-add. What is below 2^-24 is lost, so p is lifted by the power of two that
+            // keeps the weights below 2^14 while no d passes `limit`, and a block's d by one of its own (raise, above). Together the
+            // parts lost are 2^-34 of the block's largest d, or less (2^-30 where that passes 2^4), whatever the other blocks hold.
             uint32_t dv[2][NB];    // the scales of the keys 2 t + 8 j and the one behind it
             uint32_t seen[NT][2];  // these pairs of keys, by row g / 2, as masks of halves: a key that is not seen weighs nothing, whatever its scale holds
+            auto load = [&] {
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                uint32_t raw[NB];
-                load_words<NB>(raw, tile + NB * 544 + (4 * j + t) * NB * 4);
+                for (int j = 0; j < 2; ++j) {
+                    uint32_t raw[NB];
+                    load_words<NB>(raw, tile + NB * 544 + (4 * j + t) * NB * 4);
 #pragma unroll
-                for (int b = 0; b < NB; ++b) dv[j][b] = h2(pair_at(raw, b, NB + b));
+                    for (int b = 0; b < NB; ++b) dv[j][b] = h2(pair_at(raw, b, NB + b));
+                }
+            };
+            auto hide = [&] {  // keys that no row sees
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    uint32_t any = 0;
+#pragma unroll
+                    for (int m = 0; m < NT; ++m) any |= seen[m][j];
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) dv[j][b] &= any;
+                }
+            };
+            auto lift_blocks = [&] {
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    const half2 f = as_h2(unsigned(15 + lift_of[warp][b]) * 0x04000400u);  // twice: a half reaches 2^15
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) dv[j][b] = h2(__hmul2(__hmul2(as_h2(dv[j][b]), f), f));
+                }
+            };
+            load();
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
 #pragma unroll
                 for (int m = 0; m < NT; ++m) seen[m][j] = ~0u;
-            }
             if (edge(key0)) {
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     const int key = key0 + 8 * j + 2 * int(t);
-                    uint32_t any = 0;
 #pragma unroll
-                    for (int m = 0; m < NT; ++m) {
+                    for (int m = 0; m < NT; ++m)
                         seen[m][j] = (key >= wlow[m] && key <= wpos[m] ? 0x0000ffffu : 0u) | (key + 1 >= wlow[m] && key + 1 <= wpos[m] ? 0xffff0000u : 0u);
-                        any |= seen[m][j];
-                    }
-#pragma unroll
-                    for (int b = 0; b < NB; ++b) dv[j][b] &= any;
                 }
+                hide();
             }
+            if (mixed) lift_blocks();
             half2 big2 = __float2half2_rn(0.0f);
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
                 for (int b = 0; b < NB; ++b) big2 = __hmax2(big2, __habs2(as_h2(dv[j][b])));
-            float big = fmaxf(__low2float(big2), __high2float(big2));
-            if (__any_sync(~0u, big > limit)) {
-#pragma unroll
-                for (int x = 1; x < 32; x <<= 1) big = fmaxf(big, __shfl_xor_sync(~0u, big, x));
-                const float was = lift * lift_d;
-                limit = __uint_as_float((__float_as_uint(fminf(big, 65504.0f)) & 0x7f800000u) + 0x00800000u);  // the next power of two
-                lift_d = limit < 0x1p-4f ? 0x1p15f : 1.0f;
-                lift = fminf(0x1p14f / (limit * lift_d), 0x1p15f);
-                const float f = lift * lift_d / was;
-#pragma unroll
-                for (int m = 0; m < NT; ++m)
-#pragma unroll
-                    for (int i = 0; i < NB * 2; ++i)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) o[m][i][e] *= f;
-            }
-            if (lift_d != 1.0f) {
-                const half2 f = __float2half2_rn(lift_d);
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-#pragma unroll
-                    for (int b = 0; b < NB; ++b) dv[j][b] = h2(__hmul2(as_h2(dv[j][b]), f));
+            if (__any_sync(~0u, fmaxf(__low2float(big2), __high2float(big2)) > limit)) {
+                const bool was_mixed = mixed;
+                raise(tile, key0);
+                if (was_mixed) load(), hide();
+                if (mixed) lift_blocks();
             }
             // Of row g / 2 and the keys 2 t + 8 j, + 1. A lane of an upper column wants ph d, one of a lower column the rest: with
             // (x, y) = (0, ph) in the one and (ph, pl) in the other both are y d + (x d - fp16(x d)).
@@ -753,7 +805,7 @@ __global__ void __launch_bounds__(kThreads, Shape<NB, NT>::kCtas) kv4_attn_kerne
 
         // the warps' results: [warp][row][dim] (the barrier: all have read the piece before's)
         __syncthreads();
-        const float drop = 1.0f / (lift * lift_d);
+        const float drop = 1.0f / lift;
 #pragma unroll
         for (int m = 0; m < NT; ++m) {
 #pragma unroll
@@ -762,9 +814,9 @@ __global__ void __launch_bounds__(kThreads, Shape<NB, NT>::kCtas) kv4_attn_kerne
             float *to = out + (warp * S::kRows + m * 4 + t) * D + 4 * (g >> 1) + 2 * (g & 1);
 #pragma unroll
             for (int b = 0; b < NB; ++b) {  // two bytes of a word: the low nibbles, then the high ones
-                *reinterpret_cast<float2 *>(to + 32 * b) = make_float2((o[m][2 * b][0] + o[m][2 * b][1]) * drop, (o[m][2 * b + 1][0] + o[m][2 * b + 1][1]) * drop);
-                *reinterpret_cast<float2 *>(to + 32 * b + 16) =
-                    make_float2((o[m][2 * b][2] + o[m][2 * b][3]) * (0.0625f * drop), (o[m][2 * b + 1][2] + o[m][2 * b + 1][3]) * (0.0625f * drop));
+                const float f = drop * __uint_as_float(unsigned(127 - 2 * lift_of[warp][b]) << 23), f16 = 0.0625f * f;
+                *reinterpret_cast<float2 *>(to + 32 * b) = make_float2((o[m][2 * b][0] + o[m][2 * b][1]) * f, (o[m][2 * b + 1][0] + o[m][2 * b + 1][1]) * f);
+                *reinterpret_cast<float2 *>(to + 32 * b + 16) = make_float2((o[m][2 * b][2] + o[m][2 * b][3]) * f16, (o[m][2 * b + 1][2] + o[m][2 * b + 1][3]) * f16);
             }
         }
         if (__syncthreads_or(late)) {
