@@ -3,13 +3,15 @@
 // A CTA takes 128 query rows (token, head of the group) of one KV head and goes over the keys 64 at a time, with FP32
 // sums and outputs as in kv4_attn.cu:
 //   S = Q K^T        FP32 accuracy from FP16 products: q = qh + ql (22 bits; rows scaled by a power of two), and a value of
-//                    the cache is d (c - 8), 15 bits, so kh + kl holds it exactly: S = qh kh + ql kh + qh kl
-//                    (what ql kl would add is below 2^-22 of a product)
+//                    the cache is d (c - 8), a multiple of FP16's smallest number of at most 15 bits, so kh + kl holds it
+//                    exactly: S = qh kh + ql kh + qh kl (what ql kl would add is below 2^-22 of a product)
 //   P = 2^(s - m)    the running maximum m of a row moves only when a score passes it
 //   O += P V         the same way: ph vh + pl vh + ph vl, in tensor memory over all keys
-// K and V rows are scaled by a power of two each (the key's largest d becomes 1/2 to 1), so that FP16 holds them whatever
-// their magnitude. K's comes back in as a factor of the key's column of S; V's, e_t, moves into the weight:
-// w_t = 2^(s_t + log2 e_t - m), and the sum of the weights takes w_t / e_t.
+// Values of 2^16 and more do not fit FP16: a token's K or V with a d of 2^13 or more is lowered by 2^e, e = 1 to 3, so that
+// its largest d is below 2^13. All others enter as they are, whatever their magnitude and however far a token's blocks lie
+// apart. (The largest d of every token raised to 1/2, as it was once, made subnormals of d 2^14 below it and lost their bits;
+// now only such a token's d below 2^-11 lose some, 2^-37 of its largest one at most.) K's 2^e comes back in as a factor of the
+// key's column of S; V's, e_t, moves into the weight: w_t = 2^(s_t + e_t - m), and the sum of the weights takes w_t / 2^e_t.
 //
 // Operands: qh, kh, kl, vh, vl in shared memory (no swizzle; K is K-major, V MN-major, both written 16 bytes = 8 dims of a
 // key at a time by the same code), ql and P in tensor memory. kl lies behind kh, so that one product of N 128 forms qh kh and
@@ -343,7 +345,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnAr
         }
         top = fmaxf(top, __shfl_xor_sync(~0u, top, 8));
         top = fmaxf(top, __shfl_xor_sync(~0u, top, 16));
-        const int e = top == 0.0f ? 0 : int(__float_as_uint(fminf(top, 65504.0f)) >> 23) - 126;  // top / 2^e is below 1
+        const int over = int(__float_as_uint(fminf(top, 65504.0f)) >> 23) - 139, e = over > 0 ? over : 0;  // top / 2^e is below 2^13
         if (lane < 8) {
             if (is_v) v_log[key] = hidden ? -INFINITY : float(e), v_inv[key] = pow2(-e);
             else k_scale[key] = pow2(e);

@@ -1,5 +1,6 @@
 """Attention over the 4-bit cache where the 32-dim blocks of a token have scales far from one another, for single tokens and drafts
-(units of up to sixteen rows): a block's dims are as good as if the others were not there, whatever lies in them."""
+(units of up to sixteen rows) and for prompts (the tensor-memory kernel): a block's dims are as good as if the others were
+not there, whatever lies in them."""
 import math
 
 import numpy as np
@@ -16,6 +17,7 @@ torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
 FEW = [(1, 1), (1, 40), (3, 130), (1, 333), (2, 64)]
+PROMPTS = [(150, 190), (1, 300), (60, 333), (97, 97)]
 
 
 def unlike(r, n, n_kv, dim, large, small, kind):
@@ -59,17 +61,21 @@ def check(b, got, window=0, q=None):
     A weight p d is split into two FP16 numbers, off by at most 2^-25 each; a block's d are lifted so that this is 2^-34 of its
     largest d at most, for d up to 2^4. Above, p's own part counts: 2^-25 / 2^(14 - 8), times d, and what FP16 cannot hold of a d that
     is lowered by at most 2^8, 2^-17 where the largest is 2^15 (2^-23 where it is 2^8): together 2^-30 of the largest. By n keys, and a
-    sum of all p of 2^-4 at least: n 2^-30 (n 2^-26) of the largest |v| = 8 d."""
+    sum of all p of 2^-4 at least: n 2^-30 (n 2^-26) of the largest |v| = 8 d.
+    Prompts: P's parts are off by 2^-25 of 2^10 at least, and by 2^3 more where a token's values pass 2^16: n 2^-32 of the block's
+    largest |v|. Such a token's d are lowered by up to 2^3: what FP16 drops is 2^-25 2^e where the largest is 2^(12 + e) at
+    least, 2^-37 of it."""
     table, page = b.table, b.p.ref.page
     y, mag, big = ref.attention(b.p.ref, b.q if q is None else q, table, b.q_start, b.kv, b.scale, window)
     dim, n_kv, group = b.p.ref.dim, b.p.ref.n_kv, b.n_head // b.p.ref.n_kv
-    own = np.zeros(y.shape)
+    own, all_ = np.zeros(y.shape), np.zeros(y.shape)
     for i, n in enumerate(b.kv):
         v = np.abs(b.p.ref.values(1, table[i][np.arange(n) // page], np.arange(n) % page)).max(0)  # n_kv, dim
         rows = slice(int(b.q_start[i]), int(b.q_start[i + 1]))
         own[rows] = np.repeat(np.repeat(v.reshape(n_kv, -1, 32).max(-1), 32, -1), group, 0)
+        all_[rows] = np.repeat(v.max(-1, keepdims=True), group, 0)
     n = max(b.kv)
-    tol = 2.0 ** -17 * (1 + big[:, :, None] / 8) * mag + (mag > 0) * n * own * np.where(own > 128, 2.0 ** -26, 2.0 ** -30)
+    tol = 2.0 ** -17 * (1 + big[:, :, None] / 8) * mag + (mag > 0) * (n * own * np.where(own > 128, 2.0 ** -26, 2.0 ** -30) + np.where(all_ > 65536, 2.0 ** -37, 0) * all_)
     assert np.isfinite(got).all() and u32(b.status)[0] == 0
     bad = (np.abs(got - y) - tol) / (mag + 1e-300)
     assert bad.max(initial=0) <= 0, (bad.max(), np.unravel_index(bad.argmax(), bad.shape))
@@ -87,8 +93,17 @@ def test_values_of_unlike_blocks_few_rows(b2, dim, n_kv, group, large, small, ki
     check(b, b.run(pad=1))
 
 
+@pytest.mark.parametrize("large,small,kind", CASES)
+@pytest.mark.parametrize("dim,group", [(64, 12), (256, 12)])
+def test_values_of_unlike_blocks_prompts(b2, dim, group, large, small, kind):
+    r = rng(401, dim, 50 + large, -small)
+    b = Blocks(b2, r, PROMPTS, 2, group, dim, 32, v=lambda n: unlike(r, n, 2, dim, large, small, kind))
+    assert b.rows * b.n_head >= 6144
+    check(b, b.run(pad=1))
+
+
 @pytest.mark.parametrize("window", [5, 70])
-@pytest.mark.parametrize("lengths", [FEW])
+@pytest.mark.parametrize("lengths", [FEW, PROMPTS])
 def test_values_of_unlike_blocks_in_windows(b2, lengths, window):
     r = rng(404, window)
     b = Blocks(b2, r, lengths, 2, 12, 96, 16, v=lambda n: unlike(r, n, 2, 96, 10, -14, "turns"))
@@ -96,7 +111,7 @@ def test_values_of_unlike_blocks_in_windows(b2, lengths, window):
 
 
 @pytest.mark.parametrize("large,small", [(0, -12), (0, -16), (0, -20), (10, -13), (12, -10)])
-@pytest.mark.parametrize("dim,group,lengths", [(128, 8, FEW)])
+@pytest.mark.parametrize("dim,group,lengths", [(128, 8, FEW), (64, 12, PROMPTS), (256, 12, PROMPTS)])
 def test_keys_of_unlike_blocks_and_queries_that_are_zero_in_the_large_ones(b2, dim, group, lengths, large, small):
     # the scores come from the small blocks alone
     r = rng(402, dim, group)
@@ -106,7 +121,7 @@ def test_keys_of_unlike_blocks_and_queries_that_are_zero_in_the_large_ones(b2, d
     check(b, b.run())
 
 
-@pytest.mark.parametrize("lengths", [FEW])
+@pytest.mark.parametrize("lengths", [FEW, PROMPTS])
 def test_values_that_grow_from_token_to_token(b2, lengths):
     # a block's largest scale passes the ones before it again and again, each block at other tokens; some blocks begin with zeros
     r = rng(403)
