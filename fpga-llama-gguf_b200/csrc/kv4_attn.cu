@@ -11,7 +11,8 @@
 //   y_i  = sum_t (p_t d_tb) (c_ti - 8)            the weight of a token differs by block, not by dim
 // The FP32 factors (q, and p_t d_tb) are split into two FP16 numbers, 22 bits in all, which sit side by side in two columns of
 // the matrix instruction's B operand: four query rows fill its eight columns, and FP32 accuracy costs no second
-// instruction. q's rows are first scaled by a power of two to below 2^11, and their lower parts by 2048.
+// instruction. q's rows are first scaled by a power of two to below 2^15, and their lower parts by 2048, so that a number of
+// a row 2^20 below its largest has its 22 bits too.
 #include <cuda_runtime.h>
 
 #include "common.cuh"
@@ -470,7 +471,7 @@ __global__ void __launch_bounds__(kThreads, Shape<NB, NT>::kCtas) kv4_attn_kerne
 #pragma unroll
             for (int i = 0; i < kQuads; ++i) big = fmaxf(big, fmaxf(fmaxf(fabsf(x[m][i].x), fabsf(x[m][i].y)), fmaxf(fabsf(x[m][i].z), fabsf(x[m][i].w))));
             big = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(big)));
-            int ex = int(__float_as_uint(big) >> 23) - 127 - 10;  // x / 2^ex is below 2^11
+            int ex = int(__float_as_uint(big) >> 23) - 127 - 14;  // x / 2^ex is below 2^15
             ex = ex < -110 ? -110 : ex > 100 ? 100 : ex;
             const float down = __uint_as_float(unsigned(127 - ex) << 23);
             if (lane == 0) scale_of[m * 4 + warp] = a.scale * kLog2e * __uint_as_float(unsigned(127 + ex) << 23);

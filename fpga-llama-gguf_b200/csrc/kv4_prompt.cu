@@ -4,7 +4,8 @@
 // sums and outputs as in kv4_attn.cu:
 //   S = Q K^T        FP32 accuracy from FP16 products: q = qh + ql (22 bits; rows scaled by a power of two), and a value of
 //                    the cache is d (c - 8), a multiple of FP16's smallest number of at most 15 bits, so kh + kl holds it
-//                    exactly: S = qh kh + ql kh + qh kl (what ql kl would add is below 2^-22 of a product)
+//                    exactly: S = qh kh + ql kh + qh kl (what ql kl would add is below 2^-22 of a product). ql and kl are
+//                    held 2^11 times as large, so that a number of q has its 22 bits down to 2^28 below the row's largest
 //   P = 2^(s - m)    the running maximum m of a row moves only when a score passes it
 //   O += P V         the same way: ph vh + pl vh + ph vl, in tensor memory over all keys
 // Values of 2^16 and more do not fit FP16: a token's K or V with a d of 2^13 or more is lowered by 2^e, e = 1 to 3, so that
@@ -43,6 +44,7 @@ constexpr unsigned kRows = 128, kKeys = 64, kWork = 256, kThreads = kWork + 32; 
 constexpr unsigned kFold = 32;
 constexpr unsigned kBadMax = 96;  // values that are not numbers, remembered by (key, block)
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLow = 2048.0f;  // ql and kl are 2^11 times what they stand for, so that they seldom are subnormal
 
 __device__ __forceinline__ void tell(uint32_t *status, unsigned bit) {
     if (status) atomicOr(status, bit);
@@ -260,7 +262,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnAr
             __syncwarp();
         }
     } else {
-    // Q: rows scaled to below 2^11; the upper parts to shared memory, the lower ones to tensor memory, by way of V's place.
+    // Q: rows scaled to below 2^15; the upper parts to shared memory, the lower ones to tensor memory, by way of V's place.
     // A warp takes a row at a time, its lanes four dims each.
     float row_scale;
     {
@@ -289,7 +291,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnAr
                 for (unsigned n = 0; n < kTurns; ++n)
                     top = fmaxf(top, fmaxf(fmaxf(fabsf(v[i][n].x), fabsf(v[i][n].y)), fmaxf(fabsf(v[i][n].z), fabsf(v[i][n].w))));
                 for (unsigned x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, x));
-                int ex = int(__float_as_uint(top) >> 23) - 127 - 10;
+                int ex = int(__float_as_uint(top) >> 23) - 127 - 14;
                 ex = ex < -110 ? -110 : ex > 110 ? 110 : ex;
                 const float down = pow2(-ex);
                 if (lane == 0) row_top[0][r] = a.scale * kLog2e * pow2(ex);
@@ -302,7 +304,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnAr
                     const float2 bp = __half22float2(p), bq = __half22float2(q);
                     const unsigned at = r / 8 * (D * 16) + d / 8 * 128 + r % 8 * 16 + d % 8 * 2;
                     *reinterpret_cast<uint2 *>(smem + at) = make_uint2(h2(p), h2(q));
-                    *reinterpret_cast<uint2 *>(vh + at) = make_uint2(h2(__floats2half2_rn(y.x - bp.x, y.y - bp.y)), h2(__floats2half2_rn(y.z - bq.x, y.w - bq.y)));
+                    *reinterpret_cast<uint2 *>(vh + at) = make_uint2(h2(__floats2half2_rn((y.x - bp.x) * kLow, (y.y - bp.y) * kLow)), h2(__floats2half2_rn((y.z - bq.x) * kLow, (y.w - bq.y) * kLow)));
                 }
             }
         }
@@ -373,7 +375,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnAr
                             const half2 c = __hsub2(as_h2((pair >> (4 * n) & 0x000f000fu) | 0x64006400u), as_h2(0x64086408u));
                             const half2 v = __hmul2(c, dd);
                             hi_of[n][2 * i + x] = h2(v);
-                            lo_of[n][2 * i + x] = h2(__hfma2(c, dd, __hneg2(v)));
+                            const half2 rest = __hfma2(c, dd, __hneg2(v));
+                            lo_of[n][2 * i + x] = h2(is_v ? rest : __hmul2(rest, __float2half2_rn(kLow)));
                         }
                     }
                 }
@@ -448,8 +451,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnAr
 #pragma unroll
             for (unsigned e = 0; e < 2; ++e) {
                 const unsigned k = 2 * (i + e);
-                const float2 x = add2(make_float2(__uint_as_float(s[k]), __uint_as_float(s[k + 1])),
-                                      make_float2(__uint_as_float(s_low[k]), __uint_as_float(s_low[k + 1])));
+                const float2 x = fma2(make_float2(__uint_as_float(s_low[k]), __uint_as_float(s_low[k + 1])), make_float2(1.0f / kLow, 1.0f / kLow),
+                                      make_float2(__uint_as_float(s[k]), __uint_as_float(s[k + 1])));
                 w[i + e] = fma2(mul2(x, f[e]), scale2, g[e]);  // (a hidden key: -inf)
             }
         }

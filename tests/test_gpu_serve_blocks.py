@@ -121,6 +121,18 @@ def test_keys_of_unlike_blocks_and_queries_that_are_zero_in_the_large_ones(b2, d
     check(b, b.run())
 
 
+@pytest.mark.parametrize("large", [12, 20, 24])
+@pytest.mark.parametrize("dim,group,lengths", [(64, 4, FEW), (128, 8, FEW), (64, 12, PROMPTS), (256, 12, PROMPTS)])
+def test_queries_of_unlike_blocks_and_keys_that_are_zero_in_the_large_ones(b2, dim, group, lengths, large):
+    # the scores come from the blocks in which a row of q is 2^large below its largest
+    r = rng(405, dim, group)
+    small = np.arange(dim) // 32 % 2 == 1
+    b = Blocks(b2, r, lengths, 2, group, dim, 16, k=lambda n: (r.normal(0, 1, (n, 2, dim)) * small).reshape(n, -1).astype(np.float32))
+    b.q = (b.q * np.where(small, 1.0, 2.0 ** large)).astype(np.float32)
+    b.scale = math.sqrt(2.0 / dim)
+    check(b, b.run())
+
+
 @pytest.mark.parametrize("lengths", [FEW, PROMPTS])
 def test_values_that_grow_from_token_to_token(b2, lengths):
     # a block's largest scale passes the ones before it again and again, each block at other tokens; some blocks begin with zeros
