@@ -472,7 +472,7 @@ __global__ void __launch_bounds__(kThreads, Shape<NB, NT>::kCtas) kv4_attn_kerne
             for (int i = 0; i < kQuads; ++i) big = fmaxf(big, fmaxf(fmaxf(fabsf(x[m][i].x), fabsf(x[m][i].y)), fmaxf(fabsf(x[m][i].z), fabsf(x[m][i].w))));
             big = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(big)));
             int ex = int(__float_as_uint(big) >> 23) - 127 - 14;  // x / 2^ex is below 2^15
-            ex = ex < -110 ? -110 : ex > 100 ? 100 : ex;
+            ex = ex < -110 ? -110 : ex > 113 ? 113 : ex;  // (NaN, infinity: what they are)
             const float down = __uint_as_float(unsigned(127 - ex) << 23);
             if (lane == 0) scale_of[m * 4 + warp] = a.scale * kLog2e * __uint_as_float(unsigned(127 + ex) << 23);
 #pragma unroll

@@ -292,7 +292,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnAr
                     top = fmaxf(top, fmaxf(fmaxf(fabsf(v[i][n].x), fabsf(v[i][n].y)), fmaxf(fabsf(v[i][n].z), fabsf(v[i][n].w))));
                 for (unsigned x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, x));
                 int ex = int(__float_as_uint(top) >> 23) - 127 - 14;
-                ex = ex < -110 ? -110 : ex > 110 ? 110 : ex;
+                ex = ex < -110 ? -110 : ex > 113 ? 113 : ex;  // (NaN, infinity: what they are)
                 const float down = pow2(-ex);
                 if (lane == 0) row_top[0][r] = a.scale * kLog2e * pow2(ex);
 #pragma unroll

@@ -133,6 +133,15 @@ def test_queries_of_unlike_blocks_and_keys_that_are_zero_in_the_large_ones(b2, d
     check(b, b.run())
 
 
+@pytest.mark.parametrize("std", [1e-30, 1e36])
+@pytest.mark.parametrize("lengths", [FEW, PROMPTS])
+def test_queries_near_the_ends_of_fp32(b2, lengths, std):
+    b = Blocks(b2, rng(406), lengths, 2, 12, 96, 16)
+    b.q = (b.q * std).astype(np.float32)
+    b.scale = 1.0 / math.sqrt(96) / std
+    check(b, b.run())
+
+
 @pytest.mark.parametrize("lengths", [FEW, PROMPTS])
 def test_values_that_grow_from_token_to_token(b2, lengths):
     # a block's largest scale passes the ones before it again and again, each block at other tokens; some blocks begin with zeros
