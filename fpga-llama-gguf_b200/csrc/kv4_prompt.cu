@@ -7,7 +7,7 @@
 //                    exactly: S = qh kh + ql kh + qh kl (what ql kl would add is below 2^-22 of a product). ql and kl are
 //                    held 2^11 times as large, so that a number of q has its 22 bits down to 2^28 below the row's largest
 //   P = 2^(s - m)    the running maximum m of a row moves only when a score passes it
-//   O += P V         the same way: ph vh + pl vh + ph vl, in tensor memory over all keys
+//   O += P V         the same way: ph vh + pl vh + ph vl, in tensor memory and, by turns, on to FP32 sums
 // Values of 2^16 and more do not fit FP16: a token's K or V with a d of 2^13 or more is lowered by 2^e, e = 1 to 3, so that
 // its largest d is below 2^13. All others enter as they are, whatever their magnitude and however far a token's blocks lie
 // apart. (The largest d of every token raised to 1/2, as it was once, made subnormals of d 2^14 below it and lost their bits;
@@ -37,11 +37,6 @@ namespace b200q {
 namespace {
 
 constexpr unsigned kRows = 128, kKeys = 64, kWork = 256, kThreads = kWork + 32;  // 8 warps, and one that issues products and copies
-// Steps whose products tensor memory adds up before O goes over to y in FP32. Its sums drop what is below their last bit, a
-// part in 10^8 on average and 12 times a step: with 32 steps O comes out 2 parts in 10^6 too small at most, and the way to
-// y (16,000 cycles of 6500 a step) takes less than a tenth of the time. 2048 new tokens on 2560 keys, 16 heads of 256, with
-// 8 / 16 / 24 / 32 steps: off by 1.7 / 2.4 / 2.8 / 3.1 10^-6 of the result, 370 / 326 / 313 / 305 us.
-constexpr unsigned kFold = 32;
 constexpr unsigned kBadMax = 96;  // values that are not numbers, remembered by (key, block)
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLow = 2048.0f;  // ql and kl are 2^11 times what they stand for, so that they seldom are subnormal
@@ -91,6 +86,16 @@ struct Prompt {
     static constexpr unsigned kS = D, kQl = D + 128, kNeed = D + 128 + D / 2;
     static constexpr unsigned kCols = kNeed <= 256 ? 256 : 512;
     static_assert(kNeed <= 512 && kSmem <= 216 * 1024);
+    // Tensor memory's sums drop what is below their last bit, half of it on average, 12 times a step. So O moves on to FP32 sums by
+    // turns: in every step a thread adds kParts of its NB runs of 16 dims to them and clears the runs, while the tensor cores
+    // form S, and each run is moved every kTurns steps. The sums of kHeld runs are in registers (with more, others spill), those
+    // of the rest lie in y. Error of the result and us, 4 requests of 2048 on up to 2560 keys, 16 heads of 256 (of 128):
+    //   all of O to y every 32 steps, before the softmax   3.1 10^-6  307  (2.9 10^-6  221)
+    //   every 8                                            1.8        376  (1.5        246)
+    //   by turns                                           1.4        320  (1.2        227)
+    //   by turns, no run in registers                      1.4        328  (1.2        235)
+    // and FP32 arithmetic is off by 1.0 (0.8) 10^-6.
+    static constexpr unsigned kParts = (NB + 3) / 4, kTurns = (NB + kParts - 1) / kParts, kHeld = NB < 2 ? NB : 2;
 };
 
 __device__ __forceinline__ void work_sync() { asm volatile("barrier.cta.sync 1, %0;" ::"n"(kWork) : "memory"); }
@@ -253,7 +258,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnAr
                 for (unsigned k = 0; k < kKeys / 16; ++k) {
                     const uint64_t v = tm_operand(vh_at + k * (D * 32), D * 16, 128);
                     const uint32_t p = tm + S::kS + k / 2 * 32 + k % 2 * 8;
-                    tm_mma_t(tm, p, v, tm_f16(D, true), j % kFold || k);
+                    tm_mma_t(tm, p, v, tm_f16(D, true), j || k);
                     tm_mma_t(tm, p, tm_operand(vl_at + k * (D * 32), D * 16, 128), tm_f16(D, true), true);
                     tm_mma_t(tm, p + 16, v, tm_f16(D, true), true);
                 }
@@ -399,38 +404,99 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnAr
     if (!fail) unpack(0, false, kh, kl);
     hand_over(&bar_k);
     float top = -INFINITY, sum = 0.0f;
-    float y_factor = 0.0f;  // of what lies in y (0: nothing yet)
-    const bool wide_y = ((reinterpret_cast<uintptr_t>(a.y) | a.y_stride * 4) & 15) == 0;
-    // O and what lies in y, times f: of this thread's row, its half of the dims, 16 at a time
-    auto fold = [&](float f, unsigned nan_blocks, bool none) {
-        for (unsigned c = half_ * (D / 2); c < (half_ + 1) * (D / 2); c += 16) {
-            uint32_t o[16];
-            tm_load16(tm_lane + c, o);
-            if (!real) continue;
-            const bool bad_block = nan_blocks >> c / 32 & 1;
+    // The FP32 sums, and the maxima that each turn's were formed with (-inf: there is nothing in them yet)
+    float moved[S::kHeld][16], moved_top[S::kTurns];
+#pragma unroll
+    for (unsigned i = 0; i < S::kTurns; ++i) moved_top[i] = -INFINITY;
+#pragma unroll
+    for (unsigned i = 0; i < S::kHeld; ++i)
+#pragma unroll
+        for (unsigned e = 0; e < 16; ++e) moved[i][e] = 0.0f;
+    // y goes out and comes back by whole sectors of 32 bytes where it lies so (half a sector at a time takes twice as long)
+    const unsigned y_align = unsigned(reinterpret_cast<uintptr_t>(a.y) | a.y_stride * 4);
+    auto from_y = [&](unsigned c, float (&v)[16]) {
+        const float *at = y + c;
+        if (y_align % 32 == 0) {
+#pragma unroll
+            for (unsigned e = 0; e < 16; e += 8)
+                asm volatile("ld.global.L1::no_allocate.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                             : "=f"(v[e]), "=f"(v[e + 1]), "=f"(v[e + 2]), "=f"(v[e + 3]), "=f"(v[e + 4]), "=f"(v[e + 5]), "=f"(v[e + 6]), "=f"(v[e + 7])
+                             : "l"(at + e)
+                             : "memory");
+        } else if (y_align % 16 == 0) {
 #pragma unroll
             for (unsigned e = 0; e < 16; e += 4) {
-                float4 v = make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]), __uint_as_float(o[e + 2]), __uint_as_float(o[e + 3]));
-                float *to = y + c + e;
-                if (y_factor != 0.0f) {
-                    float4 was;
-                    if (wide_y) was = *reinterpret_cast<const float4 *>(to);
-                    else was = make_float4(to[0], to[1], to[2], to[3]);
-                    v.x += was.x * y_factor, v.y += was.y * y_factor, v.z += was.z * y_factor, v.w += was.w * y_factor;
-                }
-                v.x *= f, v.y *= f, v.z *= f, v.w *= f;
-                if (none) v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if (bad_block) v.x = v.y = v.z = v.w = __uint_as_float(0x7fc00000u);
-                if (wide_y) *reinterpret_cast<float4 *>(to) = v;
-                else to[0] = v.x, to[1] = v.y, to[2] = v.z, to[3] = v.w;
+                const float4 x = *reinterpret_cast<const float4 *>(at + e);
+                v[e] = x.x, v[e + 1] = x.y, v[e + 2] = x.z, v[e + 3] = x.w;
             }
+        } else {
+#pragma unroll
+            for (unsigned e = 0; e < 16; ++e) v[e] = at[e];
+        }
+    };
+    auto to_y = [&](unsigned c, const float (&v)[16]) {
+        float *at = y + c;
+        if (y_align % 32 == 0) {
+#pragma unroll
+            for (unsigned e = 0; e < 16; e += 8)
+                asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(at + e), "f"(v[e]), "f"(v[e + 1]), "f"(v[e + 2]),
+                             "f"(v[e + 3]), "f"(v[e + 4]), "f"(v[e + 5]), "f"(v[e + 6]), "f"(v[e + 7])
+                             : "memory");
+        } else if (y_align % 16 == 0) {
+#pragma unroll
+            for (unsigned e = 0; e < 16; e += 4) *reinterpret_cast<float4 *>(at + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+        } else {
+#pragma unroll
+            for (unsigned e = 0; e < 16; ++e) at[e] = v[e];
         }
     };
     unsigned j = 0;
     for (; j < steps; ++j) {
-        if (j && !fail) fail = !mbar_wait(&bar_o, (j - 1) & 1);  // V is free
+        if (j && !fail) fail = !mbar_wait(&bar_o, (j - 1) & 1);  // V is free, O is there
+        const bool move = j >= S::kTurns && !__any_sync(~0u, fail);
+        const unsigned turn = j % S::kTurns;
+        float last_top = -INFINITY, was[S::kParts][16];
+#pragma unroll
+        for (unsigned i = 0; i < S::kTurns; ++i) last_top = i == turn ? moved_top[i] : last_top;
+        const bool held = move && last_top != -INFINITY;
+        if (S::kHeld < NB) {
+#pragma unroll
+            for (unsigned i = 0; i < S::kParts; ++i) {
+                const unsigned run = turn * S::kParts + i;
+#pragma unroll
+                for (unsigned e = 0; e < 16; ++e) was[i][e] = 0.0f;
+                if (held && real && run >= S::kHeld && run < NB) from_y(half_ * (D / 2) + run * 16, was[i]);
+            }
+        }
         if (!fail) unpack(j, true, vh, vl);
         hand_over(&bar_v);
+        if (move) {
+            tm_fence_after();
+            const float f = held ? exp2_fast(last_top - top) : 0.0f;
+#pragma unroll
+            for (unsigned i = 0; i < S::kParts; ++i) {
+                const unsigned run = turn * S::kParts + i, c = half_ * (D / 2) + run * 16;
+                if (run >= NB) continue;
+                uint32_t o[16];
+                tm_load16(tm_lane + c, o);
+#pragma unroll
+                for (unsigned r = 0; r < S::kHeld; ++r) {
+                    if (r != run) continue;
+#pragma unroll
+                    for (unsigned e = 0; e < 16; ++e) moved[r][e] = fmaf(moved[r][e], f, __uint_as_float(o[e]));
+                }
+                if (run >= S::kHeld && real) {
+#pragma unroll
+                    for (unsigned e = 0; e < 16; ++e) was[i][e] = fmaf(was[i][e], f, __uint_as_float(o[e]));
+                    to_y(c, was[i]);
+                }
+#pragma unroll
+                for (unsigned e = 0; e < 16; ++e) o[e] = 0;
+                tm_store16(tm_lane + c, o);
+            }
+#pragma unroll
+            for (unsigned i = 0; i < S::kTurns; ++i) moved_top[i] = i == turn ? top : moved_top[i];
+        }
 
         // scores of the row and 32 keys, in powers of two
         if (!fail) fail = !mbar_wait(&bar_s, j & 1);
@@ -469,17 +535,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnAr
         row_top[half_][row] = mx;
         work_sync();
         mx = fmaxf(mx, row_top[half_ ^ 1][row]);
-        const bool fresh = j % kFold == 0;  // O begins again with this step
-        if (fresh && j) {
-            fold(1.0f, 0, false);
-            y_factor = 1.0f;
-        }
         if (__any_sync(~0u, mx > top)) {  // a higher maximum: 4 above the score, so that it moves seldom
             const float nt = mx > top ? mx + 4.0f : top, f = top == nt ? 1.0f : exp2_fast(top - nt);
             sum *= f;
-            y_factor *= f;
             top = nt;
-            if (!fresh) {
+            if (j) {
+                tm_wait_store();  // (of runs that were cleared)
                 for (unsigned c = half_ * (D / 2); c < (half_ + 1) * (D / 2); c += 16) {
                     uint32_t o[16];
                     tm_load16(tm_lane + c, o);
@@ -546,7 +607,30 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnAr
                     if (!(fabsf(__half2float(d[b])) <= 65504.0f)) nan_blocks |= 1u << b;
             }
         }
-        fold(f, nan_blocks, sum == 0.0f);
+        auto finish = [&](unsigned run, float (&v)[16], float back) {
+            const unsigned c = half_ * (D / 2) + run * 16;
+            uint32_t o[16];
+            tm_load16(tm_lane + c, o);
+            const bool bad_block = nan_blocks >> c / 32 & 1;
+#pragma unroll
+            for (unsigned e = 0; e < 16; ++e) {
+                v[e] = fmaf(v[e], back, __uint_as_float(o[e])) * f;
+                if (sum == 0.0f) v[e] = 0.0f;
+                if (bad_block) v[e] = __uint_as_float(0x7fc00000u);
+            }
+            if (real) to_y(c, v);
+        };
+#pragma unroll
+        for (unsigned run = 0; run < NB; ++run) {
+            const float was_top = moved_top[run / S::kParts], back = was_top != -INFINITY ? exp2_fast(was_top - top) : 0.0f;
+            if (run < S::kHeld) {
+                finish(run, moved[run < S::kHeld ? run : 0], back);
+            } else {
+                float v[16] = {};
+                if (real && was_top != -INFINITY) from_y(half_ * (D / 2) + run * 16, v);
+                finish(run, v, back);
+            }
+        }
     }
     }
     tm_fence_before();

@@ -1,6 +1,6 @@
 """Attention over the 4-bit cache where the 32-dim blocks of a token have scales far from one another, for single tokens and drafts
 (units of up to sixteen rows) and for prompts (the tensor-memory kernel): a block's dims are as good as if the others were
-not there, whatever lies in them."""
+not there, whatever lies in them. And sums over many keys, which tensor memory alone would make too small."""
 import math
 
 import numpy as np
@@ -154,3 +154,22 @@ def test_values_that_grow_from_token_to_token(b2, lengths):
 
     b = Blocks(b2, r, lengths, 2, 16, 128, 16, v=values)
     check(b, b.run())
+
+
+@pytest.mark.parametrize("dim", range(32, 257, 32))
+def test_prompts_over_many_keys_of_one_sign_do_not_come_out_small(b2, dim):
+    """Tensor memory's sums drop half of their last bit on average, at each of the 12 products of 16 keys in a step of 64: of values
+    of one sign all in one direction. A sum that moves on to FP32 every 4 steps is half of what it ends at on average, and its last
+    bit 0.72 2^-23 of it: 12 x 4 / 2 / 2 x 0.72 2^-23 = 1.03 10^-6 too small in the mean (first sums, of up to 7 steps of 40, a
+    little more), within 2^-19. Over 32 steps it would be 8 10^-6."""
+    r = rng(407, dim)
+    new, n, page = 64, 2560, 64
+    b = Blocks(b2, r, [(new, n)], 1, 96, dim, page, v=lambda n: (1 + 0.25 * r.normal(0, 1, (n, dim))).astype(np.float32))
+    got = b.run()
+    key = np.arange(n)
+    k, v = (b.p.ref.values(i, b.table[0][key // page], key % page)[:, 0] for i in (0, 1))
+    s = b.q.astype(np.float64) @ k.T * b.scale
+    s = np.where(key > n - new + np.arange(new)[:, None, None], -np.inf, s)
+    p = np.exp(s - s.max(-1, keepdims=True))
+    y = p @ v / p.sum(-1, keepdims=True)
+    assert abs((got / y - 1).mean()) < 2.0 ** -19
