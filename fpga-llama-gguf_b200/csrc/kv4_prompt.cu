@@ -400,7 +400,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnAr
         if (lane == 0) arrive(bar);
     };
 
-    fail = !mbar_wait(&bar_raw, 0);
+    // A wait that ran out, for the whole warp: its lanes stay together in what follows.
+    auto missed = [&](uint64_t *bar, unsigned phase) { return !__all_sync(~0u, mbar_wait(bar, phase & 1)); };
+    fail = missed(&bar_raw, 0);
     if (!fail) unpack(0, false, kh, kl);
     hand_over(&bar_k);
     float top = -INFINITY, sum = 0.0f;
@@ -452,8 +454,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnAr
     };
     unsigned j = 0;
     for (; j < steps; ++j) {
-        if (j && !fail) fail = !mbar_wait(&bar_o, (j - 1) & 1);  // V is free, O is there
-        const bool move = j >= S::kTurns && !__any_sync(~0u, fail);
+        if (j && !fail) fail = missed(&bar_o, j - 1);  // V is free, O is there
+        const bool move = j >= S::kTurns && !fail;
         const unsigned turn = j % S::kTurns;
         float last_top = -INFINITY, was[S::kParts][16];
 #pragma unroll
@@ -499,7 +501,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnAr
         }
 
         // scores of the row and 32 keys, in powers of two
-        if (!fail) fail = !mbar_wait(&bar_s, j & 1);
+        if (!fail) fail = missed(&bar_s, j);
         if ((fail = work_sync_or(fail))) break;  // (and all keys' scales are there)
         tm_fence_after();
         uint32_t s[32], s_low[32];
@@ -573,12 +575,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnAr
         tm_wait_store();
         hand_over(&bar_p);
         if (j + 1 < steps) {
-            fail = !mbar_wait(&bar_raw, (j + 1) & 1);
+            fail = missed(&bar_raw, j + 1);
             if (!fail) unpack(j + 1, false, kh, kl);
             hand_over(&bar_k);
         }
     }
-    if (!fail) fail = !mbar_wait(&bar_o, (steps - 1) & 1);
+    if (!fail) fail = missed(&bar_o, steps - 1);
     tm_fence_after();
     work_sync();  // (the last maxima are read)
     row_top[half_][row] = sum;
