@@ -61,11 +61,11 @@ __device__ __forceinline__ unsigned reached_by(unsigned mine, unsigned n, unsign
 // the threads' own best give a bound that n_out of them reach; what is above it in the segment's chunks, some dozens each, is
 // collected and ranked by counting at the end. Should more come together, the n_out best so far are taken out first and the
 // worst of them is the bound from then on; should ties put more there than can be held, they are taken out one by one.
-// 16 requests of 8 beams over 151,936 logits, 16 each: 26 us, and 7 for the lists' merge behind it (the bytes alone: 12). A
-// chunk takes a CTA 1.9 us (0.6 to issue the next one's copies, 0.2 maxima, 0.5 exponentials, 0.4 candidates and the barrier),
+// 16 requests of 8 beams over 151,936 logits, 16 each: 34 us with the lists' merge (the bytes alone: 12); by themselves and
+// with cold caches the kernels take 30 and 10 us. 128 rows in 3 segments are 384 of the 444 CTAs that run at once, of 7, 6 and 6
+// chunks. A chunk takes a CTA 1.9 us (0.6 to issue the next one's copies, 0.2 maxima, 0.5 exponentials, 0.4 candidates and the barrier),
 // at which three CTAs an SM ask for all of the memory's rate; the first one (2.5 with its bound) and the end (1.5) do not. With
-// a list a chunk instead, each ranked by itself and five CTAs an SM, the whole call took 40 us (35 now), with chunks of
-// 4096 57.
+// a list a chunk instead, each ranked by itself and five CTAs an SM, the whole call took 40 us, with chunks of 4096 57.
 constexpr unsigned kFound = 512, kSelCtas = 3;  // CTAs on an SM, by shared memory
 static_assert(kSelPer == 32 && kFound / 2 > kMaxBeamOut);
 template <bool kWide>  // rows on 16 bytes

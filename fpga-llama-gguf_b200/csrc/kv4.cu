@@ -151,8 +151,9 @@ __global__ void __launch_bounds__(256) map_rows_kernel(const BlockMapArgs a) {
 // rounded to FP32 by itself; a block that holds a NaN or an infinity gets a NaN scale, so that it reads back as NaN.
 // Both are bound by memory once there are rows enough: 8192 tokens of 8 heads of 128 stored and read back (145 MB) take 39 us,
 // 22 at the measured copy rate. What kept them from it was arithmetic (50 us): each thread's own divisions of the slot by the
-// page, the search for the largest value's sign, conversions at a quarter of the rate of additions. Two or eight rows a
-// turn took 43 and 45 us, a quarter of the CTAs 48.
+// page, the search for the largest value's sign, conversions at a quarter of the rate of additions. It still bounds them (72% and
+// 77% of issue slots): eight lanes a block do every block's division eight times and half of them write no code word, in the
+// load two lanes read each word. Two or eight rows a turn took 43 and 45 us, a quarter of the CTAs 48.
 //
 // A thread stays with its values of its block and goes down the rows, kRowsTurn at a time, so that what places them in a
 // row is worked out once and several rows' loads are on their way together.

@@ -32,9 +32,9 @@ constexpr unsigned kMaxRange = 1024;     // a warp adds at most 256 tiles into i
 // with 16, 74 with 24 (short requests pile up on a CTA with less, its long ones wait with more).
 constexpr unsigned kUnitCost = 16;
 // Requests with this many rows (token, head of a KV head's group) are the prompt kernel's when a call's rows and heads make
-// work enough for it. New tokens on 512 keys before them, 16 heads of 128 (of 256), us here / there: 128 tokens 32 / 46 (40 / 64),
-// 256 45 / 52 (68 / 71), 384 64 / 57 (101 / 79), 1024 204 / 87 (371 / 118); 32 requests of 16 tokens on 1000 keys, 32 heads
-// 104 / 100 (161 / 133), of 8 tokens (32 rows a request) 70 / 122 (98 / 164).
+// work enough for it. New tokens on 512 keys before them, 16 heads of 128 (of 256), us here / there: 128 tokens 32 / 47 (41 / 65),
+// 256 45 / 54 (69 / 74), 384 64 / 60 (103 / 82), 1024 202 / 92 (376 / 128); 32 requests of 17 tokens on 1000 keys, 32 heads
+// 185 / 128 (306 / 178), of 1 to 8 tokens (4 to 32 rows a request) 70 / 124 (100 / 167).
 constexpr unsigned kPromptRows = 64, kPromptWork = 6144;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -267,11 +267,11 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {  // an 8 x 8 matrix
 }
 
 // CTAs on an SM, by the accumulators a thread holds (8 for each of `blocks` = NB NT) and the registers they leave: 128, 168 or
-// 255 a thread. One query token of four heads on 131,000 keys, us a call with 2 / 3 / 4 CTAs: heads of 64 31.8 / 25.9 /
-// 24.9, of 128 35.9 / 32.3 / 33.4, of 256 47.7 / 48.9 / -.
+// 255 a thread. One query token of 16 heads (4 KV heads) on 131,000 keys, us a call with 2 / 3 / 4 CTAs: heads of 64 30.9 / 25.3 /
+// 25.1, of 128 36.4 / 31.5 / -, of 256 50.1 / 56.0 / -.
 constexpr unsigned ctas_of(unsigned blocks) { return blocks <= 2 ? 4 : blocks <= 4 ? 3 : 2; }
 // Sets of four rows that a unit may have, as far as their accumulators fit the registers. Twelve rows of heads of 128 in one
-// unit took 1430 cycles a tile, in two (of eight and four rows) 2200.
+// unit took 1410 cycles a tile, in two (of eight and four rows) 2200.
 constexpr unsigned most_sets(unsigned nb) { return nb <= 4 ? 4 : 16 / nb; }
 
 // NB: 32-dim blocks of a head; NT: sets of four query rows.
@@ -296,9 +296,11 @@ struct Shape {
 // tiles itself (one bulk copy each), so that nothing in the loop waits for another warp.
 //
 // Instructions and their latencies bound it: the registers leave two to four warps a quarter SM. A tile of 16 keys takes a
-// quarter 300 cycles at 4 rows of heads of 32, 680 at 128, 1190 at 256 (4.6 KB: 820 at the copy rate), 1380 at 12 rows of 128.
-// One row of 16 heads of 256 on 131,000 keys: 47.8 us, 3.2 TB/s; 12 us of it lie before and behind the loop (the wait for
-// the kernel before, 2 us of schedule, 2 until the first tile is there, 5 for the merge). Tried without gain: two tiles'
+// quarter 380 cycles at 4 rows of heads of 32, 710 at 128, 1290 at 256 (4.6 KB: 820 at the copy rate), 1410 at 12 rows of 128.
+// One row of 16 heads of 256 on 131,000 keys: 49 us, 3.1 TB/s; 12 us of it lie before and behind the loop (the wait for
+// the kernel before, 2 us of schedule, 2 until the first tile is there, 5 for the merge). A unit's rows follow the bound on new
+// tokens and not the request: 64 single tokens of 32 heads of 128 take 39 us where max_q is 1, 90 where it is 4 or more (of 256:
+// 65 and 92), since their units then have 16 (8) rows, 4 of them real. Tried without gain: two tiles'
 // products at a time, one tile's values beside the next one's scores, the next piece looked up before this one's tiles.
 template <int NB, int NT>
 __global__ void __launch_bounds__(kThreads, Shape<NB, NT>::kCtas) kv4_attn_kernel(const Kv4AttnArgs a, const AttnPlan plan) {

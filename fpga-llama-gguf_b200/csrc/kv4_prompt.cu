@@ -22,9 +22,10 @@
 //   unpack the next K    while the tensor cores add P V
 // A ninth warp issues the products (which holds it up while the tensor cores are busy) and the raw tiles' bulk copies.
 //
-// 4 requests of 2048 new tokens on up to 2560 keys, 16 heads of 256: 305 us, 208 TFLOP/s of the plain products, three times
-// that on the tensor cores, which are busy a third of the time. A step of 64 keys takes 6500 cycles: 2800 S, 1000 to 2000
-// the softmax, 2100 P V, one after another, since O, S and ql fill tensor memory at 256 dims.
+// 4 requests of 200 to 2048 new tokens on up to 2560 keys, 16 heads of 256: 320 us, 200 TFLOP/s of the plain products, three times
+// that on the tensor cores, which are busy a third of the time; of 128: 227 us, of 64: 196. Of a step of 64 keys at 256 dims S
+// takes 2800 cycles, the softmax 1000 to 2000, P V 2100, one after another: O, S and ql fill tensor memory. With smaller
+// heads they do not, and there it is the same order all the same.
 #include <cuda_runtime.h>
 
 #include "common.cuh"

@@ -94,6 +94,31 @@ def test_the_4bit_decoders_lists_plan(page):
         m.token_graph()
 
 
+@pytest.mark.parametrize("world", [2, 4, 8])
+def test_the_4bit_decoders_lists_plan_for_every_rank(world):
+    for rank in range(world):
+        m = D.HybridDecoder(D.SHAPE_4B, kv4_page=64, world=world, rank=rank)
+        m.handles = {name: (k + 1) * 256 for k, (name, *_) in enumerate(m.matrices())}
+        for cl in m.token_lists():
+            assert b2.plan(cl)[0] == 0
+        assert m.context_config()["kv_bytes"] == m.kv_bytes() == m.kv4_pool(m.s.n_attn)[0]
+
+
+def test_a_ranks_pages_hold_its_heads_of_the_whole_cache():
+    page, s = 16, SMALL
+    whole = D.HybridDecoder(s, seed=9, kv4_page=page)
+    raw = whole.initial_kv()
+    for rank in range(2):
+        m = D.HybridDecoder(s, seed=9, kv4_page=page, world=2, rank=rank)
+        mine = m.initial_kv()
+        for j in range(s.n_attn):
+            (at, n_pages), (at1, n1) = whole.kv4_pool(j), m.kv4_pool(j)
+            assert n_pages == n1
+            size = n_pages * b2.kv4_page_bytes(page, s.n_kv_head, s.head_dim)
+            heads = raw[at:at + size].reshape(n_pages, s.n_kv_head, -1)
+            assert np.array_equal(mine[at1:at1 + size // 2].reshape(n1, 1, -1), heads[:, rank:rank + 1])
+
+
 @pytest.mark.gpu
 def test_commands_give_the_direct_calls_bits():
     torch = pytest.importorskip("torch")
