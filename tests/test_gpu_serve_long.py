@@ -1,5 +1,6 @@
-"""Prompts over caches of many steps of 64 keys, whose outputs move from tensor memory to FP32 sums on the way: rows of y on 32, 16 and 4 bytes, maxima that rise and fall along the keys, windows, rows that see their first key late or never,
-pages that are none. Tolerances: those of test_gpu_serve_blocks.check."""
+"""Prompts over caches of many steps of 64 keys, whose outputs move from tensor memory to FP32 sums on the way: rows of y on 32, 16
+and 4 bytes, maxima that rise and fall along the keys, windows, rows that see their first key late or never, pages that are
+none. Tolerances: those of test_gpu_serve_blocks.check."""
 import numpy as np
 import pytest
 
